@@ -128,6 +128,58 @@ int llsa_rms_rope_bwd(int n_tensors, const LlsaTensor* dy, const LlsaTensor* x, 
                       float eps, const LlsaTensor* freq, const LlsaTensor* dx, const LlsaTensor* dw_partial,
                       const LlsaTensor* const* dw, void* stream);
 
+/* Rotation by positions on several axes (models/rope_dit_transformer_2d.py:71-109), without a table: the D channels of x [B,H,N,D] are cut into
+ * one part of axes_dims[a] channels per axis (positive, even, D together, at most 512; 1 to 4 axes); pair i of axis a turns by
+ * positions[n,a] * theta^(-2i/axes_dims[a]), the angle taken in 64 bits.  positions: [N,A], or [B,N,A] for samples with positions of their own; I32, I64
+ * or F32.  y has x's shape, any strides; inverse != 0 rotates back, which is the backward pass.  Rows on 16-byte boundaries are the fast form; any
+ * alignment is accepted. */
+int llsa_rope_axes(const LlsaTensor* x, const LlsaTensor* positions, int n_axes, const int32_t* axes_dims, double theta, int inverse,
+                   const LlsaTensor* y, void* stream);
+
+/* ---- layer norm with modulation (models/rope_dit_transformer_2d.py:295-337, :600-640) ----
+ * y = (h * weight + bias) * (1 + scale) + shift,  h = (x - mean) / sqrt(var + eps) over the C channels of x [B,N,C] (any batch and token strides, 1 to
+ * 16384 channels, fewer than 2^31 rows).  weight, bias [C] and scale, shift [B,C] (any row stride) are F32 or of x's type; each may be NULL.
+ * stats: F32 [B,N,2], written with (mean, 1/sqrt(var + eps)) of every row for the backward; may be NULL.  Sums are fp32; y is rounded once. */
+int llsa_layer_norm_fwd(const LlsaTensor* x, const LlsaTensor* weight, const LlsaTensor* bias, const LlsaTensor* scale, const LlsaTensor* shift,
+                        float eps, const LlsaTensor* y, const LlsaTensor* stats, void* stream);
+/* Backward: dx (x's shape, any strides) and those of dweight, dbias [C], dscale, dshift [B,C] that are not NULL (contiguous, F32 or x's type).
+ * weight, bias, scale, stats as in the forward.  partial: 1-D F32 scratch of llsa_layer_norm_bwd_partial_elems() elements, wanted where a parameter's
+ * gradient is; per_sample = scale or dshift is given.  Where neither is, the samples of dy, x and dx must follow one another
+ * (stride[0] == N * stride[1]).  Sums are added in a fixed order. */
+int64_t llsa_layer_norm_bwd_partial_elems(int64_t B, int64_t N, int64_t C, int per_sample);
+int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, const LlsaTensor* weight, const LlsaTensor* bias, const LlsaTensor* scale,
+                        const LlsaTensor* stats, const LlsaTensor* dx, const LlsaTensor* dweight, const LlsaTensor* dbias,
+                        const LlsaTensor* dscale, const LlsaTensor* dshift, const LlsaTensor* partial, void* stream);
+
+/* ---- projection with its epilogue (models/rope_dit_transformer_2d.py:205-213, :254-258, :640-711) ----
+ * y = residual + gate_b * act(x weight^T + bias); bf16 or F32 throughout, sums fp32, y rounded once.  Zero-initialise the struct. */
+enum LlsaActivation { LLSA_ACT_NONE = 0, LLSA_ACT_GELU_TANH = 1, LLSA_ACT_SILU = 2 };
+typedef struct LlsaLinearArgs {
+  const LlsaTensor* x;         /* [M,K], fewer than 2^31 rows; bf16: rows on 16-byte boundaries */
+  const LlsaTensor* weight;    /* [F,K], likewise */
+  const LlsaTensor* bias;      /* [F] contiguous, or NULL */
+  const LlsaTensor* residual;  /* [M,F], any row stride, or NULL */
+  const LlsaTensor* gate;      /* [B,F], any row stride, or NULL: row b stands for rows [b M/B, (b+1) M/B); with a residual and no activation */
+  const LlsaTensor* y;         /* [M,F] out, any row stride */
+  const LlsaTensor* pre;       /* [M,F] of x's type, contiguous: written by the forward if given, read by the backward of an activation or for dgate.
+                                  Not for other use: behind an activation of bf16 data it holds half-precision floats */
+  int32_t activation;          /* LlsaActivation */
+  /* backward: dy in, those of the others that are not NULL out */
+  const LlsaTensor* dy;        /* [M,F], any row stride */
+  const LlsaTensor* dx;        /* [M,K], any row stride */
+  const LlsaTensor* dweight;   /* [F,K] contiguous, x's type */
+  const LlsaTensor* dbias;     /* [F] contiguous, F32 or x's type */
+  const LlsaTensor* dgate;     /* [B,F] contiguous, F32 or x's type */
+  void* workspace;             /* backward: llsa_linear_bwd_workspace_bytes() bytes on a 256-byte boundary, not read before they are written */
+  int64_t workspace_bytes;
+  int32_t wait_limit;          /* as in LlsaAttnArgs */
+  int32_t* status;
+} LlsaLinearArgs;
+int llsa_linear_fwd(const LlsaLinearArgs* args, void* stream);
+/* Read from the shapes of x, weight and gate, the activation and which results are wanted; -1 where these are refused */
+int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* args);
+int llsa_linear_bwd(const LlsaLinearArgs* args, void* stream);
+
 /* ---- selection: src/llsa/kernel/triton/topk.py ----------------------------
  * Coarse: idx[b,h,i,:] = top-`topk` columns of round_dtype(pq[b,h,i,:] . pk[b,h,:,:]^T),
  * descending, ties -> smallest index.  idx is I32 or I64 [B,H,M,topk].  Replaces

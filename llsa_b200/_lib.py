@@ -40,6 +40,15 @@ class LlsaAttnArgs(C.Structure):
     ]
 
 
+class LlsaLinearArgs(C.Structure):
+    _P = C.POINTER(LlsaTensor)
+    _fields_ = [
+        ("x", _P), ("weight", _P), ("bias", _P), ("residual", _P), ("gate", _P), ("y", _P), ("pre", _P), ("activation", C.c_int32),
+        ("dy", _P), ("dx", _P), ("dweight", _P), ("dbias", _P), ("dgate", _P), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("wait_limit", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
 EXPORTS = [
     "llsa_version", "llsa_last_error_string", "llsa_mean_pool_fwd", "llsa_mean_pool_bwd", "llsa_pool_pyramid_fwd",
     "llsa_pool_pyramid_beside_fwd",
@@ -48,6 +57,8 @@ EXPORTS = [
     "llsa_rope_fwd", "llsa_rope_bwd", "llsa_coarse_topk", "llsa_coarse_topk_bounded", "llsa_refine_topk", "llsa_select_two_level", "llsa_transpose_scratch_bytes",
     "llsa_transpose_indices", "llsa_transpose_indices_pairs", "llsa_transpose_range_entries", "llsa_transpose_indices_noalloc", "llsa_attn_fwd", "llsa_attn_bwd",
     "llsa_attn_bwd_partial_elems", "llsa_attn_bwd_pds_elems", "llsa_attn_remainder_elems", "llsa_attn_fwd_redo_elems", "llsa_status_check",
+    "llsa_rope_axes", "llsa_layer_norm_fwd", "llsa_layer_norm_bwd", "llsa_layer_norm_bwd_partial_elems",
+    "llsa_linear_fwd", "llsa_linear_bwd", "llsa_linear_bwd_workspace_bytes",
 ]
 
 _lib: Optional[C.CDLL] = None
@@ -91,10 +102,20 @@ def _declare(lib: C.CDLL) -> None:
     lib.llsa_status_check.argtypes = [C.c_int32]
     lib.llsa_attn_fwd.argtypes = [C.POINTER(LlsaAttnArgs), C.c_void_p]
     lib.llsa_attn_bwd.argtypes = [C.POINTER(LlsaAttnArgs), C.c_void_p]
+    lib.llsa_rope_axes.argtypes = [TP, TP, C.c_int, C.POINTER(C.c_int32), C.c_double, C.c_int, TP, C.c_void_p]
+    lib.llsa_layer_norm_fwd.argtypes = [TP] * 5 + [C.c_float, TP, TP, C.c_void_p]
+    lib.llsa_layer_norm_bwd_partial_elems.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int]
+    lib.llsa_layer_norm_bwd_partial_elems.restype = C.c_int64
+    lib.llsa_layer_norm_bwd.argtypes = [TP] * 12 + [C.c_void_p]
+    lib.llsa_linear_fwd.argtypes = [C.POINTER(LlsaLinearArgs), C.c_void_p]
+    lib.llsa_linear_bwd.argtypes = [C.POINTER(LlsaLinearArgs), C.c_void_p]
+    lib.llsa_linear_bwd_workspace_bytes.argtypes = [C.POINTER(LlsaLinearArgs)]
+    lib.llsa_linear_bwd_workspace_bytes.restype = C.c_int64
     for name in EXPORTS:
         fn = getattr(lib, name)
         if name not in ("llsa_last_error_string", "llsa_transpose_scratch_bytes", "llsa_attn_bwd_partial_elems", "llsa_attn_bwd_pds_elems",
-                        "llsa_rms_rope_bwd_partial_elems", "llsa_attn_remainder_elems", "llsa_attn_fwd_redo_elems"):
+                        "llsa_rms_rope_bwd_partial_elems", "llsa_attn_remainder_elems", "llsa_attn_fwd_redo_elems",
+                        "llsa_layer_norm_bwd_partial_elems", "llsa_linear_bwd_workspace_bytes"):
             fn.restype = C.c_int
 
 

@@ -4,7 +4,7 @@
 
 libllsa_b200.so is a plain C-ABI library (include/llsa_b200.h): it links against
 the CUDA runtime only, not against torch or Python.  _host.so is the operators'
-host path over it (csrc/host.cpp): dispatcher operators with C++ autograd,
+host path over it (csrc/host.cpp, csrc/host_block.cpp): dispatcher operators with C++ autograd,
 linked against torch.
 """
 from __future__ import annotations
@@ -18,7 +18,9 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libllsa_b200.so")
 HOST = os.path.join(PKG, "_host.so")
 SOURCES = ["capi.cu", "pool.cu", "rope.cu", "front_bwd.cu", "topk.cu", "topk_tc.cu", "transpose.cu", "attn.cu", "attn_generic.cu",
-           "attn_fwd_mma.cu", "attn_bwd_mma.cu", "attn_pooled_tc.cu", "attn_pooled_bwd_tc.cu", "attn_pooled_loop_tc.cu", "attn_pooled_bwd_loop_tc.cu", "attn_pooled_dkv_loop_tc.cu"]
+           "attn_fwd_mma.cu", "attn_bwd_mma.cu", "attn_pooled_tc.cu", "attn_pooled_bwd_tc.cu", "attn_pooled_loop_tc.cu", "attn_pooled_bwd_loop_tc.cu", "attn_pooled_dkv_loop_tc.cu",
+           "column_sums.cu", "layer_norm.cu", "linear.cu", "rope_axes.cu"]
+HOST_SOURCES = ["host.cpp", "host_block.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O3", "-lineinfo",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
@@ -30,8 +32,8 @@ def _nvcc() -> str:
     return "nvcc"
 
 
-def _host_cmd(obj: str):
-    """Compile command of the torch-side host path."""
+def _host_cmd(src: str, obj: str):
+    """Compile command of a file of the torch-side host path."""
     import sysconfig
 
     import torch
@@ -39,14 +41,14 @@ def _host_cmd(obj: str):
     inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     return ["g++", "-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi, "-DTORCH_API_INCLUDE_EXTENSION_H",
-            *["-isystem%s" % i for i in inc], "-c", os.path.join(CSRC, "host.cpp"), "-o", obj]
+            *["-isystem%s" % i for i in inc], "-c", os.path.join(CSRC, src), "-o", obj]
 
 
-def _host_link_cmd(obj: str):
+def _host_link_cmd(objs):
     import torch
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "lib64")
-    return ["g++", "-shared", "-o", HOST, obj, "-L" + PKG, "-lllsa_b200", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch", "-ltorch_cpu", "-lc10",
+    return ["g++", "-shared", "-o", HOST, *objs, "-L" + PKG, "-lllsa_b200", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch", "-ltorch_cpu", "-lc10",
             "-ltorch_cuda", "-lc10_cuda", "-L" + cuda, "-lcudart"]
 
 
@@ -72,8 +74,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
         cmd = [_nvcc(), *NVCC_FLAGS, "-c", sp, "-o", obj] + (["-Xptxas", "-v"] if verbose else [])
         procs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
-    host_obj = os.path.join(objdir, "host.o")
-    host = subprocess.Popen(_host_cmd(host_obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    hosts = []
+    for src in HOST_SOURCES:
+        obj = os.path.join(objdir, src.replace(".cpp", ".o"))
+        hosts.append((src, obj, subprocess.Popen(_host_cmd(src, obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     objs = []
     for src, obj, p in procs:
         out, _ = p.communicate()
@@ -86,10 +90,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stdout)
-    out, _ = host.communicate()
-    if host.returncode != 0:
-        raise RuntimeError("g++ failed on host.cpp:\n%s" % out)
-    r = subprocess.run(_host_link_cmd(host_obj), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    for src, obj, p in hosts:
+        out, _ = p.communicate()
+        if p.returncode != 0:
+            raise RuntimeError("g++ failed on %s:\n%s" % (src, out))
+    r = subprocess.run(_host_link_cmd([obj for _, obj, _ in hosts]), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         raise RuntimeError("link of the host path failed:\n" + r.stdout)
     return LIB

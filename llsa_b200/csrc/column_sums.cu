@@ -1,0 +1,92 @@
+// Parameter gradients from column sums per sample (column_sums.cuh).
+#include "column_sums.cuh"
+
+namespace llsa {
+
+namespace {
+
+constexpr int kCols = 32, kLanes = 32;
+
+// blockIdx.y: 32 columns; blockIdx.x: a sample, or (the last one, with `overall`) all of them.  Thread (column, lane) adds every 32nd part;
+// the lanes are added in order through shared memory.
+__global__ void __launch_bounds__(kCols * kLanes)
+column_grads_kernel(const float* __restrict__ partial, int64_t B, int64_t chunks, int C, ParamView w, ParamView bias, ParamView s, ColumnGrads g,
+                    int overall) {
+  __shared__ float s_sum[2][kLanes][kCols + 1];
+  const int col = threadIdx.x % kCols, lane = threadIdx.x / kCols, c = blockIdx.y * kCols + col;
+  const bool all = overall && blockIdx.x == gridDim.x - 1;
+  const int64_t b = blockIdx.x, n = all ? B * chunks : chunks;
+  const float* p = partial + (all ? 0 : b * chunks * 2 * C) + c;
+  float u = 0.f, v = 0.f;
+  pdl_wait();
+  pdl_trigger();
+  if (c < C) {
+#pragma unroll 4
+    for (int64_t i = lane; i < n; i += kLanes) {
+      const float f = all && s.p ? 1.f + s.at((uint32_t) (i / chunks), c, 0.f) : 1.f;
+      u = fmaf(f, p[i * 2 * C], u);
+      v = fmaf(f, p[i * 2 * C + C], v);
+    }
+  }
+  s_sum[0][lane][col] = u;
+  s_sum[1][lane][col] = v;
+  __syncthreads();
+  if (lane >= 2 || c >= C) return;
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < kLanes; ++k) {
+    sum[0] += s_sum[0][k][col];
+    sum[1] += s_sum[1][k][col];
+  }
+  if (all) {
+    if (lane == 0 && g.weight.p) g.weight.put(c, sum[0]);
+    if (lane == 1 && g.bias.p) g.bias.put(c, sum[1]);
+  } else {
+    if (lane == 0 && g.scale.p) g.scale.put(b * C + c, fmaf(w.at(0, c, 1.f), sum[0], bias.at(0, c, 0.f) * sum[1]));
+    if (lane == 1 && g.shift.p) g.shift.put(b * C + c, sum[1]);
+  }
+}
+
+}  // namespace
+
+int make_param(ParamView* v, const LlsaTensor* t, const char* name, int dtype, int64_t B, int64_t C) {
+  v->p = nullptr;
+  v->ld = 0;
+  v->is_bf16 = 0;
+  if (!t) return LLSA_OK;
+  LLSA_REQUIRE(t->ptr, LLSA_ERR_NULL, "%s: null tensor", name);
+  LLSA_REQUIRE(t->dtype == LLSA_F32 || t->dtype == dtype, LLSA_ERR_DTYPE, "%s: must be f32 or of the data's type", name);
+  if (B) LLSA_REQUIRE(t->ndim == 2 && t->shape[0] == B && t->shape[1] == C, LLSA_ERR_SHAPE, "%s: must be [%lld,%lld]", name, (long long) B, (long long) C);
+  else LLSA_REQUIRE(t->ndim == 1 && t->shape[0] == C, LLSA_ERR_SHAPE, "%s: must be [%lld]", name, (long long) C);
+  LLSA_REQUIRE(C == 1 || t->stride[t->ndim - 1] == 1, LLSA_ERR_STRIDE, "%s: innermost stride must be 1", name);
+  v->p = t->ptr;
+  v->ld = B ? t->stride[0] : 0;
+  v->is_bf16 = t->dtype == LLSA_BF16;
+  return LLSA_OK;
+}
+
+int check_grad(const LlsaTensor* t, const char* name, int dtype, int ndim, const int64_t* shape) {
+  LLSA_REQUIRE(t->ptr, LLSA_ERR_NULL, "%s: null tensor", name);
+  LLSA_REQUIRE(t->dtype == LLSA_F32 || t->dtype == dtype, LLSA_ERR_DTYPE, "%s: must be f32 or of the data's type", name);
+  return check_contig(t, name, t->dtype, ndim, shape);
+}
+
+int finish_column_grads(const float* partial, int64_t B, int64_t chunks, int64_t C, const ParamView& w, const ParamView& bias, const ParamView& s,
+                        const ColumnGrads& g, cudaStream_t st) {
+  const int per_sample = g.scale.p || g.shift.p, overall = g.weight.p || g.bias.p;
+  const int64_t slots = (per_sample ? B : 0) + overall;
+  if (slots == 0) return LLSA_OK;
+  launch_pdl(column_grads_kernel, dim3((unsigned) slots, (unsigned) ((C + kCols - 1) / kCols)), dim3(kCols * kLanes), 0, st, partial, B, chunks, (int) C, w,
+             bias, s, g, overall);
+  LLSA_LAUNCH_OK("column_grads_kernel");
+  return LLSA_OK;
+}
+
+int clear_column_grads(const ColumnGrads& g, int64_t B, int64_t C, cudaStream_t st) {
+  const GradView* const v[4] = {&g.scale, &g.shift, &g.weight, &g.bias};
+  for (int i = 0; i < 4; ++i)
+    if (v[i]->p && (i >= 2 || B)) LLSA_CUDA_OK(cudaMemsetAsync(v[i]->p, 0, (size_t) ((i < 2 ? B : 1) * C * (v[i]->is_bf16 ? 2 : 4)), st));
+  return LLSA_OK;
+}
+
+}  // namespace llsa

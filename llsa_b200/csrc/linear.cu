@@ -1,0 +1,386 @@
+// A projection with its epilogue, forward and backward: y = residual + gate_b act(x w^T + bias)
+// (models/rope_dit_transformer_2d.py:205-213, :254-258, :640-711: to_q / to_k / to_v, to_out and the feed-forward with adaLN-zero's gates).
+//
+//   z = x w^T + bias,  dz = dy gate_b act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum dz,  dgate_b = sum_n dy z,  dresidual = dy
+//
+// This file: checks, the choice of kernels, and the passes around the products (dz and its column sums, the sum of a split product's parts).
+#include <string.h>
+
+#include "linear.cuh"
+
+namespace llsa {
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+// ------------------------------------------------------------------------------------------------ scalar products
+// fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of 256 threads owns a tile of
+// 16 TM x 16 TM outputs, a thread TM x TM of them (two groups of TM / 2 rows and columns, so that a warp's reads of shared memory are whole
+// vectors); steps of 16 along k, the next step's operands on their way in registers while this one's are multiplied.
+template <typename T>
+__device__ __forceinline__ void fetch(const Mat<const T>& m, int along_k, int64_t row0, int64_t rows, int64_t k0, int64_t k1, int r, int k, float& v) {
+  const int64_t i = row0 + r, kk = k0 + k;
+  v = i < rows && kk < k1 ? to_f32<T>(along_k ? m.p[i * m.ld + kk] : m.p[kk * m.ld + i]) : 0.f;
+}
+
+template <typename T, int TM, bool PARTIAL>
+__global__ void __launch_bounds__(256)
+product_kernel(Product<T> p, Epilogue<T> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split) {
+  constexpr int BM = 16 * TM, BK = 16, LD = BM + 4, NV = BM * BK / 256;
+  __shared__ float s_a[2][BK][LD], s_b[2][BK][LD];
+  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+  const int64_t i0 = blockIdx.x / tiles_n * BM, j0 = blockIdx.x % tiles_n * BM;
+  const int64_t k_first = blockIdx.y * per_split, k_end = PARTIAL ? min(p.K, k_first + per_split) : p.K;
+  float acc[TM][TM], ra[NV], rb[NV];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = 0.f;
+  pdl_wait();
+  pdl_trigger();
+  auto load = [&](int64_t k0) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int q = v * 256 + tid;
+      fetch(p.a, p.a_k, i0, p.M, k0, k_end, p.a_k ? q / BK : q % BM, p.a_k ? q % BK : q / BM, ra[v]);
+      fetch(p.b, p.b_k, j0, p.N, k0, k_end, p.b_k ? q / BK : q % BM, p.b_k ? q % BK : q / BM, rb[v]);
+    }
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int q = v * 256 + tid;
+      s_a[buf][p.a_k ? q % BK : q / BM][p.a_k ? q / BK : q % BM] = ra[v];
+      s_b[buf][p.b_k ? q % BK : q / BM][p.b_k ? q / BK : q % BM] = rb[v];
+    }
+  };
+  load(k_first);
+  put(0);
+  __syncthreads();
+  int buf = 0;
+  for (int64_t k0 = k_first; k0 < k_end; k0 += BK) {
+    const bool more = k0 + BK < k_end;
+    if (more) load(k0 + BK);
+#pragma unroll
+    for (int k = 0; k < BK; ++k) {
+      float a[TM], b[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        a[i] = s_a[buf][k][(i / (TM / 2)) * (BM / 2) + ty * (TM / 2) + i % (TM / 2)];
+        b[i] = s_b[buf][k][(i / (TM / 2)) * (BM / 2) + tx * (TM / 2) + i % (TM / 2)];
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+    }
+    if (more) {
+      put(buf ^ 1);
+      __syncthreads();
+      buf ^= 1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const int64_t r = i0 + (i / (TM / 2)) * (BM / 2) + ty * (TM / 2) + i % (TM / 2);
+    if (r >= p.M) continue;
+    const int64_t sample = !PARTIAL && e.gate.p ? (uint32_t) r / e.rows_per_gate : 0;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int64_t c = j0 + (j / (TM / 2)) * (BM / 2) + tx * (TM / 2) + j % (TM / 2);
+      if (c >= p.N) continue;
+      if constexpr (PARTIAL) {
+        partial[(blockIdx.y * p.M + r) * partial_ld + c] = acc[i][j];
+      } else {
+        float z = acc[i][j] + (e.bias ? to_f32<T>(e.bias[c]) : 0.f);
+        if (e.pre.p) {
+          if (sizeof(T) == 2 && e.act != kActNone) reinterpret_cast<uint16_t*>(e.pre.p)[r * e.pre.ld + c] = half_bits(z);
+          else e.pre.p[r * e.pre.ld + c] = from_f32<T>(z);
+        }
+        z = activate<sizeof(T) == 2>(z, e.act);
+        if (e.gate.p) z *= to_f32<T>(e.gate.p[sample * e.gate.ld + c]);
+        if (e.residual.p) z += to_f32<T>(e.residual.p[r * e.residual.ld + c]);
+        e.y.p[r * e.y.ld + c] = from_f32<T>(z);
+      }
+    }
+  }
+}
+
+template <typename T, bool PARTIAL>
+int launch_product(const Product<T>& p, const Epilogue<T>& e, float* partial, int64_t ld, cudaStream_t st) {
+  const int64_t split = PARTIAL ? p.split : 1;
+  auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
+  const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
+  auto go = [&](auto kernel, int64_t b) {
+    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(256), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per);
+  };
+  LLSA_REQUIRE(tiles(32) <= INT32_MAX, LLSA_ERR_SHAPE, "linear: too many outputs");
+  if (tiles(128) * split >= 148) go(product_kernel<T, 8, PARTIAL>, 128);
+  else if (tiles(64) * split >= 148) go(product_kernel<T, 4, PARTIAL>, 64);
+  else go(product_kernel<T, 2, PARTIAL>, 32);
+  LLSA_LAUNCH_OK("product_kernel");
+  return LLSA_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ dz and its column sums
+// dz = dy gate act'(z) and, per column and part of a sample's rows, P = sum dy z and S = sum dz (column_sums.cuh).  A thread owns a column of 32 rows apart..
+template <typename T>
+struct FrontArgs {
+  Mat<const T> dy, pre, gate;
+  Mat<T> dz;                   // p NULL: not written
+  float* partial;              // NULL: no sums
+  uint32_t N, chunks, per;     // rows of a sample, CTAs along them, rows of a CTA
+  int F, act;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_dz_kernel(FrontArgs<T> a) {
+  __shared__ float s_sum[2][8][33];
+  const int col = threadIdx.x % 32, lane = threadIdx.x / 32, c = blockIdx.y * 32 + col;
+  const uint32_t b = blockIdx.x / a.chunks, first = (blockIdx.x - b * a.chunks) * a.per, end = min(a.N, first + a.per);
+  pdl_wait();
+  pdl_trigger();
+  float p = 0.f, s = 0.f;
+  if (c < a.F) {
+    const float gate = a.gate.p ? to_f32<T>(a.gate.p[b * a.gate.ld + c]) : 1.f;
+    for (uint32_t n = first + lane; n < end; n += 8) {
+      const int64_t r = (int64_t) b * a.N + n;
+      const float dy = to_f32<T>(a.dy.p[r * a.dy.ld + c]);
+      float dz = dy * gate;
+      if (a.pre.p) {
+        const T raw = a.pre.p[r * a.pre.ld + c];
+        const float z = sizeof(T) == 2 && a.act != kActNone ? half_value(*reinterpret_cast<const uint16_t*>(&raw)) : to_f32<T>(raw);
+        p = fmaf(dy, z, p);
+        dz *= activate_grad<sizeof(T) == 2>(z, a.act);
+      }
+      s += dz;
+      if (a.dz.p) a.dz.p[r * a.dz.ld + c] = from_f32<T>(dz);
+    }
+  }
+  if (!a.partial) return;
+  s_sum[0][lane][col] = p;
+  s_sum[1][lane][col] = s;
+  __syncthreads();
+  if (lane < 2 && c < a.F) {
+    float u = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u += s_sum[lane][k][col];
+    a.partial[((int64_t) blockIdx.x * 2 + lane) * a.F + c] = u;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ parts of a split product
+template <typename T>
+__global__ void __launch_bounds__(256)
+sum_parts_kernel(const float* __restrict__ partial, int64_t ld, int split, int64_t rows, int64_t cols, T* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t i = blockIdx.x * (int64_t) blockDim.x + threadIdx.x; i < rows * cols; i += (int64_t) gridDim.x * blockDim.x) {
+    const int64_t r = i / cols, c = i - r * cols;
+    float u = 0.f;
+    for (int s = 0; s < split; ++s) u += partial[(s * rows + r) * ld + c];
+    out[i] = from_f32<T>(u);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ checks and plan
+// A matrix with unit column stride
+int check_matrix(const LlsaTensor* t, const char* name, int dtype, int64_t rows, int64_t cols) {
+  LLSA_REQUIRE(t && t->ptr, LLSA_ERR_NULL, "%s: null tensor", name);
+  LLSA_REQUIRE(t->dtype == dtype, LLSA_ERR_DTYPE, "%s: dtype %d, expected %d", name, t->dtype, dtype);
+  LLSA_REQUIRE(t->ndim == 2 && t->shape[0] == rows && t->shape[1] == cols, LLSA_ERR_SHAPE, "%s: must be [%lld,%lld]", name, (long long) rows, (long long) cols);
+  LLSA_REQUIRE(cols == 1 || t->stride[1] == 1, LLSA_ERR_STRIDE, "%s: innermost stride %lld, must be 1", name, (long long) t->stride[1]);
+  return LLSA_OK;
+}
+
+struct Plan {
+  int64_t M, K, F, B, N;       // rows, input and output features, samples (1 without a gate), rows of a sample
+  int dtype;
+  bool write_dz, sums;         // the pass over dy: leaves dz / column sums
+  int64_t dz_ld, chunks, per;
+  int split;
+  int64_t part_ld;
+  size_t o_dz, o_cols, o_parts, bytes;
+};
+
+int check_common(const LlsaLinearArgs* a, Plan* p) {
+  LLSA_REQUIRE(a && a->x && a->x->ptr && a->weight && a->weight->ptr, LLSA_ERR_NULL, "linear: null argument");
+  LLSA_REQUIRE(is_float_dtype(a->x->dtype), LLSA_ERR_DTYPE, "x: must be f32 or bf16");
+  LLSA_REQUIRE(a->x->ndim == 2 && a->weight->ndim == 2, LLSA_ERR_SHAPE, "linear: x must be [M,K] and weight [F,K]");
+  p->dtype = a->x->dtype;
+  p->M = a->x->shape[0];
+  p->K = a->x->shape[1];
+  p->F = a->weight->shape[0];
+  LLSA_REQUIRE(p->K >= 1 && p->F >= 1 && p->K <= (1 << 20) && p->F <= (1 << 20), LLSA_ERR_SHAPE, "linear: 1 to 2^20 features are supported");
+  LLSA_REQUIRE(p->M <= INT32_MAX, LLSA_ERR_SHAPE, "linear: more than 2^31 - 1 rows");
+  int rc;
+  if ((rc = check_matrix(a->x, "x", p->dtype, p->M, p->K)) || (rc = check_matrix(a->weight, "weight", p->dtype, p->F, p->K))) return rc;
+  LLSA_REQUIRE(a->activation >= kActNone && a->activation <= kActSilu, LLSA_ERR_ARG, "linear: activation %d is not known", a->activation);
+  p->B = 1;
+  if (a->gate) {
+    LLSA_REQUIRE(a->gate->ptr, LLSA_ERR_NULL, "gate: null tensor");
+    LLSA_REQUIRE(a->activation == kActNone, LLSA_ERR_ARG, "linear: a gate goes with no activation");
+    LLSA_REQUIRE(a->gate->ndim == 2 && (p->M == 0 || (a->gate->shape[0] >= 1 && p->M % a->gate->shape[0] == 0)), LLSA_ERR_SHAPE,
+                 "gate: must be [B,F], B a divisor of the rows of x");
+    if ((rc = check_matrix(a->gate, "gate", p->dtype, a->gate->shape[0], p->F))) return rc;
+    p->B = std::max<int64_t>(1, a->gate->shape[0]);
+  }
+  p->N = p->M / p->B;
+  if (a->pre) {
+    const int64_t s[2] = {p->M, p->F};
+    if ((rc = check_contig(a->pre, "pre", p->dtype, 2, s))) return rc;
+  }
+  return LLSA_OK;
+}
+
+// What the backward does, from the shapes and from which results are asked for
+void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
+  const int es = (int) dtype_size(p->dtype);
+  p->write_dz = a->activation != kActNone || a->gate;
+  p->sums = a->dbias || a->dgate;
+  p->dz_ld = (p->F + 7) / 8 * 8;
+  // columns in groups of 32: enough CTAs along the rows for 148 x 4 of them, 32 rows each or more
+  const int64_t cols = (p->F + 31) / 32;
+  p->chunks = std::max<int64_t>(1, std::min((148 * 4 + cols * p->B - 1) / (cols * p->B), (p->N + 31) / 32));
+  p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
+  p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
+  const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
+  p->split = (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
+  p->part_ld = p->K;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  p->o_dz = take(p->write_dz ? (size_t) (p->M * p->dz_ld * es) : 0);
+  p->o_cols = take(p->sums ? (size_t) (p->B * p->chunks * 2 * p->F * 4) : 0);
+  p->o_parts = take(a->dweight ? (size_t) (p->split * p->F * p->part_ld * 4) : 0);
+  p->bytes = at;
+}
+
+template <typename T>
+Mat<T> mat(const LlsaTensor* t) {
+  Mat<T> m;
+  m.p = t ? (T*) t->ptr : nullptr;
+  m.ld = t ? t->stride[0] : 0;
+  return m;
+}
+
+template <typename T>
+int product(const Product<T>& p, const Epilogue<T>& e, cudaStream_t st) { return launch_product<T, false>(p, e, nullptr, 0, st); }
+template <typename T>
+int product_parts(const Product<T>& p, float* partial, int64_t ld, cudaStream_t st) {
+  return launch_product<T, true>(p, Epilogue<T>{}, partial, ld, st);
+}
+
+template <typename T>
+int forward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
+  Epilogue<T> e = {};
+  e.bias = a->bias ? (const T*) a->bias->ptr : nullptr;
+  e.residual = mat<const T>(a->residual);
+  e.gate = mat<const T>(a->gate);
+  e.rows_per_gate = (uint32_t) p.N;
+  e.y = mat<T>(a->y);
+  e.pre = mat<T>(a->pre);
+  e.act = a->activation;
+  return product<T>({mat<const T>(a->x), mat<const T>(a->weight), 1, 1, p.M, p.F, p.K, 1}, e, st);
+}
+
+template <typename T>
+int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
+  char* ws = (char*) a->workspace;
+  Mat<const T> dz = mat<const T>(a->dy);
+  if (p.write_dz || p.sums) {
+    FrontArgs<T> f = {};
+    f.dy = dz;
+    f.pre = mat<const T>(a->pre);
+    f.gate = mat<const T>(a->gate);
+    if (p.write_dz) {
+      f.dz.p = (T*) (ws + p.o_dz);
+      f.dz.ld = p.dz_ld;
+      dz.p = f.dz.p;
+      dz.ld = f.dz.ld;
+    }
+    f.partial = p.sums ? (float*) (ws + p.o_cols) : nullptr;
+    f.N = (uint32_t) p.N; f.chunks = (uint32_t) p.chunks; f.per = (uint32_t) p.per;
+    f.F = (int) p.F;
+    f.act = a->activation;
+    LLSA_REQUIRE(p.B * p.chunks <= INT32_MAX, LLSA_ERR_SHAPE, "linear_bwd: too many samples");
+    launch_pdl(linear_dz_kernel<T>, dim3((unsigned) (p.B * p.chunks), (unsigned) ((p.F + 31) / 32)), dim3(256), 0, st, f);
+    LLSA_LAUNCH_OK("linear_dz_kernel");
+    if (p.sums) {
+      const ParamView none = {nullptr, 0, 0};
+      const int rc = finish_column_grads(f.partial, p.B, p.chunks, p.F, none, none, none,
+                                         {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
+      if (rc) return rc;
+    }
+  }
+  if (a->dx) {
+    Epilogue<T> e = {};
+    e.y = mat<T>(a->dx);
+    const int rc = product<T>({dz, mat<const T>(a->weight), 1, 0, p.M, p.K, p.F, 1}, e, st);
+    if (rc) return rc;
+  }
+  if (a->dweight) {
+    float* parts = (float*) (ws + p.o_parts);
+    const int rc = product_parts<T>({dz, mat<const T>(a->x), 0, 0, p.F, p.K, p.M, p.split}, parts, p.part_ld, st);
+    if (rc) return rc;
+    const int64_t blocks = std::min<int64_t>((p.F * p.K + 255) / 256, 148 * 8);
+    launch_pdl(sum_parts_kernel<T>, dim3((unsigned) blocks), dim3(256), 0, st, (const float*) parts, p.part_ld, p.split, p.F, p.K, (T*) a->dweight->ptr);
+    LLSA_LAUNCH_OK("sum_parts_kernel");
+  }
+  return LLSA_OK;
+}
+
+}  // namespace
+}  // namespace llsa
+
+using namespace llsa;
+
+extern "C" int llsa_linear_fwd(const LlsaLinearArgs* a, void* stream) {
+  Plan p;
+  int rc = check_common(a, &p);
+  if (rc) return rc;
+  const int64_t bs[1] = {p.F};
+  if (a->bias && (rc = check_contig(a->bias, "bias", p.dtype, 1, bs))) return rc;
+  if (a->residual && (rc = check_matrix(a->residual, "residual", p.dtype, p.M, p.F))) return rc;
+  LLSA_REQUIRE(!a->gate || a->residual, LLSA_ERR_ARG, "linear: a gate goes with a residual");
+  if ((rc = check_matrix(a->y, "y", p.dtype, p.M, p.F))) return rc;
+  if (p.M == 0) return LLSA_OK;
+  return p.dtype == LLSA_F32 ? forward<float>(a, p, (cudaStream_t) stream) : forward<bf16>(a, p, (cudaStream_t) stream);
+}
+
+extern "C" int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* a) {
+  Plan p;
+  if (check_common(a, &p)) return -1;
+  plan_bwd(a, &p);
+  return (int64_t) p.bytes;
+}
+
+extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
+  Plan p;
+  int rc = check_common(a, &p);
+  if (rc) return rc;
+  plan_bwd(a, &p);
+  if ((rc = check_matrix(a->dy, "dy", p.dtype, p.M, p.F))) return rc;
+  LLSA_REQUIRE(a->pre || (a->activation == kActNone && !a->dgate), LLSA_ERR_NULL, "pre: null tensor");
+  if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;
+  const int64_t ws[2] = {p.F, p.K}, gs[2] = {p.B, p.F}, bs[1] = {p.F};
+  if (a->dweight && (rc = check_contig(a->dweight, "dweight", p.dtype, 2, ws))) return rc;
+  if (a->dbias && (rc = check_grad(a->dbias, "dbias", p.dtype, 1, bs))) return rc;
+  if (a->dgate) {
+    LLSA_REQUIRE(a->gate, LLSA_ERR_NULL, "gate: null tensor");
+    if ((rc = check_grad(a->dgate, "dgate", p.dtype, 2, gs))) return rc;
+  }
+  LLSA_REQUIRE(p.bytes == 0 || (a->workspace && ((uintptr_t) a->workspace & 255) == 0 && a->workspace_bytes >= (int64_t) p.bytes), LLSA_ERR_WORKSPACE,
+               "workspace: llsa_linear_bwd_workspace_bytes() bytes on a 256-byte boundary are needed");
+  if (p.M == 0) {
+    if (a->dweight) LLSA_CUDA_OK(cudaMemsetAsync(a->dweight->ptr, 0, (size_t) (p.F * p.K) * dtype_size(p.dtype), (cudaStream_t) stream));
+    return clear_column_grads({make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, a->gate ? a->gate->shape[0] : 0, p.F,
+                              (cudaStream_t) stream);
+  }
+  return p.dtype == LLSA_F32 ? backward<float>(a, p, (cudaStream_t) stream) : backward<bf16>(a, p, (cudaStream_t) stream);
+}

@@ -1,0 +1,70 @@
+// What the projection's kernels share: the epilogue's operands, the activations, and the interface between linear.cu and the matrix products.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "column_sums.cuh"
+#include "common.cuh"
+
+namespace llsa {
+
+enum Activation { kActNone = 0, kActGeluTanh = 1, kActSilu = 2 };
+
+// A matrix with unit stride along one of its dimensions: element (i, j) at p[i * ld + j]
+template <typename T>
+struct Mat {
+  T* p;
+  int64_t ld;
+};
+
+// What stands behind the product z of a forward: y = residual + gate act(z + bias); `pre`, if given, keeps z + bias for the backward
+// (T; with an activation and bf16 data a half-precision float).
+template <typename T>
+struct Epilogue {
+  const T* bias;
+  Mat<const T> residual;
+  Mat<const T> gate;            // row = sample
+  uint32_t rows_per_gate;
+  Mat<T> y;
+  Mat<T> pre;
+  int act;
+};
+
+// 1 / (1 + e^-t).  FAST: two ulp of fp32 and what the argument's scaling by log2(e) costs, 2^-22 at |t| = 4: far below a bf16 step.
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float t) {
+  return FAST ? __fdividef(1.f, 1.f + __expf(-t)) : 1.f / (1.f + expf(-t));
+}
+constexpr float kGelu2 = 1.5957691216057308f, kGelu3 = 0.044715f;      // 2 sqrt(2 / pi)
+// gelu_tanh: z (1 + tanh(u)) / 2 = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3): no cancellation for negative z
+template <bool FAST>
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == kActGeluTanh) return z * sigmoid<FAST>(kGelu2 * z * fmaf(kGelu3 * z, z, 1.f));
+  if (act == kActSilu) return z * sigmoid<FAST>(z);
+  return z;
+}
+// The derivative; beyond |z| = 1e4 it is 0 or 1, and z^2 and an infinite z are kept out of its products with 0
+template <bool FAST>
+__device__ __forceinline__ float activate_grad(float z, int act) {
+  if (act == kActNone) return 1.f;
+  if (fabsf(z) > 1e4f) z = copysignf(1e4f, z);
+  const bool gelu = act == kActGeluTanh;
+  const float q = z * z, s = sigmoid<FAST>(gelu ? kGelu2 * z * fmaf(kGelu3, q, 1.f) : z);
+  const float du = gelu ? kGelu2 * fmaf(3.f * kGelu3, q, 1.f) : 1.f;
+  return fmaf(z * s * (1.f - s), du, s);
+}
+
+// What the backward of an activation reads back of z: bf16 data keep it as a half-precision float, in the same 16 bits.  Its rounding (2^-11) adds an eighth
+// of a bf16 step to the gradient, where z in bf16 would add a whole one; what leaves the range becomes infinite, where the derivative is 0 or 1.
+__device__ __forceinline__ uint16_t half_bits(float z) { return __half_as_ushort(__float2half_rn(z)); }
+__device__ __forceinline__ float half_value(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+
+// D[i, j] = sum_k A(i, k) B(j, k), k < K.  a_k: A(i, k) at a.p[i * ld + k] (else at a.p[k * ld + i]); b_k alike.
+template <typename T>
+struct Product {
+  Mat<const T> a, b;
+  int a_k, b_k;
+  int64_t M, N, K;
+  int split;                   // parts of the sum over k, one after another in `partial` (linear_sum_parts adds them); 1: none
+};
+
+}  // namespace llsa

@@ -3,7 +3,7 @@ training step": 12 blocks, hidden 384, 6 x 64 heads, MLP 1536, 128 x 128 x 3 syn
 ~ U{0..999}, noise-prediction MSE loss, bf16 autocast over fp32 parameters, AdamW, 8 images per GPU, data-parallel
 (DistributedDataParallel over NCCL, gradient all-reduce) when launched with torchrun.
 
-    python -m llsa_b200.dit_step_bench [--steps 10 --warmup 3 --batch 8 --layers 12 --attn sparse_l2]
+    python -m llsa_b200.dit_step_bench [--steps 10 --warmup 3 --batch 8 --layers 12 --attn sparse_l2 --fused-block]
     torchrun --nproc-per-node 8 -m llsa_b200.dit_step_bench --gpus 8
 
 Prints one JSON line: images/s over all ranks (CUDA events around K steps, max over ranks), ms per step, and the share of
@@ -30,6 +30,7 @@ def main():
     ap.add_argument("--size", type=int, default=128)
     ap.add_argument("--attn", default="sparse_l2", choices=["pixel", "sparse_l1", "sparse_l2"])
     ap.add_argument("--unfused-rope", action="store_true")
+    ap.add_argument("--fused-block", action="store_true", help="layer norms, projections and their epilogues on this package's operators")
     args = ap.parse_args()
     rank, world, local = int(os.environ.get("RANK", "0")), int(os.environ.get("WORLD_SIZE", "1")), int(os.environ.get("LOCAL_RANK", "0"))
     torch.cuda.set_device(local)
@@ -37,7 +38,8 @@ def main():
     if world > 1:
         dist.init_process_group("nccl", device_id=dev)
     torch.manual_seed(1234)
-    model = RopeDiT(layers=args.layers, sample_size=args.size, attn_type=args.attn, fused_rope=not args.unfused_rope).to(dev)
+    model = RopeDiT(layers=args.layers, sample_size=args.size, attn_type=args.attn, fused_rope=not args.unfused_rope,
+                    fused_block=args.fused_block).to(dev)
     net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local]) if world > 1 else model
     opt = torch.optim.AdamW(net.parameters(), lr=1e-4, fused=True)
     g = torch.Generator(device=dev).manual_seed(100 + rank)
@@ -97,7 +99,8 @@ def main():
                               scaling="weak", dtype="bf16 autocast, fp32 parameters", data="synthetic", loss=float(loss),
                               llsa_share_of_step=share,
                               config=dict(model="rope-DiT-S", layers=args.layers, hidden=384, heads=6, tokens=args.size * args.size,
-                                          attention=args.attn, fused_rope=not args.unfused_rope, images_per_gpu=args.batch,
+                                          attention=args.attn, fused_rope=not args.unfused_rope, fused_block=args.fused_block,
+                                          images_per_gpu=args.batch,
                                           parallelism="ddp%d" % world))), flush=True)
     if world > 1:
         dist.destroy_process_group()

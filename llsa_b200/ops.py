@@ -12,6 +12,10 @@ unchanged:
     flash_sparse_residual_attention_l1_op / _l2_op            torch_op/flash_sparse_attention_res_{1,2}.py:38, :45
     llsa_l1, llsa_l2                           torch_op/flash_sparse_attention_res_1.py:41, _res_2.py:48
 
+The operators around the attention of a block have no counterpart of their own there (the block calls torch's):
+
+    layer_norm, linear, rope_axes              models/rope_dit_transformer_2d.py:295-337, :205-258 and :640-711, :71-109
+
 Every function enqueues CUDA work on the current stream through
 libllsa_b200.so; tensors must live on a CUDA device.  llsa_l1 / llsa_l2 and their
 fused forms are one dispatcher operator each way with C++ autograd
@@ -35,7 +39,7 @@ __all__ = [
     "sparse_indices_attn_res_2_2_fwd", "sparse_indices_attn_res_scatter_2_2_bwd_v2",
     "flash_sparse_residual_attention_l1_op", "flash_sparse_residual_attention_l2_op",
     "llsa_l1", "llsa_l2", "llsa_l1_rope", "llsa_l2_rope", "pool_pyramid", "rope_pool_pyramid", "set_exact_pooled_grad",
-    "set_device_checks", "rms_norm", "rms_rope_pool_pyramid", "llsa_l1_rms_rope", "llsa_l2_rms_rope",
+    "set_device_checks", "layer_norm", "linear", "rope_axes", "rms_norm", "rms_rope_pool_pyramid", "llsa_l1_rms_rope", "llsa_l2_rms_rope",
 ]
 
 _FLOAT = (torch.float32, torch.bfloat16)
@@ -166,6 +170,33 @@ def _register_fakes() -> None:
     def _(d_o, q, k, v, o, saved, freq, xq, xk, wq, wk, eps, topk1, topk2, block_size, levels, want_dw):
         out = [torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)]
         return out + ([torch.empty_like(w) for w in (wq, wk) if w is not None] if want_dw else [])
+
+    @torch.library.register_fake("llsa_b200::layer_norm_fwd")
+    def _(x, weight, bias, scale, shift, eps, want_stats):
+        y = torch.empty_like(x)
+        return [y, x.new_empty((x.numel() // x.shape[-1] * 2,), dtype=torch.float32)] if want_stats else [y]
+
+    @torch.library.register_fake("llsa_b200::layer_norm_bwd")
+    def _(dy, x, weight, bias, scale, stats, want, shift_type, bias_type):
+        C = x.shape[-1]
+        types = (weight.dtype if weight is not None else torch.float32, bias_type, scale.dtype if scale is not None else torch.float32, shift_type)
+        return [x.new_empty(x.shape)] + [x.new_empty((C,) if i < 2 else (x.shape[0], C), dtype=types[i]) for i in range(4) if want >> i & 1]
+
+    @torch.library.register_fake("llsa_b200::linear_fwd")
+    def _(x, weight, bias, residual, gate, activation, want_pre):
+        F = weight.shape[0]
+        y = x.new_empty((*x.shape[:-1], F))
+        return [y, x.new_empty((x.numel() // x.shape[-1], F))] if want_pre else [y]
+
+    @torch.library.register_fake("llsa_b200::linear_bwd")
+    def _(dy, x, weight, pre, gate, activation, want):
+        F = weight.shape[0]
+        shapes = (x.shape, weight.shape, (F,), (x.shape[0] if gate is not None else 1, F))
+        return [x.new_empty(shapes[i]) for i in range(4) if want >> i & 1]
+
+    @torch.library.register_fake("llsa_b200::rope_axes")
+    def _(x, positions, axes_dims, theta, inverse):
+        return torch.empty_like(x)
 
     @torch.library.register_fake("llsa_b200::attn_fwd")
     def _(q, k, v, pk, pv, pk2, pv2, indices, p_indices, topk, topk_p, block_size, w1, w2):
@@ -426,6 +457,51 @@ def my_rope_fn(x: torch.Tensor, freq: torch.Tensor) -> torch.Tensor:
     """Interleaved-pair RoPE by a [S,D] (sin, cos) table; differentiable in x.
     Mirrors my_rope_fn = MyRopeFunction.apply (triton/rope.py:100-148)."""
     return _rope_fwd_op(x, freq)
+
+
+def rope_axes(x: torch.Tensor, positions: torch.Tensor, axes_dims, theta: float = 10000.0) -> torch.Tensor:
+    """Interleaved-pair RoPE of x [B,H,N,D] by positions on several axes (rows and columns of an image; time, rows and columns of a clip), without a
+    table; differentiable in x.
+
+    axes_dims: channels of each axis, 1 to 4 positive even numbers that are D together (at most 512); pair i of axis a turns by
+    positions[n, a] * theta ** (-2 i / axes_dims[a]) (models/rope_dit_transformer_2d.py:71-109), the angle taken in 64 bits, so that far
+    positions lose nothing.  positions: [N, A], or [B, N, A] for samples with positions of their own; int32, int64 or (between the points of a
+    grid) float32.  Any strides of x; what my_rope_fn does with a table of the same positions, up to the table's rounding."""
+    _ready()
+    return torch.ops.llsa_b200.rope_axes(x, positions, tuple(int(d) for d in axes_dims), float(theta), False)
+
+
+# ----------------------------------------------------------------------------- norm and projections of a block
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Layer norm over the last dimension of x [B, ..., C] (1 to 16384 channels) with what adaLN puts behind it
+    (models/rope_dit_transformer_2d.py:295-337):
+
+        y = (h * weight + bias) * (1 + scale) + shift,    h = (x - mean) / sqrt(var + eps)
+
+    weight, bias: [C]; scale, shift: [B, C], a sample's for all of its tokens (views of a modulation's output as they are).  Each may be absent, and
+    is float32 or of x's type.  Differentiable in all five.  Sums are taken in fp32 and in a fixed order; y and every gradient are rounded once."""
+    _ready()
+    return torch.ops.llsa_b200.layer_norm_fwd(x, weight, bias, scale, shift, float(eps), False)[0]
+
+
+_ACTIVATIONS = {None: 0, "gelu_tanh": 1, "silu": 2}
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A projection with what stands behind it in one kernel (models/rope_dit_transformer_2d.py:205-213, :254-258, :640-711):
+
+        y = residual + gate * act(x @ weight.T + bias)
+
+    x: [..., K]; weight: [F, K]; bias: [F]; activation: None, "gelu_tanh" or "silu"; residual: of y's shape [..., F]; gate: [B, F], a sample's
+    factors for all of its tokens (x is then [B, ..., K]), with a residual and without an activation.  All of one type, float32 or
+    bfloat16; sums are fp32.  Differentiable in all five.  For a gradient through an activation or of a gate the product is kept (16 bits a value for
+    bfloat16).  Rows that are no multiple of 16 bytes cost bfloat16 operands a copy."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError("llsa_b200: activation must be None, 'gelu_tanh' or 'silu', got %r" % (activation,))
+    _ready()
+    return torch.ops.llsa_b200.linear_fwd(x, weight, bias, residual, gate, _ACTIVATIONS[activation], False)[0]
 
 
 # ----------------------------------------------------------------------------- selection

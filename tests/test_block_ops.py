@@ -1,0 +1,585 @@
+"""layer_norm, linear and rope_axes against their formulas in 64 bits.
+
+Tolerances are counted.  u = 2^-24 is half a step of fp32; a result of type T is rounded once, which is half a step of T relative to the value (2^-24 or
+2^-8).  What fp32 arithmetic adds is at most (roundings on the way) * u * (the sum of the terms' magnitudes); each test says how many.
+"""
+import math
+
+import pytest
+import torch
+
+import llsa_b200
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(name, got, want, fp32_error, roundings=1.0):
+    """|got - want| <= `roundings` half steps of got's type, plus what fp32 sums add."""
+    tol = roundings * half_step(got.dtype) * want.abs() + fp32_error + 1e-40
+    off = (got.double() - want).abs()
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    assert bool((off <= tol).all()), "%s: off by %.3g where %.3g is allowed" % (name, float(off.max()), float(tol.flatten()[(off - tol).argmax()]))
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def normal(g, *shape, dtype=F32, std=1.0, mean=0.0):
+    return (torch.randn(shape, generator=g, device=DEV) * std + mean).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------------ layer norm
+def norm_reference(x, w, b, s, t, eps, dy=None):
+    """y and the gradients in 64 bits, and the magnitudes that rounding errors scale with.  x: [B, N, C]."""
+    x, w, b, s, t, dy = [v.detach().double() if v is not None else None for v in (x, w, b, s, t, dy)]
+    mean, mag = x.mean(-1, keepdim=True), x.abs().mean(-1, keepdim=True)
+    rstd = 1 / ((x - mean).square().mean(-1, keepdim=True) + eps).sqrt()
+    h, hb = (x - mean) * rstd, ((x - mean).abs() + mag) * rstd
+    W = w if w is not None else torch.ones_like(x[0, 0])
+    Bi = b if b is not None else torch.zeros_like(W)
+    up = 1 + s[:, None] if s is not None else torch.ones_like(x[:, :1, :])
+    sh = t[:, None] if t is not None else torch.zeros_like(x[:, :1, :])
+    y, yb = (h * W + Bi) * up + sh, (hb * W.abs() + Bi.abs()) * up.abs() + sh.abs()
+    if dy is None:
+        return dict(y=(y, yb))
+    g = dy * up * W
+    dx = rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
+    dxb = rstd * (g.abs() + g.abs().mean(-1, keepdim=True) + hb * (g.abs() * hb).mean(-1, keepdim=True))
+    return dict(y=(y, yb), x=(dx, dxb), w=((dy * up * h).sum((0, 1)), (dy.abs() * up.abs() * hb).sum((0, 1))),
+                b=((dy * up).sum((0, 1)), (dy.abs() * up.abs()).sum((0, 1))),
+                s=((dy * (h * W + Bi)).sum(1), (dy.abs() * (hb * W.abs() + Bi.abs())).sum(1)), t=(dy.sum(1), dy.abs().sum(1)))
+
+
+NORM_SHAPES = [(1, 1, 1), (1, 1, 2), (2, 3, 5), (1, 7, 32), (2, 17, 100), (3, 33, 129), (4, 9, 384), (2, 100, 390), (1, 50, 512), (2, 31, 516), (3, 11, 1155),
+               (2, 13, 2048), (1, 5, 2050), (1, 4, 4096), (2, 3, 4100), (1, 3, 5001), (1, 2, 16384), (257, 1, 48), (40, 3, 64), (2, 5000, 24)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,N,C", NORM_SHAPES)
+@pytest.mark.parametrize("given", ["", "wb", "st", "wbst", "ws"])
+def test_layer_norm_against_its_formula(B, N, C, dtype, given):
+    g = gen(B * 1000003 + N * 1009 + C)
+    eps = 1e-5
+    x = normal(g, B, N, C, dtype=dtype, std=1.5, mean=0.7)
+    made = dict(w=normal(g, C, dtype=dtype, std=0.2, mean=1), b=normal(g, C, dtype=dtype, std=0.2))
+    mod = normal(g, B, 6 * C, dtype=dtype, std=0.3).chunk(6, 1)      # rows with a stride of their own
+    made.update(s=mod[1], t=mod[4])
+    p = {k: made[k].detach().requires_grad_(True) if k in given else None for k in "wbst"}
+    x.requires_grad_(True)
+    dy = normal(g, B, N, C, dtype=dtype)
+    y = llsa_b200.layer_norm(x, p["w"], p["b"], eps, scale=p["s"], shift=p["t"])
+    names = [k for k in "wbst" if k in given]
+    grads = torch.autograd.grad(y, [x] + [p[k] for k in names], dy)
+    ref = norm_reference(x, p["w"], p["b"], p["s"], p["t"], eps, dy)
+    # 16 values of a thread, 5 steps of a warp, 32 warps: 53 additions deep, for the mean, the squares and the products; some 10 roundings beside
+    within("y", y, ref["y"][0], 120 * U * ref["y"][1])
+    within("dx", grads[0], ref["x"][0], 300 * U * ref["x"][1])
+    for k, d in zip(names, grads[1:]):      # a sum over all rows on top
+        assert d.dtype == p[k].dtype
+        within("d" + k, d, ref[k][0], (200 + B * N) * U * ref[k][1])
+
+
+@pytest.mark.parametrize("param", [BF16, F32])
+def test_layer_norm_takes_parameters_of_either_type(param):
+    g = gen(3)
+    x = normal(g, 2, 9, 96, dtype=BF16).requires_grad_(True)
+    w, b = normal(g, 96, dtype=param, std=0.1, mean=1).requires_grad_(True), normal(g, 96, dtype=param).requires_grad_(True)
+    s, t = normal(g, 2, 96, dtype=param, std=0.2).requires_grad_(True), normal(g, 2, 96, dtype=param).requires_grad_(True)
+    dy = normal(g, 2, 9, 96, dtype=BF16)
+    y = llsa_b200.layer_norm(x, w, b, 1e-5, scale=s, shift=t)
+    ref = norm_reference(x, w, b, s, t, 1e-5, dy)
+    within("y", y, ref["y"][0], 120 * U * ref["y"][1])
+    for k, d in zip("wbst", torch.autograd.grad(y, [w, b, s, t], dy)):
+        assert d.dtype == param
+        within(k, d, ref[k][0], 220 * U * ref[k][1])
+
+
+def test_layer_norm_any_rank_strides_and_alignment():
+    g = gen(4)
+    eps = 1e-6
+    base = normal(g, 3, 7, 5, 48)
+    want = norm_reference(base.reshape(3, 35, 48), None, None, None, None, eps)["y"]
+    check = lambda y, shape: within("y", y.reshape(3, 35, 48), want[0], 120 * U * want[1])
+    check(llsa_b200.layer_norm(base, eps=eps), None)
+    check(llsa_b200.layer_norm(base.reshape(105, 48), eps=eps), None)
+    room = torch.zeros(3, 7, 5, 60, device=DEV)
+    for first in (0, 1, 3, 4):                                  # rows with gaps, on any boundary
+        room[..., first:first + 48] = base
+        check(llsa_b200.layer_norm(room[..., first:first + 48], eps=eps), None)
+    check(llsa_b200.layer_norm(base.transpose(-1, -2).contiguous().transpose(-1, -2), eps=eps), None)      # channels apart
+    token_major = base.reshape(3, 35, 48).transpose(0, 1).contiguous().transpose(0, 1)                     # [B,N,C] view of [N,B,C]
+    y = llsa_b200.layer_norm(token_major, eps=eps, shift=torch.zeros(3, 48, device=DEV))
+    assert y.stride() == token_major.stride()
+    check(y, None)
+    one = llsa_b200.layer_norm(base[0, 0, 0], eps=eps)
+    assert one.shape == (48,) and torch.equal(one, llsa_b200.layer_norm(base, eps=eps)[0, 0, 0])
+    shared = base[:1, :, 0].expand(3, 7, 48)                    # samples on top of one another
+    assert torch.equal(llsa_b200.layer_norm(shared, eps=eps)[2], llsa_b200.layer_norm(base[:1, :, 0], eps=eps)[0])
+
+
+def test_layer_norm_gradient_of_an_expanded_upstream_and_without_parameters():
+    g = gen(5)
+    x = normal(g, 2, 6, 40).requires_grad_(True)
+    (d,) = torch.autograd.grad(llsa_b200.layer_norm(x).sum(), x)
+    ref = norm_reference(x, None, None, None, None, 1e-5, torch.ones_like(x))
+    within("dx", d, ref["x"][0], 300 * U * ref["x"][1])
+    w = torch.ones(40, device=DEV, requires_grad=True)          # only the weight wants a gradient
+    (dw,) = torch.autograd.grad(llsa_b200.layer_norm(x.detach(), w).sum(), w)
+    within("dw", dw, ref["w"][0], 220 * U * ref["w"][1])
+
+
+def test_layer_norm_keeps_a_bad_row_to_itself():
+    g = gen(6)
+    x = normal(g, 1, 8, 64, dtype=BF16)
+    good = llsa_b200.layer_norm(x)
+    x[0, 3, 5], x[0, 6, 1] = float("nan"), float("inf")
+    y = llsa_b200.layer_norm(x)
+    keep = [0, 1, 2, 4, 5, 7]
+    assert torch.equal(y[0, keep], good[0, keep]) and torch.isnan(y[0, [3, 6]]).any(-1).all()
+    const = llsa_b200.layer_norm(torch.full((1, 2, 64), 3.0, device=DEV), shift=torch.full((1, 64), 2.0, device=DEV))
+    assert torch.equal(const, torch.full_like(const, 2.0))      # no spread: the shift alone
+    far = torch.full((1, 1, 64), 1e4, device=DEV)
+    far[0, 0, ::2] += 1
+    assert torch.equal(llsa_b200.layer_norm(far, eps=0.0).abs(), torch.ones(1, 1, 64, device=DEV))      # a large common offset cancels nothing
+
+
+# ------------------------------------------------------------------------------------------------------ projection
+def act64(z, act):
+    """The activation and its slope."""
+    if act is None:
+        return z, torch.ones_like(z)
+    k = 1.0 if act == "silu" else 2 * math.sqrt(2 / math.pi)
+    inner, slope = (z, torch.ones_like(z)) if act == "silu" else (z + 0.044715 * z ** 3, 1 + 3 * 0.044715 * z ** 2)
+    s = torch.sigmoid(k * inner)
+    return z * s, s + z * s * (1 - s) * k * slope
+
+
+def linear_reference(x, w, b, act, r, gate, dy=None):
+    x, w, b, r, gate, dy = [v.detach().double() if v is not None else None for v in (x, w, b, r, gate, dy)]
+    K, F = w.shape[1], w.shape[0]
+    z, zb = x @ w.T, x.abs() @ w.abs().T
+    if b is not None:
+        z, zb = z + b, zb + b.abs()
+    a, slope = act64(z, act)
+    G = gate.reshape(gate.shape[0], *[1] * (x.dim() - 2), F) if gate is not None else 1.0
+    y = a * G + (r if r is not None else 0)
+    out = dict(y=y, z=z, zb=zb, G=G, slope=slope)
+    if dy is not None:
+        dz = (dy * G * slope)
+        flat, xf = dz.reshape(-1, F), x.reshape(-1, K)
+        out.update(dz=dz, x=dz @ w, xb=dz.abs() @ w.abs(), w=flat.T @ xf, wb=flat.abs().T @ xf.abs(), b=flat.sum(0), bb=flat.abs().sum(0), r=dy)
+        if gate is not None:
+            per = lambda t: t.reshape(gate.shape[0], -1, F).sum(1)
+            out.update(g=per(dy * a), gb=per(dy.abs() * zb))
+    return out
+
+
+LINEAR_SHAPES = [(1, 1, 1, 1), (1, 1, 16, 16), (8, 1, 256, 384), (1, 5, 3, 7), (2, 65, 64, 64), (1, 128, 128, 192), (2, 130, 72, 200), (3, 77, 389, 133), (1, 300, 384, 3),
+                 (2, 100, 390, 256), (1, 257, 520, 1032), (5, 60, 1536, 384), (2, 1000, 384, 1152), (1, 2049, 40, 8)]
+FORMS = [("plain", None, False, False), ("gelu", "gelu_tanh", False, False), ("silu", "silu", False, False), ("residual", None, True, False),
+         ("gated", None, True, True), ("gelu residual", "gelu_tanh", True, False)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,N,K,F", LINEAR_SHAPES)
+@pytest.mark.parametrize("form", FORMS, ids=[f[0] for f in FORMS])
+def test_linear_against_its_formula(B, N, K, F, dtype, form):
+    _, act, with_r, with_g = form
+    g = gen(B * 1000003 + N * 1009 + K * 31 + F)
+    t = dict(x=normal(g, B, N, K, dtype=dtype), w=normal(g, F, K, dtype=dtype, std=K ** -0.5), b=normal(g, F, dtype=dtype, std=0.3))
+    if with_r:
+        t["r"] = normal(g, B, N, F, dtype=dtype)
+    if with_g:
+        t["g"] = normal(g, B, 6 * F, dtype=dtype, std=0.5).chunk(6, 1)[2]
+    t = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    dy = normal(g, B, N, F, dtype=dtype)
+    y = llsa_b200.linear(t["x"], t["w"], t["b"], activation=act, residual=t.get("r"), gate=t.get("g"))
+    grads = dict(zip(t, torch.autograd.grad(y, list(t.values()), dy)))
+    check_linear(t, dy, act, y, grads, dtype)
+
+
+def check_linear(t, dy, act, y, grads, dtype):
+    M, K, F = dy.numel() // dy.shape[-1], t["x"].shape[-1], dy.shape[-1]
+    ref = linear_reference(t["x"], t["w"], t.get("b"), act, t.get("r"), t.get("g"), dy)
+    G = ref["G"].abs() if torch.is_tensor(ref["G"]) else 1.0
+    # z: K products and additions, each within 2 u of the running sum (a tensor core cuts where an FMA rounds), and the bias.  No activation's slope
+    # exceeds 1.13; the activation itself is 8 roundings, its exponential is off by 2 ulp and by u |argument| <= 80 u
+    ez = (2 * K + 4) * U * ref["zb"]
+    ea = 1.13 * ez + (100 * U if act else 0) * ref["z"].abs()
+    r_mag = t["r"].detach().double().abs() if "r" in t else 0.0
+    within("y", y, ref["y"], ea * G + 4 * U * (ref["zb"] * G + r_mag))
+    # dz is rounded to its type (bf16: one half step of every term); behind an activation of bf16 data z is kept to 2^-11 of itself, and no slope changes
+    # faster than 1.13 per unit of z (gelu's curvature at 0 is 2 sqrt(2 / pi) < 1.6; silu's 1/2)
+    hs, adz = half_step(dtype), ref["dz"].abs()
+    moved = ((2.0 ** -11 + 1e-7) if dtype == BF16 else 0.0) * ref["z"].abs() + ez + (2.0 ** -25 if dtype == BF16 else 0.0)
+    edz = (1.6 * moved + 100 * U) * (dy.double().abs() * G) if act else 2 * U * adz
+    keeps = act is not None or "g" in t                          # dz is written, and rounded
+    edz = edz + (hs * (1 + 0.01) if keeps else 0) * (adz + edz)
+    wd = t["w"].detach().double().abs()
+    xf = t["x"].detach().double().abs().reshape(-1, K)
+    within("dx", grads["x"], ref["x"], edz @ wd + (2 * F + 4) * U * (ref["xb"] + edz @ wd))
+    flat = edz.reshape(-1, F)
+    within("dw", grads["w"], ref["w"], flat.T @ xf + (2 * M + 400) * U * (ref["wb"] + flat.T @ xf))
+    if "b" in grads:                                             # the sum of dz before it is rounded
+        eb = ((1.6 * moved + 100 * U) * (dy.double().abs() * G) if act else 2 * U * adz).reshape(-1, F).sum(0)
+        within("db", grads["b"], ref["b"], eb + (M + 100) * U * ref["bb"])
+    if "r" in grads:
+        assert torch.equal(grads["r"], dy)
+    if "g" in grads:                                             # z is kept in the data's type: half a step of every term
+        B = t["g"].shape[0]
+        kept = (dy.double().abs() * (hs * 1.01 * ref["z"].abs() + ez)).reshape(B, -1, F).sum(1)
+        within("dgate", grads["g"], ref["g"], kept + (M + 100) * U * ref["gb"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_linear_strides_ranks_and_partial_gradients(dtype):
+    g = gen(11)
+    K, F = 72, 40
+    room = normal(g, 4, 21, 100, dtype=dtype)
+    w, dy = normal(g, F, K, dtype=dtype, std=0.1), normal(g, 4, 21, F, dtype=dtype)
+    for first in (0, 1, 8, 16):                                  # rows with gaps, on any boundary
+        t = dict(x=room[..., first:first + K].detach().requires_grad_(True), w=w.detach().requires_grad_(True))
+        y = llsa_b200.linear(t["x"], t["w"])
+        check_linear(t, dy, None, y, dict(zip(t, torch.autograd.grad(y, list(t.values()), dy))), dtype)
+    wt = normal(g, K, F, dtype=dtype, std=0.1).t()               # a weight stored the other way round
+    t = dict(x=room[:, ::3, :K].detach().requires_grad_(True), w=wt.detach().requires_grad_(True))
+    y = llsa_b200.linear(t["x"], t["w"])
+    check_linear(t, dy[:, ::3], None, y, dict(zip(t, torch.autograd.grad(y, list(t.values()), dy[:, ::3]))), dtype)
+    flat = llsa_b200.linear(room[0, 0, :K], w)
+    assert flat.shape == (F,)
+    deep = llsa_b200.linear(room[..., :K].reshape(2, 2, 3, 7, K), w)
+    assert deep.shape == (2, 2, 3, 7, F) and torch.equal(deep.reshape(-1, F), llsa_b200.linear(room[..., :K].reshape(-1, K), w))
+    # one gradient at a time gives the bits of all together
+    full = {}
+    names = ["x", "w", "b", "r", "g"]
+    data = dict(x=room[..., :K], w=w, b=normal(g, F, dtype=dtype), r=normal(g, 4, 21, F, dtype=dtype), g=normal(g, 4, F, dtype=dtype))
+    for wanted in [names] + [[n] for n in names]:
+        t = {k: v.detach().clone().requires_grad_(k in wanted) for k, v in data.items()}
+        y = llsa_b200.linear(t["x"], t["w"], t["b"], residual=t["r"], gate=t["g"])
+        for k, d in zip(wanted, torch.autograd.grad(y, [t[k] for k in wanted], dy)):
+            assert torch.equal(full.setdefault(k, d), d), k
+    # an upstream gradient that is one number everywhere
+    x = room[..., :K].detach().requires_grad_(True)
+    (d,) = torch.autograd.grad(llsa_b200.linear(x, w).sum(), x)
+    t = dict(x=x, w=w)
+    check_linear(t, torch.ones(4, 21, F, device=DEV, dtype=dtype), None, llsa_b200.linear(x, w), dict(x=d, w=linear_reference(x, w, None, None, None, None, torch.ones(4, 21, F, device=DEV))["w"]), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_linear_far_values(dtype):
+    """Activations far out on either side, a zero gate, and rows that are not numbers."""
+    z = torch.tensor([-1e30, -7e4, -300.0, -30.0, -8.0, 0.0, 8.0, 300.0, 7e4, 1e30], device=DEV)
+    x = torch.zeros(1, len(z), 16, device=DEV, dtype=dtype)
+    x[0, :, 0] = z.to(dtype)
+    w = torch.zeros(16, 16, device=DEV, dtype=dtype)
+    w[:, 0] = 1
+    zz = x[0, :, 0].double()
+    for act in ("gelu_tanh", "silu"):
+        xg = x.detach().requires_grad_(True)
+        y = llsa_b200.linear(xg, w, activation=act)
+        arg = zz if act == "silu" else 2 * math.sqrt(2 / math.pi) * (zz + 0.044715 * zz ** 3)
+        s = torch.sigmoid(arg)
+        # e^-t with t off by 3 roundings, 3 u |t|, is off by that much relative to itself; below e^-100 nothing of an fp32 result is left
+        rel = 2 * half_step(dtype) + 4 * U * arg.abs().clamp(max=100)
+        assert ((y[0, :, 3].double() - zz * s).abs() <= rel * (zz * s).abs() + 1e-30).all(), act
+        (d,) = torch.autograd.grad(y[..., 3].sum(), xg)
+        _, slope = act64(zz.clamp(-1e4, 1e4), act)
+        assert torch.isfinite(d).all() and ((d[0, :, 0].double() - slope).abs() <= 4 * half_step(dtype) * slope.abs() + 1e-6).all(), act
+    g = gen(12)
+    x, w, r = normal(g, 1, 9, 64, dtype=dtype), normal(g, 24, 64, dtype=dtype), normal(g, 1, 9, 24, dtype=dtype)
+    closed = torch.zeros(1, 24, device=DEV, dtype=dtype).requires_grad_(True)
+    y = llsa_b200.linear(x, w, residual=r, gate=closed)
+    assert torch.equal(y, r)                                      # as a freshly initialised adaLN-zero block leaves its input
+    (d,) = torch.autograd.grad(y.sum(), closed)
+    assert (d != 0).all()
+    good = llsa_b200.linear(x, w)
+    x[0, 4, 7] = float("nan")
+    bad = llsa_b200.linear(x, w)
+    keep = [0, 1, 2, 3, 5, 6, 7, 8]
+    assert torch.isnan(bad[0, 4]).all() and torch.equal(bad[0, keep], good[0, keep])
+
+
+# ------------------------------------------------------------------------------------------------------ rotary positions
+def rope_reference(x, pos, axes, theta, sign=1.0):
+    x = x.detach().double()
+    ang = torch.cat([pos[..., a, None].double() * theta ** (-torch.arange(0, d, 2, device=DEV, dtype=torch.float64) / d) for a, d in enumerate(axes)], -1)
+    ang = sign * (ang[:, None] if ang.dim() == 3 else ang)
+    e, o = x[..., 0::2], x[..., 1::2]
+    y = torch.stack([ang.cos() * e - ang.sin() * o, ang.sin() * e + ang.cos() * o], -1).flatten(-2)
+    mag = torch.stack([e.abs() + o.abs()] * 2, -1).flatten(-2)
+    return y, mag
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,H,N,axes", [(1, 1, 1, (2,)), (1, 2, 3, (2, 4)), (2, 3, 65, (32, 32)), (1, 6, 100, (16, 24, 24)), (3, 5, 33, (10,)), (2, 4, 17, (6, 6, 2, 4)),
+                                        (4, 6, 257, (64, 64)), (1, 1, 5000, (64,)), (2, 1, 7, (256, 256))])
+@pytest.mark.parametrize("kind", ["int64", "int32", "float32", "per sample"])
+def test_rope_axes_against_its_formula(B, H, N, axes, dtype, kind):
+    g = gen(B + 7 * H + 31 * N + sum(axes))
+    x = normal(g, B, N, H, sum(axes), dtype=dtype).transpose(1, 2).requires_grad_(True)      # heads side by side, as a projection leaves them
+    shape = (B, N, len(axes)) if kind == "per sample" else (N, len(axes))
+    pos = torch.randint(-1000, 1 << 20, shape, generator=g, device=DEV)
+    if kind == "int32":
+        pos = pos.int()
+    if kind == "float32":
+        pos = pos.float() * 0.01
+    y = llsa_b200.rope_axes(x, pos, axes, 10000.0)
+    assert y.stride() == x.stride()
+    dy = normal(g, B, H, N, sum(axes), dtype=dtype)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    # the angle in units of pi is rounded to fp32 once (pi u / 2), sine and cosine are off by 2 ulp, and three more roundings: below 8 u
+    for got, (want, mag) in ((y, rope_reference(x, pos, axes, 10000.0)), (dx, rope_reference(dy, pos, axes, 10000.0, -1.0))):
+        within("rope", got, want, 8 * U * mag)
+
+
+def test_rope_axes_strides_alignment_and_table():
+    g = gen(21)
+    pos = torch.randint(0, 64, (40, 2), generator=g, device=DEV)
+    room = normal(g, 2, 3, 40, 80, dtype=BF16)
+    want = llsa_b200.rope_axes(room[..., :64].contiguous(), pos, (32, 32))
+    for first in (0, 1, 2, 8):
+        room2 = torch.zeros(2, 3, 40, 80, device=DEV, dtype=BF16)
+        room2[..., first:first + 64] = room[..., :64]
+        assert torch.equal(llsa_b200.rope_axes(room2[..., first:first + 64], pos, (32, 32)), want)
+    apart = room[..., :64].transpose(2, 3).contiguous().transpose(2, 3)
+    assert torch.equal(llsa_b200.rope_axes(apart, pos, (32, 32)), want)
+    shared = room[:, :1, :, :64].expand(2, 3, 40, 64)
+    assert torch.equal(llsa_b200.rope_axes(shared, pos, (32, 32))[:, 2], want[:, 0])
+    assert torch.equal(llsa_b200.rope_axes(room[..., :64], pos.repeat(1, 2)[:, :2], (32, 32)), want)           # positions with a row stride
+    assert torch.equal(llsa_b200.rope_axes(room[..., :64], pos.t().contiguous().t(), (32, 32)), want)          # and axis by axis
+    # my_rope_fn with an fp32 table of the same angles: equal up to the table's rounding and the order of the arithmetic
+    x = normal(g, 1, 2, 40, 64)
+    om = 10000.0 ** (-torch.arange(0, 32, 2, device=DEV, dtype=torch.float64) / 32)
+    ang = torch.cat([pos[:, a, None].double() * om for a in range(2)], -1)
+    table = torch.stack([ang.sin(), ang.cos()], -1).flatten(-2).float()
+    _, mag = rope_reference(x, pos, (32, 32), 10000.0)
+    assert ((llsa_b200.rope_axes(x, pos, (32, 32)) - llsa_b200.my_rope_fn(x, table)).double().abs() <= 12 * U * mag).all()
+
+
+def test_rope_axes_turns_back_and_differentiates_twice():
+    g = gen(22)
+    x = normal(g, 1, 2, 9, 32).requires_grad_(True)
+    pos = torch.arange(9, device=DEV)[:, None]
+    y = llsa_b200.rope_axes(x, pos, (32,))
+    dy = normal(g, 1, 2, 9, 32).requires_grad_(True)
+    (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    (ddy,) = torch.autograd.grad(dx, dy, x.detach())              # the rotation again
+    assert torch.equal(ddy, y)
+
+
+# ------------------------------------------------------------------------------------------------------ differences, streams, graphs, compiler
+@pytest.mark.parametrize("what", ["norm", "linear gelu", "linear gated", "rope"])
+def test_gradients_against_differences(what):
+    """The kernel's gradient along a direction against central differences of the formula in 64 bits.  The step of 1e-4 leaves an error of
+    about 1e-8 of the third derivative; fp32 gradients carry some 1e-6."""
+    g = gen(31)
+    if what == "norm":
+        leaves = [normal(g, 2, 5, 33), normal(g, 33, mean=1.0, std=0.2), normal(g, 33), normal(g, 2, 33, std=0.3), normal(g, 2, 33)]
+        f = lambda x, w, b, s, t: llsa_b200.layer_norm(x, w, b, 1e-3, scale=s, shift=t)
+        ref = lambda x, w, b, s, t: norm_reference(x, w, b, s, t, 1e-3)["y"][0]
+    elif what == "linear gelu":
+        leaves = [normal(g, 2, 5, 20), normal(g, 11, 20, std=0.3), normal(g, 11)]
+        f = lambda x, w, b: llsa_b200.linear(x, w, b, activation="gelu_tanh")
+        ref = lambda x, w, b: linear_reference(x, w, b, "gelu_tanh", None, None)["y"]
+    elif what == "linear gated":
+        leaves = [normal(g, 2, 5, 20), normal(g, 11, 20, std=0.3), normal(g, 11), normal(g, 2, 5, 11), normal(g, 2, 11)]
+        f = lambda x, w, b, r, gt: llsa_b200.linear(x, w, b, residual=r, gate=gt)
+        ref = lambda x, w, b, r, gt: linear_reference(x, w, b, None, r, gt)["y"]
+    else:
+        leaves, pos = [normal(g, 2, 3, 5, 12)], torch.randint(0, 50, (5, 2), generator=g, device=DEV)
+        f = lambda x: llsa_b200.rope_axes(x, pos, (4, 8))
+        ref = lambda x: rope_reference(x, pos, (4, 8), 10000.0)[0]
+    leaves = [t.requires_grad_(True) for t in leaves]
+    y = f(*leaves)
+    dy = normal(g, *y.shape)
+    grads = torch.autograd.grad(y, leaves, dy)
+    for i, (leaf, grad) in enumerate(zip(leaves, grads)):
+        v = normal(g, *leaf.shape).double()
+        at = lambda e: (ref(*[t.detach().double() + (e * v if j == i else 0) for j, t in enumerate(leaves)]) * dy.double()).sum()
+        want = float((at(1e-4) - at(-1e-4)) / 2e-4)
+        got = float((grad.double() * v).sum())
+        scale = float((grad.double() * v).abs().sum())
+        assert abs(got - want) <= 2e-5 * scale + 1e-6, (what, i, got, want)
+
+
+def _block(x, w1, b1, w2, mod, pos):
+    """One run of the operators together, as a block calls them."""
+    shift, scale, gate = mod.chunk(3, 1)
+    B, N, C = x.shape
+    h = llsa_b200.layer_norm(x, eps=1e-6, scale=scale, shift=shift)
+    h = llsa_b200.rope_axes(h.view(B, N, 2, C // 2).transpose(1, 2), pos, (C // 4, C // 4)).transpose(1, 2).reshape(B, N, C)
+    return llsa_b200.linear(llsa_b200.linear(h, w1, b1, activation="gelu_tanh"), w2, residual=x, gate=gate)
+
+
+def _block_leaves(seed, dtype=BF16, B=2, N=150, C=128):
+    g = gen(seed)
+    leaves = [normal(g, B, N, C, dtype=dtype), normal(g, 4 * C, C, dtype=dtype, std=C ** -0.5), normal(g, 4 * C, dtype=dtype),
+              normal(g, C, 4 * C, dtype=dtype, std=C ** -0.5 / 2), normal(g, B, 3 * C, dtype=dtype, std=0.4)]
+    return leaves, normal(g, B, N, C, dtype=dtype), torch.stack([torch.arange(N, device=DEV) // 16, torch.arange(N, device=DEV) % 16], -1)
+
+
+def _pass(leaves, dy, pos):
+    leaves = [t.detach().requires_grad_(True) for t in leaves]
+    y = _block(*leaves, pos)
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+
+def test_operators_together_against_64_bits():
+    leaves, dy, pos = _block_leaves(41)
+    wide = [t.double().requires_grad_(True) for t in leaves]
+    x, w1, b1, w2, mod = wide
+    shift, scale, gate = mod.chunk(3, 1)
+    B, N, C = x.shape
+    mean = x.mean(-1, keepdim=True)
+    h = (x - mean) / ((x - mean).square().mean(-1, keepdim=True) + 1e-6).sqrt() * (1 + scale[:, None]) + shift[:, None]
+    om = 10000.0 ** (-torch.arange(0, C // 4, 2, device=DEV, dtype=torch.float64) / (C // 4))
+    ang = torch.cat([pos[:, a, None].double() * om for a in range(2)], -1)
+    hh = h.view(B, N, 2, C // 2).transpose(1, 2)
+    e, o = hh[..., 0::2], hh[..., 1::2]
+    h = torch.stack([ang.cos() * e - ang.sin() * o, ang.sin() * e + ang.cos() * o], -1).flatten(-2).transpose(1, 2).reshape(B, N, C)
+    z = h @ w1.T + b1
+    y = x + gate[:, None] * ((z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))) @ w2.T)
+    want = [y.detach(), *torch.autograd.grad(y, wide, dy.double())]
+    # four values rounded to bf16 on the way forward and six on the way back, each 2^-8 of itself at most and independent: in the norm at most 10 of them
+    for name, a, b in zip(["y", "dx", "dw1", "db1", "dw2", "dmod"], _pass(leaves, dy, pos), want):
+        assert float((a.double() - b).norm()) <= 10 * 2.0 ** -8 * float(b.norm()), name
+
+
+def test_same_bits_every_time_on_any_stream_and_in_graphs():
+    sets = [_block_leaves(s) for s in (51, 52)]
+    want = [_pass(*s) for s in sets]
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(_pass(*s), w))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    torch.cuda.synchronize()
+    for _ in range(3):                                            # two streams at once
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i] = _pass(*sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], [None, None]
+    ins = [[t.clone() for t in sets[0][0]], [t.clone() for t in sets[0][0]]]
+    for i in range(2):                                            # two captured graphs, replayed on other inputs, at the same time
+        with torch.cuda.graph(graphs[i]):
+            outs[i] = _pass(ins[i], sets[0][1], sets[0][2])
+    for i in range(2):
+        for t, v in zip(ins[i], sets[i][0]):
+            t.copy_(v)
+    w1 = _pass(sets[1][0], sets[0][1], sets[0][2])
+    torch.cuda.synchronize()
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            graphs[i].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(outs[0], want[0])) and all(torch.equal(p, q) for p, q in zip(outs[1], w1))
+
+
+def test_operators_trace():
+    leaves, dy, pos = _block_leaves(61)
+    want = _pass(leaves, dy, pos)
+    fn = torch.compile(_block, backend="aot_eager", fullgraph=True)
+    leaves = [t.detach().requires_grad_(True) for t in leaves]
+    y = fn(*leaves, pos)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_nothing_to_do(dtype):
+    """No rows: empty results, and gradients of the parameters that are zero."""
+    w, b = torch.ones(24, 16, device=DEV, dtype=dtype, requires_grad=True), torch.ones(24, device=DEV, dtype=dtype, requires_grad=True)
+    for shape in ((0, 5, 16), (3, 0, 16)):
+        x = torch.zeros(shape, device=DEV, dtype=dtype, requires_grad=True)
+        s = torch.ones(shape[0], 16, device=DEV, dtype=dtype, requires_grad=True)
+        lw = torch.ones(16, device=DEV, dtype=dtype, requires_grad=True)
+        y = llsa_b200.layer_norm(x, lw, None, scale=s)
+        assert y.shape == shape
+        for d in torch.autograd.grad(y.sum(), [lw, s]):
+            assert not d.any()
+        gate = torch.ones(shape[0], 24, device=DEV, dtype=dtype, requires_grad=True)
+        y = llsa_b200.linear(x, w, b, residual=torch.zeros(*shape[:2], 24, device=DEV, dtype=dtype), gate=gate)
+        assert y.shape == (*shape[:2], 24)
+        for d, t in zip(torch.autograd.grad(y.sum(), [x, w, b, gate]), (x, w, b, gate)):
+            assert d.shape == t.shape and not d.any()
+    x = torch.zeros(2, 0, 5, 16, device=DEV, dtype=dtype)
+    assert llsa_b200.rope_axes(x, torch.zeros(5, 1, device=DEV), (16,)).shape == x.shape
+
+
+def test_refusals():
+    x, w = torch.zeros(2, 4, 16, device=DEV), torch.zeros(8, 16, device=DEV)
+    r, gate = torch.zeros(2, 4, 8, device=DEV), torch.zeros(2, 8, device=DEV)
+    pos = torch.zeros(4, 1, device=DEV)
+    x4 = torch.zeros(1, 2, 4, 16, device=DEV)
+    for exc, call in [
+        (TypeError, lambda: llsa_b200.linear(x.half(), w.half())), (TypeError, lambda: llsa_b200.linear(x, w.bfloat16())),
+        (TypeError, lambda: llsa_b200.linear(x, w, residual=r.bfloat16())), (TypeError, lambda: llsa_b200.layer_norm(x.half())),
+        (TypeError, lambda: llsa_b200.layer_norm(x, torch.ones(16, device=DEV, dtype=BF16))), (TypeError, lambda: llsa_b200.rope_axes(x4, pos.double(), (16,))),
+        (ValueError, lambda: llsa_b200.linear(x, w, activation="relu")),
+        (RuntimeError, lambda: llsa_b200.linear(x, w.t())), (RuntimeError, lambda: llsa_b200.linear(x, w, torch.zeros(16, device=DEV))),
+        (RuntimeError, lambda: llsa_b200.linear(x, w, residual=r[:1])), (RuntimeError, lambda: llsa_b200.linear(x, w, gate=gate)),
+        (RuntimeError, lambda: llsa_b200.linear(x, w, activation="silu", residual=r, gate=gate)), (RuntimeError, lambda: llsa_b200.linear(x, w, residual=r, gate=gate[:1])),
+        (RuntimeError, lambda: llsa_b200.linear(x, w.cpu())), (RuntimeError, lambda: llsa_b200.layer_norm(x, torch.ones(15, device=DEV))),
+        (RuntimeError, lambda: llsa_b200.layer_norm(x, scale=torch.ones(1, 16, device=DEV))), (RuntimeError, lambda: llsa_b200.layer_norm(x, eps=float("nan"))),
+        (RuntimeError, lambda: llsa_b200.layer_norm(x, eps=-1.0)), (RuntimeError, lambda: llsa_b200.layer_norm(torch.zeros(1, 16385, device=DEV))),
+        (RuntimeError, lambda: llsa_b200.layer_norm(x, torch.ones(16))), (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos, (8, 8))),
+        (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos, (14,))), (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos[:3], (16,))),
+        (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos.repeat(1, 2), (15, 1))), (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos, (16,), theta=0.0)),
+        (RuntimeError, lambda: llsa_b200.rope_axes(x4, pos.requires_grad_(True), (16,))), (RuntimeError, lambda: llsa_b200.rope_axes(x, pos, (16,))),
+    ]:
+        with pytest.raises(exc):
+            call()
+    xg = x.requires_grad_(True)                                   # what cannot be differentiated again says so
+    (d,) = torch.autograd.grad(llsa_b200.linear(xg, w, activation="silu").sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises(NotImplementedError):
+        llsa_b200.layer_norm(fwd.make_dual(x.detach(), torch.ones_like(x)))
+
+
+# ------------------------------------------------------------------------------------------------------ the model
+@pytest.mark.parametrize("attn,fused_rope,side", [("sparse_l2", True, 128), ("sparse_l1", False, 32), ("pixel", True, 16)])
+def test_model_on_the_fused_block_agrees_with_the_eager_block(attn, fused_rope, side):
+    from llsa_b200.dit import RopeDiT
+    torch.manual_seed(1)
+    a = RopeDiT(layers=2, sample_size=side, attn_type=attn, fused_rope=fused_rope).to(DEV)
+    b = RopeDiT(layers=2, sample_size=side, attn_type=attn, fused_rope=fused_rope, fused_block=True).to(DEV)
+    b.load_state_dict(a.state_dict())
+    x, t = torch.randn(2, 3, side, side, device=DEV), torch.tensor([321, 7], device=DEV)
+    out = []
+    for m in (a, b):
+        with torch.autocast("cuda", dtype=BF16):
+            y = m(x, t)
+        y.float().square().mean().backward()
+        out.append(y)
+    # two bf16 evaluations of one model whose selections may differ in a few blocks
+    assert out[0].shape == out[1].shape and float((out[0].float() - out[1].float()).norm()) <= 3e-2 * float(out[0].float().norm())
+    for (n, p), (_, q) in zip(a.named_parameters(), b.named_parameters()):
+        assert torch.isfinite(q.grad).all(), n
+        assert float((p.grad - q.grad).norm()) <= 0.1 * float(p.grad.norm()) + 1e-12, n
+
+
+def test_model_on_the_fused_block_in_fp32():
+    from llsa_b200.dit import RopeDiT
+    torch.manual_seed(2)
+    a = RopeDiT(heads=2, layers=2, sample_size=16, attn_type="pixel").to(DEV)
+    b = RopeDiT(heads=2, layers=2, sample_size=16, attn_type="pixel", fused_block=True).to(DEV)
+    b.load_state_dict(a.state_dict())
+    x, t = torch.randn(2, 3, 16, 16, device=DEV), torch.tensor([321, 7], device=DEV)
+    ya, yb = a(x, t), b(x, t)
+    ya.square().mean().backward()
+    yb.square().mean().backward()
+    assert float((ya - yb).norm()) <= 1e-5 * float(ya.norm())
+    for (n, p), (_, q) in zip(a.named_parameters(), b.named_parameters()):
+        assert float((p.grad - q.grad).norm()) <= 1e-4 * float(p.grad.norm()) + 1e-12, n
