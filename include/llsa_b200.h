@@ -176,7 +176,7 @@ typedef struct LlsaLinearArgs {
   int32_t* status;
 } LlsaLinearArgs;
 int llsa_linear_fwd(const LlsaLinearArgs* args, void* stream);
-/* Read from the shapes of x, weight and gate, the activation and which results are wanted; -1 where these are refused */
+/* Read from the shapes of x, weight and gate, dy, the activation and which results are wanted; -1 where these are refused */
 int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* args);
 int llsa_linear_bwd(const LlsaLinearArgs* args, void* stream);
 

@@ -3,7 +3,8 @@
 //
 //   z = x w^T + bias,  dz = dy gate_b act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum dz,  dgate_b = sum_n dy z,  dresidual = dy
 //
-// This file: checks, the choice of kernels, and the passes around the products (dz and its column sums, the sum of a split product's parts).
+// This file: checks, the products of fp32 data, and the passes around the products (dz and its column sums, the sum of a split product's parts).  bf16 data:
+// linear_tc.cu.
 #include <string.h>
 
 #include "linear.cuh"
@@ -18,15 +19,14 @@ using bf16 = __nv_bfloat16;
 // fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of 256 threads owns a tile of
 // 16 TM x 16 TM outputs, a thread TM x TM of them (two groups of TM / 2 rows and columns, so that a warp's reads of shared memory are whole
 // vectors); steps of 16 along k, the next step's operands on their way in registers while this one's are multiplied.
-template <typename T>
-__device__ __forceinline__ void fetch(const Mat<const T>& m, int along_k, int64_t row0, int64_t rows, int64_t k0, int64_t k1, int r, int k, float& v) {
+__device__ __forceinline__ void fetch(const Mat<const float>& m, int along_k, int64_t row0, int64_t rows, int64_t k0, int64_t k1, int r, int k, float& v) {
   const int64_t i = row0 + r, kk = k0 + k;
-  v = i < rows && kk < k1 ? to_f32<T>(along_k ? m.p[i * m.ld + kk] : m.p[kk * m.ld + i]) : 0.f;
+  v = i < rows && kk < k1 ? along_k ? m.p[i * m.ld + kk] : m.p[kk * m.ld + i] : 0.f;
 }
 
-template <typename T, int TM, bool PARTIAL>
+template <int TM, bool PARTIAL>
 __global__ void __launch_bounds__(256)
-product_kernel(Product<T> p, Epilogue<T> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split) {
+product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split) {
   constexpr int BM = 16 * TM, BK = 16, LD = BM + 4, NV = BM * BK / 256;
   __shared__ float s_a[2][BK][LD], s_b[2][BK][LD];
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
@@ -93,22 +93,19 @@ product_kernel(Product<T> p, Epilogue<T> e, float* __restrict__ partial, int64_t
       if constexpr (PARTIAL) {
         partial[(blockIdx.y * p.M + r) * partial_ld + c] = acc[i][j];
       } else {
-        float z = acc[i][j] + (e.bias ? to_f32<T>(e.bias[c]) : 0.f);
-        if (e.pre.p) {
-          if (sizeof(T) == 2 && e.act != kActNone) reinterpret_cast<uint16_t*>(e.pre.p)[r * e.pre.ld + c] = half_bits(z);
-          else e.pre.p[r * e.pre.ld + c] = from_f32<T>(z);
-        }
-        z = activate<sizeof(T) == 2>(z, e.act);
-        if (e.gate.p) z *= to_f32<T>(e.gate.p[sample * e.gate.ld + c]);
-        if (e.residual.p) z += to_f32<T>(e.residual.p[r * e.residual.ld + c]);
-        e.y.p[r * e.y.ld + c] = from_f32<T>(z);
+        float z = acc[i][j] + (e.bias ? e.bias[c] : 0.f);
+        if (e.pre.p) e.pre.p[r * e.pre.ld + c] = z;
+        z = activate<false>(z, e.act);
+        if (e.gate.p) z *= e.gate.p[sample * e.gate.ld + c];
+        if (e.residual.p) z += e.residual.p[r * e.residual.ld + c];
+        e.y.p[r * e.y.ld + c] = z;
       }
     }
   }
 }
 
-template <typename T, bool PARTIAL>
-int launch_product(const Product<T>& p, const Epilogue<T>& e, float* partial, int64_t ld, cudaStream_t st) {
+template <bool PARTIAL>
+int launch_product(const Product<float>& p, const Epilogue<float>& e, float* partial, int64_t ld, cudaStream_t st) {
   const int64_t split = PARTIAL ? p.split : 1;
   auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
   const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
@@ -116,9 +113,9 @@ int launch_product(const Product<T>& p, const Epilogue<T>& e, float* partial, in
     launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(256), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per);
   };
   LLSA_REQUIRE(tiles(32) <= INT32_MAX, LLSA_ERR_SHAPE, "linear: too many outputs");
-  if (tiles(128) * split >= 148) go(product_kernel<T, 8, PARTIAL>, 128);
-  else if (tiles(64) * split >= 148) go(product_kernel<T, 4, PARTIAL>, 64);
-  else go(product_kernel<T, 2, PARTIAL>, 32);
+  if (tiles(128) * split >= 148) go(product_kernel<8, PARTIAL>, 128);
+  else if (tiles(64) * split >= 148) go(product_kernel<4, PARTIAL>, 64);
+  else go(product_kernel<2, PARTIAL>, 32);
   LLSA_LAUNCH_OK("product_kernel");
   return LLSA_OK;
 }
@@ -195,6 +192,8 @@ int check_matrix(const LlsaTensor* t, const char* name, int dtype, int64_t rows,
   return LLSA_OK;
 }
 
+bool rows16(const LlsaTensor* t) { return (uintptr_t) t->ptr % 16 == 0 && (t->shape[0] == 1 || t->stride[0] * (int64_t) dtype_size(t->dtype) % 16 == 0); }
+
 struct Plan {
   int64_t M, K, F, B, N;       // rows, input and output features, samples (1 without a gate), rows of a sample
   int dtype;
@@ -217,6 +216,7 @@ int check_common(const LlsaLinearArgs* a, Plan* p) {
   LLSA_REQUIRE(p->M <= INT32_MAX, LLSA_ERR_SHAPE, "linear: more than 2^31 - 1 rows");
   int rc;
   if ((rc = check_matrix(a->x, "x", p->dtype, p->M, p->K)) || (rc = check_matrix(a->weight, "weight", p->dtype, p->F, p->K))) return rc;
+  if (p->dtype == LLSA_BF16) LLSA_REQUIRE(rows16(a->x) && rows16(a->weight), LLSA_ERR_STRIDE, "linear: rows of x and weight must start on 16-byte boundaries");
   LLSA_REQUIRE(a->activation >= kActNone && a->activation <= kActSilu, LLSA_ERR_ARG, "linear: activation %d is not known", a->activation);
   p->B = 1;
   if (a->gate) {
@@ -238,7 +238,8 @@ int check_common(const LlsaLinearArgs* a, Plan* p) {
 // What the backward does, from the shapes and from which results are asked for
 void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   const int es = (int) dtype_size(p->dtype);
-  p->write_dz = a->activation != kActNone || a->gate;
+  // dy itself is dz without an activation and a gate, where the tensor cores can read it
+  p->write_dz = a->activation != kActNone || a->gate || (p->dtype == LLSA_BF16 && !(a->dy && rows16(a->dy)));
   p->sums = a->dbias || a->dgate;
   p->dz_ld = (p->F + 7) / 8 * 8;
   // columns in groups of 32: enough CTAs along the rows for 148 x 4 of them, 32 rows each or more
@@ -247,8 +248,8 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
   p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
-  p->split = (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
-  p->part_ld = p->K;
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
+  p->part_ld = (p->K + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -265,15 +266,19 @@ template <typename T>
 Mat<T> mat(const LlsaTensor* t) {
   Mat<T> m;
   m.p = t ? (T*) t->ptr : nullptr;
-  m.ld = t ? t->stride[0] : 0;
+  m.ld = !t ? 0 : t->shape[0] == 1 ? (t->shape[1] + 7) / 8 * 8 : t->stride[0];      // one row: a stride that a tensor map takes
   return m;
 }
 
-template <typename T>
-int product(const Product<T>& p, const Epilogue<T>& e, cudaStream_t st) { return launch_product<T, false>(p, e, nullptr, 0, st); }
-template <typename T>
-int product_parts(const Product<T>& p, float* partial, int64_t ld, cudaStream_t st) {
-  return launch_product<T, true>(p, Epilogue<T>{}, partial, ld, st);
+int product(const Product<float>& p, const Epilogue<float>& e, const LlsaLinearArgs*, cudaStream_t st) { return launch_product<false>(p, e, nullptr, 0, st); }
+int product(const Product<bf16>& p, const Epilogue<bf16>& e, const LlsaLinearArgs* a, cudaStream_t st) {
+  return linear_tc_product(p, e, a->wait_limit, a->status, st);
+}
+int product_parts(const Product<float>& p, float* partial, int64_t ld, const LlsaLinearArgs*, cudaStream_t st) {
+  return launch_product<true>(p, Epilogue<float>{}, partial, ld, st);
+}
+int product_parts(const Product<bf16>& p, float* partial, int64_t ld, const LlsaLinearArgs* a, cudaStream_t st) {
+  return linear_tc_parts(p, partial, ld, a->wait_limit, a->status, st);
 }
 
 template <typename T>
@@ -286,7 +291,7 @@ int forward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   e.y = mat<T>(a->y);
   e.pre = mat<T>(a->pre);
   e.act = a->activation;
-  return product<T>({mat<const T>(a->x), mat<const T>(a->weight), 1, 1, p.M, p.F, p.K, 1}, e, st);
+  return product(Product<T>{mat<const T>(a->x), mat<const T>(a->weight), 1, 1, p.M, p.F, p.K, 1}, e, a, st);
 }
 
 template <typename T>
@@ -321,12 +326,12 @@ int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   if (a->dx) {
     Epilogue<T> e = {};
     e.y = mat<T>(a->dx);
-    const int rc = product<T>({dz, mat<const T>(a->weight), 1, 0, p.M, p.K, p.F, 1}, e, st);
+    const int rc = product(Product<T>{dz, mat<const T>(a->weight), 1, 0, p.M, p.K, p.F, 1}, e, a, st);
     if (rc) return rc;
   }
   if (a->dweight) {
     float* parts = (float*) (ws + p.o_parts);
-    const int rc = product_parts<T>({dz, mat<const T>(a->x), 0, 0, p.F, p.K, p.M, p.split}, parts, p.part_ld, st);
+    const int rc = product_parts(Product<T>{dz, mat<const T>(a->x), 0, 0, p.F, p.K, p.M, p.split}, parts, p.part_ld, a, st);
     if (rc) return rc;
     const int64_t blocks = std::min<int64_t>((p.F * p.K + 255) / 256, 148 * 8);
     launch_pdl(sum_parts_kernel<T>, dim3((unsigned) blocks), dim3(256), 0, st, (const float*) parts, p.part_ld, p.split, p.F, p.K, (T*) a->dweight->ptr);

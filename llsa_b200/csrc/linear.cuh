@@ -67,4 +67,10 @@ struct Product {
   int split;                   // parts of the sum over k, one after another in `partial` (linear_sum_parts adds them); 1: none
 };
 
+// bf16, on tcgen05 (linear_tc.cu).  Operands: rows on 16-byte boundaries.  The forward and the input's gradient (A along k), with their epilogue;
+int linear_tc_product(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, int wait_limit, int32_t* status, cudaStream_t st);
+// the weight's gradient (both operands across), in p.split parts of [M][ld], ld a multiple of 8; the number of parts to take
+int linear_tc_parts(const Product<__nv_bfloat16>& p, float* partial, int64_t ld, int wait_limit, int32_t* status, cudaStream_t st);
+int linear_tc_split(int64_t M, int64_t N, int64_t K);
+
 }  // namespace llsa
