@@ -166,6 +166,12 @@ Tensor matrix(const Tensor& t, int64_t M, int64_t C, bool aligned) {
   return c;
 }
 
+// A vector, dense and on a 16-byte boundary
+Tensor aligned_vector(const Tensor& t) {
+  const Tensor c = cont(t);
+  return (uintptr_t) c.data_ptr() % 16 ? c.clone() : c;
+}
+
 struct Shape {
   int64_t M, K, F, B;
   Shape(const Tensor& x, const Tensor& w, const Tensor& gate) {
@@ -219,7 +225,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
   a.x = &xd; a.weight = &wd; a.y = &yd;
   Tensor b, r, g;
   LlsaTensor bd, rd, gd, pd;
-  if (b_.defined()) { b = cont(b_); bd = desc(b); a.bias = &bd; }
+  if (b_.defined()) { b = aligned_vector(b_); bd = desc(b); a.bias = &bd; }
   if (r_.defined()) { r = matrix(r_, s.M, s.F, false); rd = desc(r); a.residual = &rd; }
   if (g_.defined()) { g = unit_columns(g_); gd = desc(g); a.gate = &gd; }
   if (want_pre) { pd = desc(out[1]); a.pre = &pd; }
@@ -231,12 +237,13 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
 }
 
 // want: 1 x, 2 weight, 4 bias, 8 gate; the gradients asked for, in that order
-std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& w_, const OptTensor& pre, const OptTensor& gate, int64_t act,
-                               int64_t want) {
-  const Tensor p_ = or_none(pre), g_ = or_none(gate);
-  same_device(x_, {dy_, w_, p_, g_});
+std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& w_, const OptTensor& bias, const OptTensor& pre, const OptTensor& gate,
+                               int64_t act, int64_t want) {
+  const Tensor b_ = or_none(bias), p_ = or_none(pre), g_ = or_none(gate);
+  same_device(x_, {dy_, w_, b_, p_, g_});
   check_float({&x_, &w_, &dy_});
-  if (g_.defined()) check_float({&x_, &g_});
+  for (const Tensor& t : {b_, p_, g_})
+    if (t.defined()) check_float({&x_, &t});
   const Shape s(x_, w_, g_);
   TORCH_CHECK(dy_.sizes() == at::IntArrayRef(with_last(x_, s.F)), "llsa_b200.linear_bwd: dy must be ", at::IntArrayRef(with_last(x_, s.F)), ", got ",
               dy_.sizes());
@@ -255,8 +262,14 @@ std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor
   LlsaLinearArgs a = linear_args(act, status);
   const LlsaTensor xd = desc(x), wd = desc(w), dyd = desc(dy);
   a.x = &xd; a.weight = &wd; a.dy = &dyd;
-  Tensor g;
-  LlsaTensor gd, pd, o[4];
+  Tensor b, g;
+  LlsaTensor bd, gd, pd, o[4];
+  if (b_.defined()) {
+    TORCH_CHECK(b_.dim() == 1 && b_.size(0) == s.F, "llsa_b200: bias must be [F]");
+    b = aligned_vector(b_);
+    bd = desc(b);
+    a.bias = &bd;
+  }
   if (g_.defined()) { g = unit_columns(g_); gd = desc(g); a.gate = &gd; }
   if (p_.defined()) {
     TORCH_CHECK(p_.dim() == 2 && p_.size(0) == s.M && p_.size(1) == s.F && p_.is_contiguous(), "llsa_b200.linear_bwd: `pre` is not from the matching linear_fwd");
@@ -317,7 +330,7 @@ using NormFwd = std::vector<Tensor>(const Tensor&, const OptTensor&, const OptTe
 using NormBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Tensor&, int64_t, at::ScalarType,
                                     at::ScalarType);
 using LinearFwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool);
-using LinearBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, int64_t, int64_t);
+using LinearBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, int64_t);
 using Rope = Tensor(const Tensor&, const Tensor&, at::IntArrayRef, double, bool);
 const auto& norm_fwd_op() { return op<NormFwd>("llsa_b200::layer_norm_fwd"); }
 const auto& norm_bwd_op() { return op<NormBwd>("llsa_b200::layer_norm_bwd"); }
@@ -381,8 +394,8 @@ std::vector<Tensor> layer_norm_autograd(const Tensor& x, const OptTensor& w, con
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r,
                                const OptTensor& gate, int64_t act) {
-    // z is kept where an activation's slope or a gate's gradient will ask for it
-    const bool pre = act != LLSA_ACT_NONE || (gate && gate->requires_grad());
+    // z is kept where a gate's gradient or, of fp32 data, an activation's slope will ask for it
+    const bool pre = (act != LLSA_ACT_NONE && x.scalar_type() == at::kFloat) || (gate && gate->requires_grad());
     variable_list out;
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -390,27 +403,26 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     }
     ctx->set_materialize_grads(false);
     if (pre) ctx->mark_non_differentiable({out[1]});
-    ctx->save_for_backward({x, w, pre ? out[1] : Tensor(), or_none(gate)});
+    ctx->save_for_backward({x, w, pre ? out[1] : Tensor(), or_none(gate), or_none(b)});
     ctx->saved_data["act"] = act;
-    ctx->saved_data["given"] = (int64_t) ((b ? 1 : 0) | (r ? 2 : 0));
+    ctx->saved_data["residual"] = r.has_value();
     return out;
   }
   static variable_list backward(torch::autograd::AutogradContext* ctx, variable_list grads) {
     variable_list g(6);
     if (!grads[0].defined()) return g;
     const variable_list s = ctx->get_saved_variables();
-    const int64_t given = ctx->saved_data["given"].toInt(), act = ctx->saved_data["act"].toInt();
+    const int64_t act = ctx->saved_data["act"].toInt();
     Edges e{ctx};
-    const Tensor& there = s[0];
     int64_t want = 0;
     if (e.wants(s[0])) want |= 1;
     if (e.wants(s[1])) want |= 2;
-    if (e.wants(given & 1 ? there : Tensor())) want |= 4;
-    const bool want_residual = e.wants(given & 2 ? there : Tensor());
+    if (e.wants(s[4])) want |= 4;
+    const bool want_residual = e.wants(ctx->saved_data["residual"].toBool() ? s[0] : Tensor());
     if (e.wants(s[3])) want |= 8;
     if (want) {
       const std::vector<Tensor> r =
-          below_unless_recorded([&] { return linear_bwd_op().call(grads[0], s[0], s[1], opt(s[2]), opt(s[3]), act, want); });
+          below_unless_recorded([&] { return linear_bwd_op().call(grads[0], s[0], s[1], opt(s[4]), opt(s[2]), opt(s[3]), act, want); });
       size_t at = 0;
       if (want & 1) g[0] = r[at++];
       if (want & 2) g[1] = r[at++];
@@ -467,7 +479,7 @@ TORCH_LIBRARY_FRAGMENT(llsa_b200, m) {
   m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor stats, int want, ScalarType shift_type, "
         "ScalarType bias_type) -> Tensor[]");
   m.def("linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, int activation, bool want_pre) -> Tensor[]");
-  m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, Tensor? pre, Tensor? gate, int activation, int want) -> Tensor[]");
+  m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, Tensor? bias, Tensor? pre, Tensor? gate, int activation, int want) -> Tensor[]");
   m.def("rope_axes(Tensor x, Tensor positions, int[] axes_dims, float theta, bool inverse) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(llsa_b200, CUDA, m) {

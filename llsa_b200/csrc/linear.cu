@@ -95,7 +95,7 @@ product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial,
       } else {
         float z = acc[i][j] + (e.bias ? e.bias[c] : 0.f);
         if (e.pre.p) e.pre.p[r * e.pre.ld + c] = z;
-        z = activate<false>(z, e.act);
+        z = activate(z, e.act);
         if (e.gate.p) z *= e.gate.p[sample * e.gate.ld + c];
         if (e.residual.p) z += e.residual.p[r * e.residual.ld + c];
         e.y.p[r * e.y.ld + c] = z;
@@ -121,51 +121,91 @@ int launch_product(const Product<float>& p, const Epilogue<float>& e, float* par
 }
 
 // ------------------------------------------------------------------------------------------------ dz and its column sums
-// dz = dy gate act'(z) and, per column and part of a sample's rows, P = sum dy z and S = sum dz (column_sums.cuh).  A thread owns a column of 32 rows apart..
+// dz = dy gate act'(z) and, per column and part of a sample's rows, P = sum dy z and S = sum dz (column_sums.cuh).  bf16 data: act' by linear_tc_slope.  A
+// thread owns V neighbouring columns and every (256 / tx)th row of its CTA's; U rows are on their way at once.
 template <typename T>
 struct FrontArgs {
   Mat<const T> dy, pre, gate;
   Mat<T> dz;                   // p NULL: not written
   float* partial;              // NULL: no sums
   uint32_t N, chunks, per;     // rows of a sample, CTAs along them, rows of a CTA
-  int F, act;
+  int F, act, tx;              // tx: threads along the columns, a power of two
+};
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Piece {
+  T v[V];
 };
 
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 linear_dz_kernel(FrontArgs<T> a) {
-  __shared__ float s_sum[2][8][33];
-  const int col = threadIdx.x % 32, lane = threadIdx.x / 32, c = blockIdx.y * 32 + col;
+  constexpr int U = 4;
+  using P = Piece<T, V>;
+  extern __shared__ float s_part[];                        // [2][256 / tx][tx * V]
+  const int tx = a.tx, lanes = 256 / tx, col = threadIdx.x % tx, lane = threadIdx.x / tx, c = (blockIdx.y * tx + col) * V;
   const uint32_t b = blockIdx.x / a.chunks, first = (blockIdx.x - b * a.chunks) * a.per, end = min(a.N, first + a.per);
   pdl_wait();
   pdl_trigger();
-  float p = 0.f, s = 0.f;
+  float p[V], s[V], gate[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) p[i] = s[i] = 0.f;
   if (c < a.F) {
-    const float gate = a.gate.p ? to_f32<T>(a.gate.p[b * a.gate.ld + c]) : 1.f;
-    for (uint32_t n = first + lane; n < end; n += 8) {
-      const int64_t r = (int64_t) b * a.N + n;
-      const float dy = to_f32<T>(a.dy.p[r * a.dy.ld + c]);
-      float dz = dy * gate;
-      if (a.pre.p) {
-        const T raw = a.pre.p[r * a.pre.ld + c];
-        const float z = sizeof(T) == 2 && a.act != kActNone ? half_value(*reinterpret_cast<const uint16_t*>(&raw)) : to_f32<T>(raw);
-        p = fmaf(dy, z, p);
-        dz *= activate_grad<sizeof(T) == 2>(z, a.act);
-      }
-      s += dz;
-      if (a.dz.p) a.dz.p[r * a.dz.ld + c] = from_f32<T>(dz);
+#pragma unroll
+    for (int i = 0; i < V; ++i) gate[i] = a.gate.p ? to_f32<T>(a.gate.p[b * a.gate.ld + c + i]) : 1.f;
+    for (uint32_t n0 = first + lane; n0 < end; n0 += U * lanes) {
+      P dy[U], pre[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (n0 + u * lanes < end) {
+          const int64_t r = (int64_t) b * a.N + n0 + u * lanes;
+          dy[u] = *reinterpret_cast<const P*>(a.dy.p + r * a.dy.ld + c);
+          if (a.pre.p) pre[u] = *reinterpret_cast<const P*>(a.pre.p + r * a.pre.ld + c);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (n0 + u * lanes < end) {
+          P dz;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float g = to_f32<T>(dy[u].v[i]);
+            float d = __fmul_rn(g, gate[i]);      // never contracted: the sums' bits do not depend on what else is asked for
+            if (a.pre.p) {
+              const float z = to_f32<T>(pre[u].v[i]);
+              p[i] = fmaf(g, z, p[i]);
+              if constexpr (sizeof(T) == 4) d *= activate_grad(z, a.act);
+            }
+            s[i] = __fadd_rn(s[i], d);
+            dz.v[i] = from_f32<T>(d);
+          }
+          if (a.dz.p) *reinterpret_cast<P*>(a.dz.p + ((int64_t) b * a.N + n0 + u * lanes) * a.dz.ld + c) = dz;
+        }
     }
   }
   if (!a.partial) return;
-  s_sum[0][lane][col] = p;
-  s_sum[1][lane][col] = s;
-  __syncthreads();
-  if (lane < 2 && c < a.F) {
-    float u = 0.f;
+  const int width = tx * V;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u += s_sum[lane][k][col];
-    a.partial[((int64_t) blockIdx.x * 2 + lane) * a.F + c] = u;
+  for (int i = 0; i < V; ++i) {
+    s_part[lane * width + col * V + i] = p[i];
+    s_part[(lanes + lane) * width + col * V + i] = s[i];
   }
+  __syncthreads();
+  for (int k = threadIdx.x; k < 2 * width; k += 256) {
+    const int which = k / width, at = k - which * width;
+    if (blockIdx.y * width + at >= a.F) continue;
+    float u = 0.f;
+    for (int j = 0; j < lanes; ++j) u += s_part[(which * lanes + j) * width + at];
+    a.partial[((int64_t) blockIdx.x * 2 + which) * a.F + blockIdx.y * width + at] = u;
+  }
+}
+
+template <typename T, int V>
+int launch_dz(FrontArgs<T>& f, int64_t blocks, int tx, cudaStream_t st) {
+  f.tx = tx;
+  const int64_t cols = (f.F + tx * V - 1) / (tx * V);
+  LLSA_REQUIRE(blocks <= INT32_MAX && cols <= 65535, LLSA_ERR_SHAPE, "linear_bwd: too many samples or features");
+  launch_pdl(linear_dz_kernel<T, V>, dim3((unsigned) blocks, (unsigned) cols), dim3(256), (size_t) (f.partial ? 2 * 256 * V * 4 : 0), st, f);
+  LLSA_LAUNCH_OK("linear_dz_kernel");
+  return LLSA_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ parts of a split product
@@ -198,6 +238,8 @@ struct Plan {
   int64_t M, K, F, B, N;       // rows, input and output features, samples (1 without a gate), rows of a sample
   int dtype;
   bool write_dz, sums;         // the pass over dy: leaves dz / column sums
+  bool slope;                  // bf16 with an activation: that pass is a product
+  int vec, tx;                 // its columns of a thread, threads along the columns
   int64_t dz_ld, chunks, per;
   int split;
   int64_t part_ld;
@@ -228,6 +270,8 @@ int check_common(const LlsaLinearArgs* a, Plan* p) {
     p->B = std::max<int64_t>(1, a->gate->shape[0]);
   }
   p->N = p->M / p->B;
+  const int64_t bs[1] = {p->F};
+  if (a->bias && (rc = check_contig(a->bias, "bias", p->dtype, 1, bs))) return rc;
   if (a->pre) {
     const int64_t s[2] = {p->M, p->F};
     if ((rc = check_contig(a->pre, "pre", p->dtype, 2, s))) return rc;
@@ -242,11 +286,25 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   p->write_dz = a->activation != kActNone || a->gate || (p->dtype == LLSA_BF16 && !(a->dy && rows16(a->dy)));
   p->sums = a->dbias || a->dgate;
   p->dz_ld = (p->F + 7) / 8 * 8;
-  // columns in groups of 32: enough CTAs along the rows for 148 x 4 of them, 32 rows each or more
-  const int64_t cols = (p->F + 31) / 32;
-  p->chunks = std::max<int64_t>(1, std::min((148 * 4 + cols * p->B - 1) / (cols * p->B), (p->N + 31) / 32));
-  p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
-  p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
+  p->slope = p->dtype == LLSA_BF16 && a->activation != kActNone;
+  if (p->slope) {
+    p->chunks = linear_tc_slope_groups(p->M, p->F);
+  } else {
+    // a CTA: tx threads along the columns, the width of 16, 32 or 64 that leaves the fewest idle; enough CTAs along the rows for 148 x 6, 16 rows a thread or more
+    p->vec = p->F % 8 == 0 && a->dy && rows16(a->dy) ? 16 / es : 1;
+    int64_t idle = INT64_MAX;
+    for (int tx : {64, 32, 16}) {
+      const int64_t w = tx * p->vec, left = (p->F + w - 1) / w * w;
+      if (left < idle) {
+        idle = left;
+        p->tx = tx;
+      }
+    }
+    const int64_t cols = (p->F + p->tx * p->vec - 1) / (p->tx * p->vec), lanes = 256 / p->tx;
+    p->chunks = std::max<int64_t>(1, std::min((148 * 6 + cols * p->B - 1) / (cols * p->B), (p->N + 16 * lanes - 1) / (16 * lanes)));
+    p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
+    p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
+  }
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
   p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
   p->part_ld = (p->K + 7) / 8 * 8;
@@ -294,6 +352,16 @@ int forward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   return product(Product<T>{mat<const T>(a->x), mat<const T>(a->weight), 1, 1, p.M, p.F, p.K, 1}, e, a, st);
 }
 
+int slope(const LlsaLinearArgs* a, const Plan& p, const Mat<bf16>& dz, float* sums, cudaStream_t st) {
+  Epilogue<bf16> e = {};
+  e.bias = a->bias ? (const bf16*) a->bias->ptr : nullptr;
+  e.y = dz;
+  e.act = a->activation;
+  return linear_tc_slope(Product<bf16>{mat<const bf16>(a->x), mat<const bf16>(a->weight), 1, 1, p.M, p.F, p.K, 1}, e, mat<const bf16>(a->dy), sums, a->wait_limit,
+                         a->status, st);
+}
+int slope(const LlsaLinearArgs*, const Plan&, const Mat<float>&, float*, cudaStream_t) { return LLSA_ERR_ARG; }      // not asked for
+
 template <typename T>
 int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   char* ws = (char*) a->workspace;
@@ -301,8 +369,6 @@ int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   if (p.write_dz || p.sums) {
     FrontArgs<T> f = {};
     f.dy = dz;
-    f.pre = mat<const T>(a->pre);
-    f.gate = mat<const T>(a->gate);
     if (p.write_dz) {
       f.dz.p = (T*) (ws + p.o_dz);
       f.dz.ld = p.dz_ld;
@@ -310,16 +376,22 @@ int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
       dz.ld = f.dz.ld;
     }
     f.partial = p.sums ? (float*) (ws + p.o_cols) : nullptr;
-    f.N = (uint32_t) p.N; f.chunks = (uint32_t) p.chunks; f.per = (uint32_t) p.per;
-    f.F = (int) p.F;
-    f.act = a->activation;
-    LLSA_REQUIRE(p.B * p.chunks <= INT32_MAX, LLSA_ERR_SHAPE, "linear_bwd: too many samples");
-    launch_pdl(linear_dz_kernel<T>, dim3((unsigned) (p.B * p.chunks), (unsigned) ((p.F + 31) / 32)), dim3(256), 0, st, f);
-    LLSA_LAUNCH_OK("linear_dz_kernel");
+    int rc;
+    if (p.slope) {
+      rc = slope(a, p, f.dz, f.partial, st);
+    } else {
+      if (a->activation != kActNone || a->dgate) f.pre = mat<const T>(a->pre);
+      f.gate = mat<const T>(a->gate);
+      f.N = (uint32_t) p.N; f.chunks = (uint32_t) p.chunks; f.per = (uint32_t) p.per;
+      f.F = (int) p.F;
+      f.act = a->activation;
+      rc = p.vec > 1 ? launch_dz<T, 16 / sizeof(T)>(f, p.B * p.chunks, p.tx, st) : launch_dz<T, 1>(f, p.B * p.chunks, p.tx, st);
+    }
+    if (rc) return rc;
     if (p.sums) {
       const ParamView none = {nullptr, 0, 0};
-      const int rc = finish_column_grads(f.partial, p.B, p.chunks, p.F, none, none, none,
-                                         {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
+      rc = finish_column_grads(f.partial, p.B, p.chunks, p.F, none, none, none,
+                               {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
       if (rc) return rc;
     }
   }
@@ -349,8 +421,6 @@ extern "C" int llsa_linear_fwd(const LlsaLinearArgs* a, void* stream) {
   Plan p;
   int rc = check_common(a, &p);
   if (rc) return rc;
-  const int64_t bs[1] = {p.F};
-  if (a->bias && (rc = check_contig(a->bias, "bias", p.dtype, 1, bs))) return rc;
   if (a->residual && (rc = check_matrix(a->residual, "residual", p.dtype, p.M, p.F))) return rc;
   LLSA_REQUIRE(!a->gate || a->residual, LLSA_ERR_ARG, "linear: a gate goes with a residual");
   if ((rc = check_matrix(a->y, "y", p.dtype, p.M, p.F))) return rc;
@@ -371,7 +441,7 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
   if (rc) return rc;
   plan_bwd(a, &p);
   if ((rc = check_matrix(a->dy, "dy", p.dtype, p.M, p.F))) return rc;
-  LLSA_REQUIRE(a->pre || (a->activation == kActNone && !a->dgate), LLSA_ERR_NULL, "pre: null tensor");
+  LLSA_REQUIRE(a->pre || !(a->dgate || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
   if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;
   const int64_t ws[2] = {p.F, p.K}, gs[2] = {p.B, p.F}, bs[1] = {p.F};
   if (a->dweight && (rc = check_contig(a->dweight, "dweight", p.dtype, 2, ws))) return rc;

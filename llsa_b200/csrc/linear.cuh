@@ -1,7 +1,5 @@
 // What the projection's kernels share: the epilogue's operands, the activations, and the interface between linear.cu and the matrix products.
 #pragma once
-#include <cuda_fp16.h>
-
 #include "column_sums.cuh"
 #include "common.cuh"
 
@@ -16,8 +14,7 @@ struct Mat {
   int64_t ld;
 };
 
-// What stands behind the product z of a forward: y = residual + gate act(z + bias); `pre`, if given, keeps z + bias for the backward
-// (T; with an activation and bf16 data a half-precision float).
+// What stands behind the product z of a forward: y = residual + gate act(z + bias); `pre`, if given, keeps z + bias for the backward.
 template <typename T>
 struct Epilogue {
   const T* bias;
@@ -29,34 +26,24 @@ struct Epilogue {
   int act;
 };
 
-// 1 / (1 + e^-t).  FAST: two ulp of fp32 and what the argument's scaling by log2(e) costs, 2^-22 at |t| = 4: far below a bf16 step.
-template <bool FAST>
-__device__ __forceinline__ float sigmoid(float t) {
-  return FAST ? __fdividef(1.f, 1.f + __expf(-t)) : 1.f / (1.f + expf(-t));
-}
 constexpr float kGelu2 = 1.5957691216057308f, kGelu3 = 0.044715f;      // 2 sqrt(2 / pi)
+// 1 / (1 + e^-t)
+__device__ __forceinline__ float sigmoid(float t) { return 1.f / (1.f + expf(-t)); }
 // gelu_tanh: z (1 + tanh(u)) / 2 = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3): no cancellation for negative z
-template <bool FAST>
 __device__ __forceinline__ float activate(float z, int act) {
-  if (act == kActGeluTanh) return z * sigmoid<FAST>(kGelu2 * z * fmaf(kGelu3 * z, z, 1.f));
-  if (act == kActSilu) return z * sigmoid<FAST>(z);
+  if (act == kActGeluTanh) return z * sigmoid(kGelu2 * z * fmaf(kGelu3 * z, z, 1.f));
+  if (act == kActSilu) return z * sigmoid(z);
   return z;
 }
 // The derivative; beyond |z| = 1e4 it is 0 or 1, and z^2 and an infinite z are kept out of its products with 0
-template <bool FAST>
 __device__ __forceinline__ float activate_grad(float z, int act) {
   if (act == kActNone) return 1.f;
   if (fabsf(z) > 1e4f) z = copysignf(1e4f, z);
   const bool gelu = act == kActGeluTanh;
-  const float q = z * z, s = sigmoid<FAST>(gelu ? kGelu2 * z * fmaf(kGelu3, q, 1.f) : z);
+  const float q = z * z, s = sigmoid(gelu ? kGelu2 * z * fmaf(kGelu3, q, 1.f) : z);
   const float du = gelu ? kGelu2 * fmaf(3.f * kGelu3, q, 1.f) : 1.f;
   return fmaf(z * s * (1.f - s), du, s);
 }
-
-// What the backward of an activation reads back of z: bf16 data keep it as a half-precision float, in the same 16 bits.  Its rounding (2^-11) adds an eighth
-// of a bf16 step to the gradient, where z in bf16 would add a whole one; what leaves the range becomes infinite, where the derivative is 0 or 1.
-__device__ __forceinline__ uint16_t half_bits(float z) { return __half_as_ushort(__float2half_rn(z)); }
-__device__ __forceinline__ float half_value(uint16_t b) { return __half2float(__ushort_as_half(b)); }
 
 // D[i, j] = sum_k A(i, k) B(j, k), k < K.  a_k: A(i, k) at a.p[i * ld + k] (else at a.p[k * ld + i]); b_k alike.
 template <typename T>
@@ -69,6 +56,10 @@ struct Product {
 
 // bf16, on tcgen05 (linear_tc.cu).  Operands: rows on 16-byte boundaries.  The forward and the input's gradient (A along k), with their epilogue;
 int linear_tc_product(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, int wait_limit, int32_t* status, cudaStream_t st);
+// dz = dy act'(z) with z computed once more, e.y = dz (rows on 16-byte boundaries), and the column sums of dz: sums[group][1][N], linear_tc_slope_groups of them;
+int linear_tc_slope(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, const Mat<const __nv_bfloat16>& dy, float* sums, int wait_limit,
+                    int32_t* status, cudaStream_t st);
+int64_t linear_tc_slope_groups(int64_t M, int64_t N);
 // the weight's gradient (both operands across), in p.split parts of [M][ld], ld a multiple of 8; the number of parts to take
 int linear_tc_parts(const Product<__nv_bfloat16>& p, float* partial, int64_t ld, int wait_limit, int32_t* status, cudaStream_t st);
 int linear_tc_split(int64_t M, int64_t N, int64_t K);

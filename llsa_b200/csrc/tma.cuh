@@ -28,6 +28,16 @@ inline EncodeFn encode_fn() {
   return fn;
 }
 
+// The encoder wants a context on the calling thread, and a thread whose first CUDA call this is (the autograd engine's, a worker's) has none until the
+// runtime makes one current there.
+template <typename... A>
+inline CUresult encode(EncodeFn fn, A... args) {
+  CUresult r = fn(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = fn(args...);
+  return r;
+}
+
 // bf16 tensor of `rank` dims (dims[0] = 64 channels, unit stride), byte strides for dims 1..rank-1,
 // box = box_rows rows of 64 channels, 128-byte swizzle.
 inline int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes, uint32_t box_rows) {
@@ -40,7 +50,7 @@ inline int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* 
   for (int i = 0; i + 1 < rank; ++i) gs[i] = strides_bytes[i];
   box[0] = 64;
   box[1] = box_rows;
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t) rank, const_cast<void*>(base), gd, gs, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUresult r = encode(fn, m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t) rank, const_cast<void*>(base), (const cuuint64_t*) gd, (const cuuint64_t*) gs, (const cuuint32_t*) box, (const cuuint32_t*) es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   LLSA_REQUIRE(r == CUDA_SUCCESS, LLSA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int) r);
   return LLSA_OK;
@@ -70,7 +80,7 @@ inline int make_map_acc(CUtensorMap* m, void* base, uint64_t rows, uint32_t box_
   LLSA_REQUIRE(fn != nullptr, LLSA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t gd[2] = {64, rows}, gs[1] = {256};
   const cuuint32_t box[2] = {32, box_rows}, es[2] = {1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, base, gd, gs, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = encode(fn, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, (cuuint32_t) 2, base, gd, gs, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   LLSA_REQUIRE(r == CUDA_SUCCESS, LLSA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int) r);
   return LLSA_OK;
@@ -113,6 +123,11 @@ __device__ __forceinline__ void store_4d_w(const CUtensorMap* map, int c0, int c
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                "@e cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(c2),
                "r"(c3), "r"(smem_src)
+               : "memory");
+}
+__device__ __forceinline__ void store_2d_w(const CUtensorMap* map, int c0, int c1, uint32_t smem_src) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(smem_src)
                : "memory");
 }
 __device__ __forceinline__ void reduce_commit_w() {

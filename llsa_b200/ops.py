@@ -189,7 +189,7 @@ def _register_fakes() -> None:
         return [y, x.new_empty((x.numel() // x.shape[-1], F))] if want_pre else [y]
 
     @torch.library.register_fake("llsa_b200::linear_bwd")
-    def _(dy, x, weight, pre, gate, activation, want):
+    def _(dy, x, weight, bias, pre, gate, activation, want):
         F = weight.shape[0]
         shapes = (x.shape, weight.shape, (F,), (x.shape[0] if gate is not None else 1, F))
         return [x.new_empty(shapes[i]) for i in range(4) if want >> i & 1]
@@ -496,8 +496,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x: [..., K]; weight: [F, K]; bias: [F]; activation: None, "gelu_tanh" or "silu"; residual: of y's shape [..., F]; gate: [B, F], a sample's
     factors for all of its tokens (x is then [B, ..., K]), with a residual and without an activation.  All of one type, float32 or
-    bfloat16; sums are fp32.  Differentiable in all five.  For a gradient through an activation or of a gate the product is kept (16 bits a value for
-    bfloat16).  Rows that are no multiple of 16 bytes cost bfloat16 operands a copy."""
+    bfloat16; sums are fp32.  Differentiable in all five.  For the gradient of a gate, and of float32 data through an activation, the product
+    is kept between the passes; bfloat16 data compute it again for an activation.  Rows that are no multiple of 16 bytes cost bfloat16 operands a copy."""
     if activation not in _ACTIVATIONS:
         raise ValueError("llsa_b200: activation must be None, 'gelu_tanh' or 'silu', got %r" % (activation,))
     _ready()

@@ -266,6 +266,10 @@ def test_linear_strides_ranks_and_partial_gradients(dtype):
         y = llsa_b200.linear(t["x"], t["w"], t["b"], residual=t["r"], gate=t["g"])
         for k, d in zip(wanted, torch.autograd.grad(y, [t[k] for k in wanted], dy)):
             assert torch.equal(full.setdefault(k, d), d), k
+    # a bias on no 16-byte boundary, a gate and a residual with gaps
+    wide = normal(g, 4, 21, F + 3, dtype=dtype)
+    same = llsa_b200.linear(data["x"], w, normal(gen(12), F + 1, dtype=dtype)[1:], residual=wide[..., 1:F + 1], gate=wide[:, 0, 3:])
+    assert torch.equal(same, llsa_b200.linear(data["x"], w, normal(gen(12), F + 1, dtype=dtype)[1:].clone(), residual=wide[..., 1:F + 1].clone(), gate=wide[:, 0, 3:].clone()))
     # an upstream gradient that is one number everywhere
     x = room[..., :K].detach().requires_grad_(True)
     (d,) = torch.autograd.grad(llsa_b200.linear(x, w).sum(), x)
@@ -483,6 +487,31 @@ def test_same_bits_every_time_on_any_stream_and_in_graphs():
             graphs[i].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(outs[0], want[0])) and all(torch.equal(p, q) for p, q in zip(outs[1], w1))
+
+
+def test_first_call_of_a_thread():
+    """A thread that has made no CUDA call yet, as the autograd engine's before its first backward: tensor maps need a context there."""
+    import threading
+    leaves, dy, pos = _block_leaves(63)
+    want = _pass(leaves, dy, pos)
+    t, w = torch.randn(64, 64, device=DEV).bfloat16(), torch.randn(64, 64, device=DEV).bfloat16()
+    one = llsa_b200.linear(t, w)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work():
+        try:
+            got["one"] = llsa_b200.linear(t, w)
+            got["pass"] = _pass(leaves, dy, pos)
+            torch.cuda.synchronize()
+        except Exception as e:      # shown by the assertion below
+            got["error"] = e
+
+    th = threading.Thread(target=work)
+    th.start()
+    th.join()
+    assert "error" not in got, got["error"]
+    assert torch.equal(got["one"], one) and all(torch.equal(a, b) for a, b in zip(got["pass"], want))
 
 
 def test_operators_trace():
