@@ -161,7 +161,7 @@ typedef struct LlsaLinearArgs {
   const LlsaTensor* residual;  /* [M,F], any row stride, or NULL */
   const LlsaTensor* gate;      /* [B,F], any row stride, or NULL: row b stands for rows [b M/B, (b+1) M/B); with a residual and no activation */
   const LlsaTensor* y;         /* [M,F] out, any row stride */
-  const LlsaTensor* pre;       /* x weight^T + bias, [M,F] of x's type, contiguous: written by the forward if given (bf16: without an activation), read by the
+  const LlsaTensor* pre;       /* x weight^T + bias, [M,F] of x's type, contiguous: written by the forward if given (bf16: only with a gate), read by the
                                   backward for dgate and, F32, through an activation; bf16 data compute it again there (bias as in the forward) */
   int32_t activation;          /* LlsaActivation */
   /* backward: dy in, those of the others that are not NULL out */

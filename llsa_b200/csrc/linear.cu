@@ -209,17 +209,46 @@ int launch_dz(FrontArgs<T>& f, int64_t blocks, int tx, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ parts of a split product
-template <typename T>
+// out[r, c] = sum of the parts' (r, c), or, TURNED, of their (c, r).  A CTA takes 32 x 32 of them through shared memory, 8 rows of threads; the parts are
+// added in order, four on their way at once.
+template <typename T, bool TURNED>
 __global__ void __launch_bounds__(256)
 sum_parts_kernel(const float* __restrict__ partial, int64_t ld, int split, int64_t rows, int64_t cols, T* __restrict__ out) {
+  __shared__ float s_tile[32][33];
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const int64_t r0 = blockIdx.y * (int64_t) 32, c0 = blockIdx.x * (int64_t) 32;
+  const int64_t part = (TURNED ? cols : rows) * ld, prow = TURNED ? c0 : r0, pcol = (TURNED ? r0 : c0) + x;
+  const int64_t prows = TURNED ? cols : rows, pcols = TURNED ? rows : cols;
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = blockIdx.x * (int64_t) blockDim.x + threadIdx.x; i < rows * cols; i += (int64_t) gridDim.x * blockDim.x) {
-    const int64_t r = i / cols, c = i - r * cols;
-    float u = 0.f;
-    for (int s = 0; s < split; ++s) u += partial[(s * rows + r) * ld + c];
-    out[i] = from_f32<T>(u);
+  float u[4] = {0.f, 0.f, 0.f, 0.f};
+  if (pcol < pcols) {
+#pragma unroll 4
+    for (int s = 0; s < split; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (prow + y + 8 * i < prows) u[i] += partial[s * part + (prow + y + 8 * i) * ld + pcol];
   }
+  if constexpr (TURNED) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_tile[y + 8 * i][x] = u[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = s_tile[x][y + 8 * i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r0 + y + 8 * i < rows && c0 + x < cols) out[(r0 + y + 8 * i) * cols + c0 + x] = from_f32<T>(u[i]);
+}
+
+template <typename T>
+int sum_parts(const float* partial, int64_t ld, int split, bool turned, int64_t rows, int64_t cols, T* out, cudaStream_t st) {
+  const dim3 grid((unsigned) ((cols + 31) / 32), (unsigned) ((rows + 31) / 32));
+  LLSA_REQUIRE(grid.y <= 65535, LLSA_ERR_SHAPE, "linear_bwd: too many features");
+  if (turned) launch_pdl(sum_parts_kernel<T, true>, grid, dim3(256), 0, st, partial, ld, split, rows, cols, out);
+  else launch_pdl(sum_parts_kernel<T, false>, grid, dim3(256), 0, st, partial, ld, split, rows, cols, out);
+  LLSA_LAUNCH_OK("sum_parts_kernel");
+  return LLSA_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ checks and plan
@@ -241,7 +270,8 @@ struct Plan {
   bool slope;                  // bf16 with an activation: that pass is a product
   int vec, tx;                 // its columns of a thread, threads along the columns
   int64_t dz_ld, chunks, per;
-  int split;
+  int split;                   // dw: parts of the sum over the rows, of [F][part_ld], or turned [K][part_ld]
+  bool turned;
   int64_t part_ld;
   size_t o_dz, o_cols, o_parts, bytes;
 };
@@ -288,7 +318,7 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   p->dz_ld = (p->F + 7) / 8 * 8;
   p->slope = p->dtype == LLSA_BF16 && a->activation != kActNone;
   if (p->slope) {
-    p->chunks = linear_tc_slope_groups(p->M, p->F);
+    p->chunks = linear_tc_slope_groups(p->M, p->F, p->K);
   } else {
     // a CTA: tx threads along the columns, the width of 16, 32 or 64 that leaves the fewest idle; enough CTAs along the rows for 148 x 6, 16 rows a thread or more
     p->vec = p->F % 8 == 0 && a->dy && rows16(a->dy) ? 16 / es : 1;
@@ -306,8 +336,9 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
     p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
   }
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
-  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
-  p->part_ld = (p->K + 7) / 8 * 8;
+  p->turned = false;
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
+  p->part_ld = ((p->turned ? p->F : p->K) + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -316,7 +347,7 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   };
   p->o_dz = take(p->write_dz ? (size_t) (p->M * p->dz_ld * es) : 0);
   p->o_cols = take(p->sums ? (size_t) (p->B * p->chunks * 2 * p->F * 4) : 0);
-  p->o_parts = take(a->dweight ? (size_t) (p->split * p->F * p->part_ld * 4) : 0);
+  p->o_parts = take(a->dweight ? (size_t) (p->split * (p->turned ? p->K : p->F) * p->part_ld * 4) : 0);
   p->bytes = at;
 }
 
@@ -403,11 +434,11 @@ int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   }
   if (a->dweight) {
     float* parts = (float*) (ws + p.o_parts);
-    const int rc = product_parts(Product<T>{dz, mat<const T>(a->x), 0, 0, p.F, p.K, p.M, p.split}, parts, p.part_ld, a, st);
+    const Mat<const T> x = mat<const T>(a->x);
+    const int rc = p.turned ? product_parts(Product<T>{x, dz, 0, 0, p.K, p.F, p.M, p.split}, parts, p.part_ld, a, st)
+                            : product_parts(Product<T>{dz, x, 0, 0, p.F, p.K, p.M, p.split}, parts, p.part_ld, a, st);
     if (rc) return rc;
-    const int64_t blocks = std::min<int64_t>((p.F * p.K + 255) / 256, 148 * 8);
-    launch_pdl(sum_parts_kernel<T>, dim3((unsigned) blocks), dim3(256), 0, st, (const float*) parts, p.part_ld, p.split, p.F, p.K, (T*) a->dweight->ptr);
-    LLSA_LAUNCH_OK("sum_parts_kernel");
+    return sum_parts<T>(parts, p.part_ld, p.split, p.turned, p.F, p.K, (T*) a->dweight->ptr, st);
   }
   return LLSA_OK;
 }
@@ -423,6 +454,7 @@ extern "C" int llsa_linear_fwd(const LlsaLinearArgs* a, void* stream) {
   if (rc) return rc;
   if (a->residual && (rc = check_matrix(a->residual, "residual", p.dtype, p.M, p.F))) return rc;
   LLSA_REQUIRE(!a->gate || a->residual, LLSA_ERR_ARG, "linear: a gate goes with a residual");
+  LLSA_REQUIRE(!a->pre || a->gate || p.dtype == LLSA_F32, LLSA_ERR_ARG, "linear: bf16 products are kept for a gate only");
   if ((rc = check_matrix(a->y, "y", p.dtype, p.M, p.F))) return rc;
   if (p.M == 0) return LLSA_OK;
   return p.dtype == LLSA_F32 ? forward<float>(a, p, (cudaStream_t) stream) : forward<bf16>(a, p, (cudaStream_t) stream);

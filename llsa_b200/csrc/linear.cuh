@@ -59,9 +59,10 @@ int linear_tc_product(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloa
 // dz = dy act'(z) with z computed once more, e.y = dz (rows on 16-byte boundaries), and the column sums of dz: sums[group][1][N], linear_tc_slope_groups of them;
 int linear_tc_slope(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, const Mat<const __nv_bfloat16>& dy, float* sums, int wait_limit,
                     int32_t* status, cudaStream_t st);
-int64_t linear_tc_slope_groups(int64_t M, int64_t N);
+int64_t linear_tc_slope_groups(int64_t M, int64_t N, int64_t K);
 // the weight's gradient (both operands across), in p.split parts of [M][ld], ld a multiple of 8; the number of parts to take
 int linear_tc_parts(const Product<__nv_bfloat16>& p, float* partial, int64_t ld, int wait_limit, int32_t* status, cudaStream_t st);
-int linear_tc_split(int64_t M, int64_t N, int64_t K);
+// `turned`: the parts are better taken of the transposed result, A and B changing places
+int linear_tc_split(int64_t M, int64_t N, int64_t K, bool* turned);
 
 }  // namespace llsa

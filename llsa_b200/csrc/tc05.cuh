@@ -237,6 +237,59 @@ __device__ __forceinline__ void umma_commit_w(uint64_t* bar) {
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
+// ---- pairs of CTAs (a cluster of two): one product of 256 rows, 128 of them in either CTA's tensor memory, with half of B in either CTA's shared
+// memory at the same offsets.  The CTA of rank 0 issues; both allocate and free.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared variable in the CTA of rank `rank`
+__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
+  uint32_t d;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_u32(p)), "r"(rank));
+  return d;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int AS = 2, int BS = 2>
+__device__ __forceinline__ void umma_pair_ss_k64(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred f, t, e;\n\t.reg .b32 al, bl;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 f, %7, 0; setp.eq.b32 t, %6, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "add.u32 al, %1, 0; add.u32 bl, %3, 0;\n\t"
+      "mov.b64 da, {al, %2}; mov.b64 db, {bl, %4};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%6, %6, %6, %6, %6, %6, %6, %6}, f;\n\t"
+      "add.u32 al, %1, %8; add.u32 bl, %3, %9;\n\t"
+      "mov.b64 da, {al, %2}; mov.b64 db, {bl, %4};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%6, %6, %6, %6, %6, %6, %6, %6}, t;\n\t"
+      "add.u32 al, %1, %10; add.u32 bl, %3, %11;\n\t"
+      "mov.b64 da, {al, %2}; mov.b64 db, {bl, %4};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%6, %6, %6, %6, %6, %6, %6, %6}, t;\n\t"
+      "add.u32 al, %1, %12; add.u32 bl, %3, %13;\n\t"
+      "mov.b64 da, {al, %2}; mov.b64 db, {bl, %4};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, {%6, %6, %6, %6, %6, %6, %6, %6}, t;\n\t"
+      "}"
+      :
+      : "r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(0u), "r"(accumulate), "n"(AS), "n"(BS), "n"(2 * AS),
+        "n"(2 * BS), "n"(3 * AS), "n"(3 * BS)
+      : "memory");
+}
+// Arrives on this barrier in both CTAs of the pair
+__device__ __forceinline__ void umma_commit_pair_w(uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+               "h"((uint16_t) 3)
+               : "memory");
+}
 // ---- TMEM -> registers: lane (32 * (warp % 4) + lane id) gets 32 consecutive fp32 columns ----
 // Asynchronous: the registers may be read only after tmem_ld_wait(v) (which ties them to the wait).
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) {
@@ -271,6 +324,22 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 64 columns of 16 lanes (those at taddr), spread as the accumulators of an m16n8 product are: this thread gets columns 8 j + 2 (lane % 4) + {0, 1} of rows
+// lane / 4 (v[4 j], v[4 j + 1]) and lane / 4 + 8 (v[4 j + 2], v[4 j + 3]), j < 8
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
 }

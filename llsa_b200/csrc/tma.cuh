@@ -96,6 +96,14 @@ __device__ __forceinline__ void load_2d_w(void* smem_dst, const CUtensorMap* map
                "l"(map), "r"((uint32_t) __cvta_generic_to_shared(mbar)), "r"(c0), "r"(c1)
                : "memory");
 }
+// A copy into this CTA's shared memory that completes on a barrier of the pair's other CTA, or of this one: `mbar` is its address in the cluster
+__device__ __forceinline__ void load_2d_pair_w(void* smem_dst, const CUtensorMap* map, uint32_t mbar, int c0, int c1) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(
+                   (uint32_t) __cvta_generic_to_shared(smem_dst)),
+               "l"(map), "r"(mbar), "r"(c0), "r"(c1)
+               : "memory");
+}
 __device__ __forceinline__ void load_4d_w(void* smem_dst, const CUtensorMap* map, uint64_t* mbar, int c0, int c1, int c2, int c3) {
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(
