@@ -153,6 +153,12 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Op
 }
 
 // ------------------------------------------------------------------ projection
+// Room for a matrix whose rows start on 16-byte boundaries
+Tensor padded(std::array<int64_t, 2> shape, const Tensor& like) {
+  const int64_t per = 16 / like.element_size(), ld = (shape[1] + per - 1) / per * per;
+  return at::empty_strided(shape, {ld, 1}, like.options());
+}
+
 // [M, C] with unit column stride and, for bf16, rows on 16-byte boundaries where `aligned` (a copy in padded rows where the tensor has none)
 Tensor matrix(const Tensor& t, int64_t M, int64_t C, bool aligned) {
   const Tensor m = t.reshape({M, C});
@@ -160,8 +166,7 @@ Tensor matrix(const Tensor& t, int64_t M, int64_t C, bool aligned) {
   const bool rows = (C == 1 || m.stride(1) == 1) && (M == 1 || m.stride(0) >= C);
   const bool fits = !aligned || m.scalar_type() != at::kBFloat16 || ((uintptr_t) m.data_ptr() % 16 == 0 && (M == 1 || m.stride(0) % per == 0));
   if (rows && fits) return m;
-  const Tensor room = at::empty({M, aligned ? (C + per - 1) / per * per : C}, m.options());
-  Tensor c = room.narrow(1, 0, C);
+  Tensor c = aligned ? padded({M, C}, m) : at::empty({M, C}, m.options());
   c.copy_(m);
   return c;
 }
@@ -201,8 +206,11 @@ LlsaLinearArgs linear_args(int64_t act, const Status& status) {
   return a;
 }
 
+// Rows that are no multiple of 16 bytes cost a copy of x and the weight, which a backward wants as well.  [y], then with want_pre z, with want_copies and such rows the
+// copies of x [M, K] and of the weight.
+bool rows_want_copies(const Tensor& x, int64_t K) { return x.scalar_type() == at::kBFloat16 && K % 8; }
 std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTensor& bias, const OptTensor& residual, const OptTensor& gate, int64_t act,
-                               bool want_pre) {
+                               bool want_pre, bool want_copies) {
   const Tensor b_ = or_none(bias), r_ = or_none(residual), g_ = or_none(gate);
   same_device(x_, {w_, b_, r_, g_});
   check_float({&x_, &w_});
@@ -217,7 +225,13 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
   const c10::cuda::CUDAGuard guard(x_.device());
   std::vector<Tensor> out = {at::empty(shape, x_.options())};
   if (want_pre) out.push_back(at::empty({s.M, s.F}, x_.options()));
-  if (s.M == 0) return out;
+  if (s.M == 0) {
+    if (want_copies && rows_want_copies(x_, s.K)) {
+      out.push_back(padded({s.M, s.K}, x_));
+      out.push_back(padded({s.F, s.K}, x_).copy_(w_));
+    }
+    return out;
+  }
   const Tensor x = matrix(x_, s.M, s.K, true), w = matrix(w_, s.F, s.K, true), y = out[0].view({s.M, s.F});
   const LlsaTensor xd = desc(x), wd = desc(w), yd = desc(y);
   const Status status(x);
@@ -233,14 +247,18 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
   ok(llsa_linear_fwd(&a, at::cuda::getCurrentCUDAStream(x.device().index())), "linear_fwd");
   mark("end");
   status.check("linear_fwd");
+  if (want_copies && rows_want_copies(x_, s.K)) {      // an output must not be an input, such as rows that came padded
+    out.push_back(x.is_alias_of(x_) ? padded({s.M, s.K}, x_).copy_(x) : x);
+    out.push_back(w.is_alias_of(w_) ? padded({s.F, s.K}, x_).copy_(w) : w);
+  }
   return out;
 }
 
 // want: 1 x, 2 weight, 4 bias, 8 gate; the gradients asked for, in that order
 std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& w_, const OptTensor& bias, const OptTensor& pre, const OptTensor& gate,
-                               int64_t act, int64_t want) {
+                               const OptTensor& x_copy, const OptTensor& w_copy, int64_t act, int64_t want) {
   const Tensor b_ = or_none(bias), p_ = or_none(pre), g_ = or_none(gate);
-  same_device(x_, {dy_, w_, b_, p_, g_});
+  same_device(x_, {dy_, w_, b_, p_, g_, or_none(x_copy), or_none(w_copy)});
   check_float({&x_, &w_, &dy_});
   for (const Tensor& t : {b_, p_, g_})
     if (t.defined()) check_float({&x_, &t});
@@ -257,7 +275,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor
   if (want & 4) out.push_back(db = room({s.F}));
   if (want & 8) out.push_back(dg = room({s.B, s.F}));
   if (s.M == 0 || !want) return out;
-  const Tensor x = matrix(x_, s.M, s.K, true), w = matrix(w_, s.F, s.K, true), dy = matrix(dy_, s.M, s.F, false);
+  const Tensor x = matrix(x_copy ? *x_copy : x_, s.M, s.K, true), w = matrix(w_copy ? *w_copy : w_, s.F, s.K, true), dy = matrix(dy_, s.M, s.F, false);
   const Status status(x);
   LlsaLinearArgs a = linear_args(act, status);
   const LlsaTensor xd = desc(x), wd = desc(w), dyd = desc(dy);
@@ -329,8 +347,9 @@ const c10::TypedOperatorHandle<Sig>& op(const char* name) {      // once per sig
 using NormFwd = std::vector<Tensor>(const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, double, bool);
 using NormBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Tensor&, int64_t, at::ScalarType,
                                     at::ScalarType);
-using LinearFwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool);
-using LinearBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, int64_t);
+using LinearFwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool, bool);
+using LinearBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                                      const OptTensor&, int64_t, int64_t);
 using Rope = Tensor(const Tensor&, const Tensor&, at::IntArrayRef, double, bool);
 const auto& norm_fwd_op() { return op<NormFwd>("llsa_b200::layer_norm_fwd"); }
 const auto& norm_bwd_op() { return op<NormBwd>("llsa_b200::layer_norm_bwd"); }
@@ -399,11 +418,12 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     variable_list out;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      out = linear_fwd_op().call(x, w, b, r, gate, act, pre);
+      out = linear_fwd_op().call(x, w, b, r, gate, act, pre, true);
     }
     ctx->set_materialize_grads(false);
-    if (pre) ctx->mark_non_differentiable({out[1]});
-    ctx->save_for_backward({x, w, pre ? out[1] : Tensor(), or_none(gate), or_none(b)});
+    ctx->mark_non_differentiable(variable_list(out.begin() + 1, out.end()));
+    const bool copies = out.size() > 2u + pre;
+    ctx->save_for_backward({x, w, pre ? out[1] : Tensor(), or_none(gate), or_none(b), copies ? out[1 + pre] : Tensor(), copies ? out[2 + pre] : Tensor()});
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = r.has_value();
     return out;
@@ -422,7 +442,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     if (e.wants(s[3])) want |= 8;
     if (want) {
       const std::vector<Tensor> r =
-          below_unless_recorded([&] { return linear_bwd_op().call(grads[0], s[0], s[1], opt(s[4]), opt(s[2]), opt(s[3]), act, want); });
+          below_unless_recorded([&] { return linear_bwd_op().call(grads[0], s[0], s[1], opt(s[4]), opt(s[2]), opt(s[3]), opt(s[5]), opt(s[6]), act, want); });
       size_t at = 0;
       if (want & 1) g[0] = r[at++];
       if (want & 2) g[1] = r[at++];
@@ -435,11 +455,11 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 };
 
 std::vector<Tensor> linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, const OptTensor& gate, int64_t act,
-                                    bool want_pre) {
+                                    bool want_pre, bool want_copies) {
   no_tangents("linear", {x, w, or_none(b), or_none(r), or_none(gate)});
   if (any_grad({x, w, or_none(b), or_none(r), or_none(gate)})) return LinearFunction::apply(x, w, b, r, gate, act);
   at::AutoDispatchBelowADInplaceOrView below;
-  return linear_fwd_op().call(x, w, b, r, gate, act, want_pre);
+  return linear_fwd_op().call(x, w, b, r, gate, act, want_pre, want_copies);
 }
 
 struct RopeFunction : torch::autograd::Function<RopeFunction> {
@@ -478,8 +498,9 @@ TORCH_LIBRARY_FRAGMENT(llsa_b200, m) {
   m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, float eps, bool want_stats) -> Tensor[]");
   m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor stats, int want, ScalarType shift_type, "
         "ScalarType bias_type) -> Tensor[]");
-  m.def("linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, int activation, bool want_pre) -> Tensor[]");
-  m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, Tensor? bias, Tensor? pre, Tensor? gate, int activation, int want) -> Tensor[]");
+  m.def("linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, int activation, bool want_pre, bool want_copies) -> "
+        "Tensor[]");
+  m.def("linear_bwd(Tensor dy, Tensor x, Tensor weight, Tensor? bias, Tensor? pre, Tensor? gate, Tensor? x_copy, Tensor? w_copy, int activation, int want) -> Tensor[]");
   m.def("rope_axes(Tensor x, Tensor positions, int[] axes_dims, float theta, bool inverse) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(llsa_b200, CUDA, m) {

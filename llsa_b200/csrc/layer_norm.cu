@@ -9,37 +9,17 @@
 // the sums (mean first, then the squares of the centred values: no cancellation) and A, T of the sample stay there from row to row.  All sums are
 // fp32; results are rounded once.  Column sums go through registers, shared memory and one partial per CTA to a second kernel that adds
 // them in a fixed order: the same bits from run to run.
+// Reading and writing the rows once each is what there is to do; what costs beside it is a row's chain of sums and the instructions around it, some 200 a
+// warp, so the pairs of values share instructions, a row is on its way while another is worked on, and enough warps fit an SM.
 #include "column_sums.cuh"
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace llsa {
 
 namespace {
 
 using bf16 = __nv_bfloat16;
-
-template <typename T, int VEC>
-struct Pack;
-template <>
-struct Pack<bf16, 4> {
-  using type = uint2;
-  static __device__ __forceinline__ void unpack(uint2 r, float* v) {
-    v[0] = bf16_lo(r.x); v[1] = bf16_hi(r.x); v[2] = bf16_lo(r.y); v[3] = bf16_hi(r.y);
-  }
-  static __device__ __forceinline__ uint2 pack(const float* v) { return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])); }
-};
-template <>
-struct Pack<float, 4> {
-  using type = float4;
-  static __device__ __forceinline__ void unpack(float4 r, float* v) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-  static __device__ __forceinline__ float4 pack(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
-};
-template <typename T>
-struct Pack<T, 1> {
-  using type = T;
-  static __device__ __forceinline__ void unpack(T r, float* v) { v[0] = to_f32<T>(r); }
-  static __device__ __forceinline__ T pack(const float* v) { return from_f32<T>(v[0]); }
-};
 
 // [B,N,C] tensor with unit channel stride
 template <typename T>
@@ -54,50 +34,106 @@ struct NormParams {
   ParamView w, bias, scale, shift;
 };
 
-// The part of a row that one thread of a group of `threads` holds: R vectors of VEC channels, `threads` vectors apart
-template <typename T, int VEC, int R>
+// The part of a row that one thread of a group of `threads` holds: R vectors of VEC channels, `threads` vectors apart.
+//   kWhole   vectors of four on their boundaries; R is no larger than C asks for, and only the last one may lie behind the row's end
+//   kLoose   the same, with any of them behind the end
+//   kShifted rows of any length, whose vectors of four begin `m` channels in front of the row, on their boundary; those over the row's ends go element by element
+//   kSingle  element by element
+enum Form { kWhole, kLoose, kShifted, kSingle };
+template <typename T, int FORM, int R>
 struct Slice {
-  using P = Pack<T, VEC>;
+  static constexpr int VEC = FORM == kSingle ? 1 : 4, E = R * VEC;
+  using P = Vec<T, VEC>;
   typename P::type raw[R];
-  __device__ __forceinline__ void load(const T* row, int t, int threads, int C) {
+  static __device__ __forceinline__ int channel(int e, int t, int threads, int m) { return ((e / VEC) * threads + t) * VEC + e % VEC - (FORM == kShifted ? m : 0); }
+  static __device__ __forceinline__ bool there(int e, int c, int C) {
+    if (FORM == kWhole) return e / VEC < R - 1 || c < C;
+    return FORM == kShifted ? (unsigned) c < (unsigned) C : c < C;
+  }
+  __device__ __forceinline__ void load(const T* row, int t, int threads, int C, int m) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int c = (i * threads + t) * VEC;
-      if (c < C) raw[i] = *reinterpret_cast<const typename P::type*>(row + c);
+      const int c = channel(i * VEC, t, threads, m);
+      if (FORM != kShifted ? there(i * VEC, c, C) : c >= 0 && c + VEC <= C) {
+        raw[i] = *reinterpret_cast<const typename P::type*>(row + c);
+      } else if (FORM == kShifted) {
+        T* u = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (there(0, c + j, C)) u[j] = row[c + j];
+      }
     }
   }
-  __device__ __forceinline__ void values(float (&v)[R * VEC], int t, int threads, int C) const {
+  // The values in pairs, for instructions that take two; zeros where there is none
+  __device__ __forceinline__ void values(float2 (&v)[E / 2], int t, int threads, int C, int m) const {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      P::unpack(raw[i], v + i * VEC);
-      if ((i * threads + t) * VEC >= C)
+      float u[VEC];
+      P::unpack(raw[i], u);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0.f;
+      for (int j = 0; j < VEC; ++j) {
+        const int e = i * VEC + j;
+        const float x = there(e, channel(e, t, threads, m), C) ? u[j] : 0.f;
+        if (e & 1) v[e / 2].y = x;
+        else v[e / 2].x = x;
+      }
     }
   }
-  static __device__ __forceinline__ void store(T* row, const float (&v)[R * VEC], int t, int threads, int C) {
+  static __device__ __forceinline__ void store(T* row, const float2 (&v)[E / 2], int t, int threads, int C, int m) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int c = (i * threads + t) * VEC;
-      if (c < C) *reinterpret_cast<typename P::type*>(row + c) = P::pack(v + i * VEC);
+      const int c = channel(i * VEC, t, threads, m);
+      const typename P::type w = P::pack(reinterpret_cast<const float*>(v) + i * VEC);
+      if (FORM != kShifted ? there(i * VEC, c, C) : c >= 0 && c + VEC <= C) {
+        *reinterpret_cast<typename P::type*>(row + c) = w;
+      } else if (FORM == kShifted) {
+        const T* u = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (there(0, c + j, C)) row[c + j] = u[j];
+      }
     }
   }
 };
+// A parameter's part beside a slice; `absent` where it or the channel is not there.  One look at its type, not one for every channel
+template <typename S>
+__device__ __forceinline__ void load_param(float (&v)[S::E], const ParamView& p, uint32_t b, float absent, int t, int threads, int C, int m) {
+  if (p.p && p.is_bf16) {
+    const bf16* row = reinterpret_cast<const bf16*>(p.p) + b * p.ld;
+#pragma unroll
+    for (int e = 0; e < S::E; ++e) {
+      const int c = S::channel(e, t, threads, m);
+      v[e] = S::there(e, c, C) ? __bfloat162float(row[c]) : absent;
+    }
+  } else if (p.p) {
+    const float* row = reinterpret_cast<const float*>(p.p) + b * p.ld;
+#pragma unroll
+    for (int e = 0; e < S::E; ++e) {
+      const int c = S::channel(e, t, threads, m);
+      v[e] = S::there(e, c, C) ? row[c] : absent;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < S::E; ++e) v[e] = absent;
+  }
+}
+template <typename T>
+__device__ __forceinline__ int shift_of(const T* row) { return (int) ((uintptr_t) row / sizeof(T) & 3); }
 
-// Sums of N values over a group: a warp, or `warps` warps of the CTA (then every thread of the CTA calls).  Two buffers in turn: a warp that
-// is one sum ahead writes the other one, and it cannot be two ahead.
+// Sums of N values over a group: a warp, or `warps` warps of the CTA that meet at a barrier of their own.  Two buffers in turn: a warp that is one sum
+// ahead writes the other one, and it cannot be two ahead.
 template <bool MULTI, int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], int& turn, int warps) {
+__device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], int& turn, int warps, int group) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   if constexpr (MULTI) {
-    const int warp = threadIdx.x >> 5, first = warp / warps * warps;
+    const int warp = threadIdx.x >> 5, first = group * warps;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) s_red[turn][warp][i] = v[i];
-    __syncthreads();
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * warps) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.f;
     for (int w = 0; w < warps; ++w)
@@ -107,186 +143,210 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], 
   }
 }
 
-// TPB: threads of a CTA; MULTI: more than one warp to a row
-template <typename T, int VEC, int R, bool MULTI, int TPB>
-__global__ void __launch_bounds__(TPB)
-layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, float2* __restrict__ stats, uint32_t M, uint32_t N, int C, int warps) {
-  constexpr int E = R * VEC;
+// CTAs that an SM should hold, by threads and by values of a thread: registers are what decides
+constexpr int fwd_ctas(int tpb, int e) { return tpb > 256 ? 1 : e <= 12 ? 4 : 3; }
+constexpr int bwd_ctas(int tpb) { return tpb > 256 ? 1 : 2; }
+
+// TPB: threads of a CTA; MULTI: more than one warp to a row.  A CTA takes rows [blockIdx.x * per, + per): neighbours, so that a group's sample, and with it A and
+// T, changes rarely.  (Rows a grid apart had them loaded for nearly every row: 8 x 16384 rows of 384 channels 77 us, 44 so.)
+template <typename T, int FORM, int R, bool MULTI, int TPB>
+__global__ void __launch_bounds__(TPB, fwd_ctas(TPB, R * (FORM == kSingle ? 1 : 4)))
+layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, float2* __restrict__ stats, uint32_t M, uint32_t N, uint32_t per, int C, int warps) {
+  using S = Slice<T, FORM, R>;
+  constexpr int E = S::E;
   __shared__ float s_red[2][32][2];
-  const int threads = 32 * warps, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = blockDim.x / threads;
+  const int threads = MULTI ? 32 * warps : 32, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = TPB / threads;
   const float inv_c = 1.f / (float) C;
-  int turn = 0;
+  const uint32_t end = min(M, (blockIdx.x + 1) * per);
+  int turn = 0, m = 0;
   pdl_wait();
   pdl_trigger();
-  float a[E], sh[E];
-  uint32_t cur = ~0u;
-  const uint64_t step = (uint64_t) gridDim.x * groups;
-  Slice<T, VEC, R> next;
-  uint64_t r = (uint64_t) blockIdx.x * groups + group;
-  uint32_t b = 0, n = 0;
-  if (r < M) {
-    b = (uint32_t) r / N; n = (uint32_t) r - b * N;
-    next.load(x.row(b, n), t, threads, C);
+  float2 a[E / 2], sh[E / 2];
+  uint32_t cur = ~0u, r = blockIdx.x * per + group, b = r / N, n = r - b * N;
+  S raw;
+  if (r < end) {
+    const T* row = x.row(b, n);
+    if (FORM == kShifted) m = shift_of(row);                   // of all the group's rows: they are a multiple of four apart
+    raw.load(row, t, threads, C, m);
   }
-  for (uint64_t base = (uint64_t) blockIdx.x * groups; base < M; base += step) {      // the same number of rounds for every group of the CTA
-    const bool valid = r < M;
-    const uint32_t rb = b, rn = n;
-    float v[E];
-    next.values(v, t, threads, C);
-    if (r + step < M) {
-      b = (uint32_t) (r + step) / N; n = (uint32_t) (r + step) - b * N;
-      next.load(x.row(b, n), t, threads, C);
+  while (r < end) {
+    const uint32_t rb = b, rn = n, rr = r;
+    float2 v[E / 2];
+    raw.values(v, t, threads, C, m);
+    r += groups;
+    n += groups;
+    if (n >= N) {
+      const uint32_t q = n / N;
+      b += q;
+      n -= q * N;
     }
-    if (valid && rb != cur) {
+    if (r < end) raw.load(x.row(b, n), t, threads, C, m);
+    if (rb != cur) {
       cur = rb;
+      float u[E], w[E];
+      load_param<S>(u, par.scale, rb, 0.f, t, threads, C, m);
+      load_param<S>(w, par.w, 0, 1.f, t, threads, C, m);
 #pragma unroll
-      for (int i = 0; i < R; ++i)
+      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(a)[e] = w[e] * (1.f + u[e]);
+      load_param<S>(w, par.bias, 0, 0.f, t, threads, C, m);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const int c = (i * threads + t) * VEC + j;
-          if (c < C) {
-            const float up = 1.f + par.scale.at(rb, c, 0.f);
-            a[i * VEC + j] = par.w.at(0, c, 1.f) * up;
-            sh[i * VEC + j] = fmaf(par.bias.at(0, c, 0.f), up, par.shift.at(rb, c, 0.f));
-          }
-        }
+      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] = w[e] * (1.f + u[e]);
+      load_param<S>(u, par.shift, rb, 0.f, t, threads, C, m);
+#pragma unroll
+      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] += u[e];
     }
-    float s[1] = {0.f}, q[1] = {0.f};
+    float2 s2 = v[0];
 #pragma unroll
-    for (int i = 0; i < E; ++i) s[0] += v[i];
-    group_sum<MULTI>(s, s_red, turn, warps);
+    for (int i = 1; i < E / 2; ++i) s2 = __fadd2_rn(s2, v[i]);
+    float s[1] = {s2.x + s2.y};
+    group_sum<MULTI>(s, s_red, turn, warps, group);
     const float mean = s[0] * inv_c;
+    float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      v[i] -= mean;
-      if (((i / VEC) * threads + t) * VEC < C) q[0] = fmaf(v[i], v[i], q[0]);
+    for (int i = 0; i < E / 2; ++i) {
+      v[i] = __fadd2_rn(v[i], make_float2(-mean, -mean));
+      float2 u = v[i];                                         // what is not there stays out of the squares
+      if (!S::there(2 * i, S::channel(2 * i, t, threads, m), C)) u.x = 0.f;
+      if (!S::there(2 * i + 1, S::channel(2 * i + 1, t, threads, m), C)) u.y = 0.f;
+      q2 = __ffma2_rn(u, u, q2);
     }
-    group_sum<MULTI>(q, s_red, turn, warps);
+    float q[1] = {q2.x + q2.y};
+    group_sum<MULTI>(q, s_red, turn, warps, group);
     const float rstd = rsqrtf(fmaf(q[0], inv_c, eps));
-    if (valid) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = fmaf(v[i] * rstd, a[i], sh[i]);
-      Slice<T, VEC, R>::store(y.row(rb, rn), v, t, threads, C);
-      if (stats && t == 0) stats[r] = make_float2(mean, rstd);
-    }
-    r += step;
+    for (int i = 0; i < E / 2; ++i) v[i] = __ffma2_rn(__fmul2_rn(v[i], make_float2(rstd, rstd)), a[i], sh[i]);
+    S::store(y.row(rb, rn), v, t, threads, C, m);
+    if (stats && t == 0) stats[rr] = make_float2(mean, rstd);
   }
 }
 
-// A CTA takes rows [s * per, (s + 1) * per) of sample b, chunk = b * chunks + s, and leaves its two column sums in partial[chunk][2][C].
-template <typename T, int VEC, int R, bool MULTI, int TPB, bool SUMS>
-__global__ void __launch_bounds__(TPB)
+// A CTA takes rows [s * per, (s + 1) * per) of sample b, chunk = b * chunks + s, and leaves its two column sums in partial[chunk][2][C] (NULL: none are wanted).
+// Of shifted rows every group holds other channels in a thread than its neighbour: the sums meet by channel in shared memory.
+template <typename T, int FORM, int R, bool MULTI, int TPB>
+__global__ void __launch_bounds__(TPB, bwd_ctas(TPB))
 layer_norm_bwd_kernel(Rows<const T> dy, Rows<const T> x, NormParams par, const float2* __restrict__ stats, Rows<T> dx, float* __restrict__ partial,
                       uint32_t N, uint32_t chunks, uint32_t per, int C, int warps) {
-  constexpr int E = R * VEC;
+  using S = Slice<T, FORM, R>;
+  constexpr int E = S::E;
   __shared__ float s_red[2][32][2];
-  __shared__ float s_col[SUMS ? 4096 : 1];
-  const int threads = 32 * warps, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = blockDim.x / threads;
+  __shared__ float s_col[TPB > 512 ? 1 : 16 * TPB];
+  const int threads = MULTI ? 32 * warps : 32, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = TPB / threads;
   const float inv_c = 1.f / (float) C;
   const uint32_t b = blockIdx.x / chunks, first = (blockIdx.x - b * chunks) * per, end = min(N, first + per);
-  int turn = 0;
+  int turn = 0, m = 0;
   pdl_wait();
   pdl_trigger();
-  float a[E], p[SUMS ? E : 1], sum[SUMS ? E : 1];
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const int c = (i * threads + t) * VEC + j;
-      a[i * VEC + j] = c < C ? par.w.at(0, c, 1.f) * (1.f + par.scale.at(b, c, 0.f)) : 0.f;
-      if constexpr (SUMS) p[i * VEC + j] = sum[i * VEC + j] = 0.f;
-    }
+  float2 a[E / 2], p[E / 2], sum[E / 2];
   uint32_t n = first + group;
-  Slice<T, VEC, R> nx, ng;
-  float2 nst = make_float2(0.f, 0.f);
+  if (FORM == kShifted) m = shift_of(x.row(b, n));
+  {
+    float u[E], w[E];
+    load_param<S>(u, par.scale, b, 0.f, t, threads, C, m);
+    load_param<S>(w, par.w, 0, 1.f, t, threads, C, m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(a)[e] = S::there(e, S::channel(e, t, threads, m), C) ? w[e] * (1.f + u[e]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) p[i] = sum[i] = make_float2(0.f, 0.f);
+  S rx, rg;
+  float2 rs = make_float2(0.f, 0.f);
   if (n < end) {
-    nx.load(x.row(b, n), t, threads, C);
-    ng.load(dy.row(b, n), t, threads, C);
-    nst = stats[(uint64_t) b * N + n];
+    rx.load(x.row(b, n), t, threads, C, m);
+    rg.load(dy.row(b, n), t, threads, C, m);
+    rs = stats[(uint64_t) b * N + n];
   }
-  for (uint32_t base = first; base < end; base += groups, n += groups) {
-    const bool valid = n < end;
-    float h[E], g[E];
-    nx.values(h, t, threads, C);
-    ng.values(g, t, threads, C);
-    const float mean = nst.x, rstd = nst.y;
-    if (n + groups < end) {
-      nx.load(x.row(b, n + groups), t, threads, C);
-      ng.load(dy.row(b, n + groups), t, threads, C);
-      nst = stats[(uint64_t) b * N + n + groups];
+  while (n < end) {
+    const uint32_t rn = n;
+    float2 h[E / 2], g[E / 2];
+    rx.values(h, t, threads, C, m);
+    rg.values(g, t, threads, C, m);
+    const float2 minus = make_float2(-rs.x, -rs.x), r2 = make_float2(rs.y, rs.y);
+    n += groups;
+    if (n < end) {
+      rx.load(x.row(b, n), t, threads, C, m);
+      rg.load(dy.row(b, n), t, threads, C, m);
+      rs = stats[(uint64_t) b * N + n];
     }
-    float m[2] = {0.f, 0.f};
+    float2 m1 = make_float2(0.f, 0.f), m2 = m1;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      h[i] = (h[i] - mean) * rstd;
-      if constexpr (SUMS)
-        if (valid) {
-          p[i] = fmaf(g[i], h[i], p[i]);
-          sum[i] += g[i];
-        }
-      g[i] *= a[i];
-      m[0] += g[i];
-      m[1] = fmaf(g[i], h[i], m[1]);
+    for (int i = 0; i < E / 2; ++i) {
+      h[i] = __fmul2_rn(__fadd2_rn(h[i], minus), r2);
+      p[i] = __ffma2_rn(g[i], h[i], p[i]);
+      sum[i] = __fadd2_rn(sum[i], g[i]);
+      g[i] = __fmul2_rn(g[i], a[i]);                           // 0 where nothing is there
+      m1 = __fadd2_rn(m1, g[i]);
+      m2 = __ffma2_rn(g[i], h[i], m2);
     }
-    group_sum<MULTI>(m, s_red, turn, warps);
-    m[0] *= inv_c;
-    m[1] *= inv_c;
-    if (valid) {
+    float s[2] = {m1.x + m1.y, m2.x + m2.y};
+    group_sum<MULTI>(s, s_red, turn, warps, group);
+    const float2 k1 = make_float2(-s[0] * inv_c, -s[0] * inv_c), k2 = make_float2(-s[1] * inv_c, -s[1] * inv_c);
 #pragma unroll
-      for (int i = 0; i < E; ++i) g[i] = rstd * (g[i] - m[0] - h[i] * m[1]);
-      Slice<T, VEC, R>::store(dx.row(b, n), g, t, threads, C);
-    }
+    for (int i = 0; i < E / 2; ++i) g[i] = __fmul2_rn(r2, __ffma2_rn(h[i], k2, __fadd2_rn(g[i], k1)));
+    S::store(dx.row(b, rn), g, t, threads, C, m);
   }
-  if constexpr (SUMS) {
-    float* out = partial + (int64_t) blockIdx.x * 2 * C;
-    if (groups == 1) {
+  if (!partial) return;
+  float* out = partial + (int64_t) blockIdx.x * 2 * C;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int c = ((i / VEC) * threads + t) * VEC + i % VEC;
-        if (c < C) {
-          out[c] = p[i];
-          out[C + c] = sum[i];
-        }
+  for (int which = 0; which < 2; ++which) {
+    const float* mine = reinterpret_cast<const float*>(which ? sum : p);
+    if (TPB > 512 || groups == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = S::channel(e, t, threads, m);
+        if (S::there(e, c, C)) out[which * C + c] = mine[e];
       }
     } else {
+      __syncthreads();
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int c = ((i / VEC) * threads + t) * VEC + i % VEC;
-          if (c < C) s_col[group * C + c] = which ? sum[i] : p[i];
-        }
-        __syncthreads();
-        for (int c = threadIdx.x; c < C; c += blockDim.x) {
-          float u = 0.f;
-          for (int k = 0; k < groups; ++k) u += s_col[k * C + c];
-          out[which * C + c] = u;
-        }
+      for (int e = 0; e < E; ++e) {
+        const int c = S::channel(e, t, threads, m);
+        if (S::there(e, c, C)) s_col[group * C + c] = mine[e];
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += TPB) {
+        float u = 0.f;
+        for (int k = 0; k < groups; ++k) u += s_col[k * C + c];
+        out[which * C + c] = u;
       }
     }
   }
 }
 
-// Warps of a group and vectors of a thread: the fewest warps whose threads hold at most 16 channels each.
+// ------------------------------------------------------------------------------------------------ choice of the kernel
+// The fewest warps to a row whose threads hold at most 16 channels each.
 struct Split {
-  int vec, r, warps, threads;
+  int form, r, warps, threads;
 };
-inline Split split_of(int64_t C, bool vec4) {
+// whole: rows on the boundaries of their vectors; alike: all of a call's rows begin equally far behind one, and four rows on again
+Split split_of(int64_t C, bool whole, bool alike) {
   Split s;
-  s.vec = vec4 ? 4 : 1;
+  s.form = whole ? kWhole : alike && C + 3 <= 2048 ? kShifted : kSingle;
+  const int64_t vec = s.form == kSingle ? 1 : 4, span = C + (s.form == kShifted ? 3 : 0);
   s.warps = 1;
-  while ((C + s.vec * 32 * s.warps - 1) / (s.vec * 32 * s.warps) * s.vec > 16) s.warps *= 2;
-  s.r = (int) ((C + s.vec * 32 * s.warps - 1) / (s.vec * 32 * s.warps));
-  if (!vec4) s.r = (s.r + 3) / 4 * 4;
-  s.threads = s.warps > 8 ? 32 * s.warps : 256;
+  while ((span + vec * 32 * s.warps - 1) / (vec * 32 * s.warps) * vec > 16) s.warps *= 2;
+  s.r = (int) ((span + vec * 32 * s.warps - 1) / (vec * 32 * s.warps));
+  // rows a multiple of four apart begin alike: four groups at least
+  s.threads = s.form == kShifted && s.warps == 4 ? 512 : 256;
+  if (s.warps > 8) {
+    s.threads = 1024;
+    s.warps = 32;
+    if (s.form == kWhole) s.form = kLoose;
+  }
   return s;
 }
-
-template <typename T>
-bool rows_vec4(const LlsaTensor* t) {
-  const int64_t bytes = 4 * sizeof(T);
-  return t->shape[2] % 4 == 0 && (uintptr_t) t->ptr % bytes == 0 && (t->shape[0] == 1 || t->stride[0] % 4 == 0) && (t->shape[1] == 1 || t->stride[1] % 4 == 0);
+template <typename T, typename... Ts>
+Split split_for(const LlsaTensor* x, Ts... others) {
+  const LlsaTensor* const t[] = {x, others...};
+  const int64_t es = sizeof(T);
+  bool whole = true, alike = true;
+  for (const LlsaTensor* u : t) {
+    const int64_t sb = u->shape[0] == 1 ? 0 : u->stride[0], sn = u->shape[1] == 1 ? 0 : u->stride[1];
+    whole = whole && u->shape[2] % 4 == 0 && (uintptr_t) u->ptr % (4 * es) == 0 && sb % 4 == 0 && sn % 4 == 0;
+    const int64_t sn0 = x->shape[1] == 1 ? 0 : x->stride[1], sb0 = x->shape[0] == 1 ? 0 : x->stride[0];
+    alike = alike && ((uintptr_t) u->ptr / es) % 4 == ((uintptr_t) x->ptr / es) % 4 && sn % 4 == sn0 % 4 && sb % 4 == sb0 % 4 &&
+            (x->shape[0] == 1 || sb % 4 == (x->shape[1] * u->stride[1]) % 4) && (x->shape[1] > 1 || sb % 4 == u->stride[1] % 4);
+  }
+  return split_of(x->shape[2], whole, alike);
 }
 template <typename T>
 Rows<T> make_rows(const LlsaTensor* t) {
@@ -321,66 +381,69 @@ struct Chunks {
   int64_t B, N, chunks, per;
 };
 Chunks chunks_of(int64_t B, int64_t N, int64_t C) {
-  const Split s = split_of(C, C % 4 == 0);
-  const int64_t groups = s.threads / (32 * s.warps), ctas = 148 * (s.threads > 256 ? 1 : 3);
+  const int64_t ctas = 148 * (C > 4096 ? 1 : 2);               // what the SMs hold at once
   Chunks c;
   c.B = B;
   c.N = N;
-  c.chunks = std::max<int64_t>(1, std::min((ctas + B - 1) / B, (N + 4 * groups - 1) / (4 * groups)));
-  c.per = (N + c.chunks - 1) / c.chunks;
-  c.per = (c.per + groups - 1) / groups * groups;
+  c.chunks = std::max<int64_t>(1, std::min((ctas + B - 1) / B, (N + 15) / 16));
+  c.per = ((N + c.chunks - 1) / c.chunks + 7) / 8 * 8;
   c.chunks = (N + c.per - 1) / c.per;
   return c;
 }
 
-// The kernel for a split: rows of one warp, of several warps of 256 threads, or (above 4096 channels) of up to 1024 threads, whose threads hold 16 channels each.
-#define LLSA_NORM_CASE(V_, R_, ...)                                                                 \
-  if (sp.vec == V_ && sp.r <= R_) {                                                                 \
-    constexpr int VEC = V_, R = R_;                                                                 \
-    if (sp.warps == 1) { constexpr bool MULTI = false; constexpr int TPB = 256; __VA_ARGS__; }      \
-    else { constexpr bool MULTI = true; constexpr int TPB = 256; __VA_ARGS__; }                     \
+// The kernel for a split.  Rows of one warp; of several warps of 256 threads; of 512, which has four groups of four; of all of 1024, above 4096 channels.
+#define LLSA_NORM_R(F_, R_, W_, T_, ...)                                                                        \
+  if (sp.form == F_ && sp.r <= R_ && (sp.warps > 1) == W_ && sp.threads == T_) {                                 \
+    constexpr int FORM = F_, R = R_, TPB = T_;                                                                  \
+    constexpr bool MULTI = W_;                                                                                  \
+    __VA_ARGS__;                                                                                                \
   }
-#define LLSA_NORM_KERNEL(...)                                                                       \
-  if (sp.threads > 256) {                                                                           \
-    constexpr bool MULTI = true;                                                                    \
-    constexpr int TPB = 1024;                                                                       \
-    if (sp.vec == 4) { constexpr int VEC = 4, R = 4; __VA_ARGS__; }                                 \
-    else { constexpr int VEC = 1, R = 16; __VA_ARGS__; }                                            \
-  } else                                                                                            \
-    LLSA_NORM_CASE(4, 1, __VA_ARGS__)                                                               \
-  else LLSA_NORM_CASE(4, 2, __VA_ARGS__)                                                            \
-  else LLSA_NORM_CASE(4, 3, __VA_ARGS__)                                                            \
-  else LLSA_NORM_CASE(4, 4, __VA_ARGS__)                                                            \
-  else LLSA_NORM_CASE(1, 4, __VA_ARGS__)                                                            \
-  else LLSA_NORM_CASE(1, 8, __VA_ARGS__)                                                            \
-  else LLSA_NORM_CASE(1, 12, __VA_ARGS__)                                                           \
-  else LLSA_NORM_CASE(1, 16, __VA_ARGS__)
+#define LLSA_NORM_KERNEL(...)                                                                                   \
+  LLSA_NORM_R(kWhole, 1, false, 256, __VA_ARGS__)                                                               \
+  else LLSA_NORM_R(kWhole, 2, false, 256, __VA_ARGS__)                                                          \
+  else LLSA_NORM_R(kWhole, 3, false, 256, __VA_ARGS__)                                                          \
+  else LLSA_NORM_R(kWhole, 4, false, 256, __VA_ARGS__)                                                          \
+  else LLSA_NORM_R(kWhole, 3, true, 256, __VA_ARGS__)                                                           \
+  else LLSA_NORM_R(kWhole, 4, true, 256, __VA_ARGS__)                                                           \
+  else LLSA_NORM_R(kLoose, 4, true, 1024, __VA_ARGS__)                                                          \
+  else LLSA_NORM_R(kShifted, 2, false, 256, __VA_ARGS__)                                                        \
+  else LLSA_NORM_R(kShifted, 4, false, 256, __VA_ARGS__)                                                        \
+  else LLSA_NORM_R(kShifted, 3, true, 256, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kShifted, 4, true, 256, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kShifted, 3, true, 512, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kShifted, 4, true, 512, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kSingle, 16, false, 256, __VA_ARGS__)                                                        \
+  else LLSA_NORM_R(kSingle, 16, true, 256, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kSingle, 16, true, 1024, __VA_ARGS__)                                                        \
+  else LLSA_REQUIRE(false, LLSA_ERR_SHAPE, "layer_norm: no kernel for %d channels", C);
 
 template <typename T>
 int launch_fwd(const LlsaTensor* x, const NormParams& par, float eps, const LlsaTensor* y, float2* stats, cudaStream_t st) {
   const uint32_t M = (uint32_t) (x->shape[0] * x->shape[1]), N = (uint32_t) x->shape[1];
   const int C = (int) x->shape[2];
-  const Split sp = split_of(C, rows_vec4<T>(x) && rows_vec4<T>(y));
+  const Split sp = split_for<T>(x, y);
   const int64_t groups = sp.threads / (32 * sp.warps);
-  const int64_t grid = std::min<int64_t>((M + groups - 1) / groups, 148 * (sp.threads > 256 ? 2 : 4));
   const Rows<const T> xr = make_rows<const T>(x);
   const Rows<T> yr = make_rows<T>(y);
-  LLSA_NORM_KERNEL(launch_pdl(layer_norm_fwd_kernel<T, VEC, R, MULTI, TPB>, dim3((unsigned) grid), dim3(sp.threads), 0, st, xr, par, eps, yr, stats, M, N, C,
-                              sp.warps))
+  LLSA_NORM_KERNEL({
+    // as many CTAs as the SMs hold at once, an equal share of rows each
+    const int64_t most = 148 * fwd_ctas(TPB, R * (FORM == kSingle ? 1 : 4)), per = ((M + most - 1) / most + groups - 1) / groups * groups, grid = (M + per - 1) / per;
+    launch_pdl(layer_norm_fwd_kernel<T, FORM, R, MULTI, TPB>, dim3((unsigned) grid), dim3(TPB), 0, st, xr, par, eps, yr, stats, M, N, (uint32_t) per, C, sp.warps);
+  })
   LLSA_LAUNCH_OK("layer_norm_fwd_kernel");
   return LLSA_OK;
 }
 
-template <typename T, bool SUMS>
+template <typename T>
 int launch_bwd(const LlsaTensor* dy, const LlsaTensor* x, const NormParams& par, const float2* stats, const LlsaTensor* dx, float* partial,
                const Chunks& ch, cudaStream_t st) {
   const int C = (int) x->shape[2];
-  const Split sp = split_of(C, rows_vec4<T>(x) && rows_vec4<T>(dy) && rows_vec4<T>(dx));
+  const Split sp = split_for<T>(x, dy, dx);
   const Rows<const T> gr = make_rows<const T>(dy), xr = make_rows<const T>(x);
   const Rows<T> dr = make_rows<T>(dx);
   const unsigned grid = (unsigned) (ch.B * ch.chunks);
-  LLSA_NORM_KERNEL(launch_pdl(layer_norm_bwd_kernel<T, VEC, R, MULTI, TPB, SUMS>, dim3(grid), dim3(sp.threads), 0, st, gr, xr, par, stats, dr, partial,
-                              (uint32_t) ch.N, (uint32_t) ch.chunks, (uint32_t) ch.per, C, sp.warps))
+  LLSA_NORM_KERNEL(launch_pdl(layer_norm_bwd_kernel<T, FORM, R, MULTI, TPB>, dim3(grid), dim3(TPB), 0, st, gr, xr, par, stats, dr, partial, (uint32_t) ch.N,
+                              (uint32_t) ch.chunks, (uint32_t) ch.per, C, sp.warps))
   LLSA_LAUNCH_OK("layer_norm_bwd_kernel");
   return LLSA_OK;
 }
@@ -412,7 +475,7 @@ extern "C" int llsa_layer_norm_fwd(const LlsaTensor* x, const LlsaTensor* weight
   if (shape[0] * shape[1] == 0) return LLSA_OK;
   float2* st = stats ? (float2*) stats->ptr : nullptr;
   return x->dtype == LLSA_F32 ? launch_fwd<float>(x, par, eps, y, st, (cudaStream_t) stream)
-                              : launch_fwd<__nv_bfloat16>(x, par, eps, y, st, (cudaStream_t) stream);
+                              : launch_fwd<bf16>(x, par, eps, y, st, (cudaStream_t) stream);
 }
 
 extern "C" int64_t llsa_layer_norm_bwd_partial_elems(int64_t B, int64_t N, int64_t C, int per_sample) {
@@ -468,10 +531,9 @@ extern "C" int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, co
   const float2* sv = (const float2*) stats->ptr;
   const cudaStream_t st = (cudaStream_t) stream;
   if (x->dtype == LLSA_F32)
-    rc = sums ? launch_bwd<float, true>(&f[0], &f[1], par, sv, &f[2], part, ch, st) : launch_bwd<float, false>(&f[0], &f[1], par, sv, &f[2], part, ch, st);
+    rc = launch_bwd<float>(&f[0], &f[1], par, sv, &f[2], part, ch, st);
   else
-    rc = sums ? launch_bwd<__nv_bfloat16, true>(&f[0], &f[1], par, sv, &f[2], part, ch, st)
-              : launch_bwd<__nv_bfloat16, false>(&f[0], &f[1], par, sv, &f[2], part, ch, st);
+    rc = launch_bwd<bf16>(&f[0], &f[1], par, sv, &f[2], part, ch, st);
   if (rc || !sums) return rc;
   return finish_column_grads(part, ch.B, ch.chunks, C, par.w, par.bias, par.scale, grads, st);
 }

@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include "linear.cuh"
+#include "vec.cuh"
 
 namespace llsa {
 
@@ -17,78 +18,111 @@ using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------ scalar products
 // fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of 256 threads owns a tile of
-// 16 TM x 16 TM outputs, a thread TM x TM of them (two groups of TM / 2 rows and columns, so that a warp's reads of shared memory are whole
-// vectors); steps of 16 along k, the next step's operands on their way in registers while this one's are multiplied.
-__device__ __forceinline__ void fetch(const Mat<const float>& m, int along_k, int64_t row0, int64_t rows, int64_t k0, int64_t k1, int r, int k, float& v) {
-  const int64_t i = row0 + r, kk = k0 + k;
-  v = i < rows && kk < k1 ? along_k ? m.p[i * m.ld + kk] : m.p[kk * m.ld + i] : 0.f;
-}
+// 16 TM x 16 TM outputs, a thread TM x TM of them.  Steps of 16 along k are copied ahead into a ring of buffers as they lie in
+// memory: rows of 16 k's (20 apart, so that eight rows' vectors fall into different banks; a thread's rows are then 16 apart), or 16 rows of
+// i's or j's (a thread's are then fours of neighbours).  TM^2 multiply-adds a k against TM / 2 vector loads of shared memory: the FMA pipe is what bounds it.
+template <int TM, bool ALONG_K>
+struct Operand {
+  static constexpr int kRows = 16 * TM, kK = 16, kLd = ALONG_K ? kK + 4 : kRows + 4, kFloats = ALONG_K ? kRows * kLd : kK * kLd;
+  static constexpr int kVecs = kRows * kK / 4;
+  // The place of the thread's u-th row (t: its number along the tile)
+  static __device__ __forceinline__ int row(int t, int u) { return ALONG_K ? t + 16 * u : TM >= 4 ? (u / 4) * 64 + 4 * t + u % 4 : 2 * t + u; }
+  static __device__ __forceinline__ void copy(float* buf, const Mat<const float>& m, int vec, int64_t row0, int64_t rows, int64_t k0, int64_t k1) {
+#pragma unroll
+    for (int v0 = 0; v0 < kVecs; v0 += 256) {
+      const int v = v0 + threadIdx.x;
+      if (kVecs < 256 && v >= kVecs) break;
+      const int r = ALONG_K ? v / 4 : v % (kRows / 4) * 4, k = ALONG_K ? v % 4 * 4 : v / (kRows / 4);
+      const int64_t i = row0 + r, kk = k0 + k;
+      const float* src = ALONG_K ? m.p + i * m.ld + kk : m.p + kk * m.ld + i;
+      const int n = ALONG_K ? (i < rows ? (int) max((int64_t) 0, min((int64_t) 4, k1 - kk)) : 0) : (kk < k1 ? (int) max((int64_t) 0, min((int64_t) 4, rows - i)) : 0);
+      const uint32_t dst = (uint32_t) __cvta_generic_to_shared(buf + (ALONG_K ? r * kLd + k : k * kLd + r));
+      if (vec) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(n ? src : m.p), "r"(4 * n) : "memory");
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * j), "l"(j < n ? src + j : m.p), "r"(j < n ? 4 : 0) : "memory");
+      }
+    }
+  }
+  // Four k's of the thread's TM rows
+  static __device__ __forceinline__ void read(const float* buf, int t, int k, float (&x)[4][TM]) {
+    if constexpr (ALONG_K) {
+#pragma unroll
+      for (int u = 0; u < TM; ++u) {
+        const float4 f = *reinterpret_cast<const float4*>(buf + (t + 16 * u) * kLd + k);
+        x[0][u] = f.x; x[1][u] = f.y; x[2][u] = f.z; x[3][u] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if constexpr (TM >= 4) {
+#pragma unroll
+          for (int u = 0; u < TM; u += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(buf + (k + j) * kLd + (u / 4) * 64 + 4 * t);
+            x[j][u] = f.x; x[j][u + 1] = f.y; x[j][u + 2] = f.z; x[j][u + 3] = f.w;
+          }
+        } else {
+          const float2 f = *reinterpret_cast<const float2*>(buf + (k + j) * kLd + 2 * t);
+          x[j][0] = f.x; x[j][1] = f.y;
+        }
+    }
+  }
+};
 
-template <int TM, bool PARTIAL>
+template <int TM, bool A_K, bool B_K, bool PARTIAL>
 __global__ void __launch_bounds__(256)
-product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split) {
-  constexpr int BM = 16 * TM, BK = 16, LD = BM + 4, NV = BM * BK / 256;
-  __shared__ float s_a[2][BK][LD], s_b[2][BK][LD];
-  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split, int vec_a, int vec_b) {
+  using A = Operand<TM, A_K>;
+  using B = Operand<TM, B_K>;
+  constexpr int BM = 16 * TM, BK = 16;
+  constexpr int kStages = TM >= 8 ? 2 : 4;                 // 41 KB of shared memory at most
+  __shared__ __align__(16) float s_a[kStages][A::kFloats], s_b[kStages][B::kFloats];
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int64_t i0 = blockIdx.x / tiles_n * BM, j0 = blockIdx.x % tiles_n * BM;
   const int64_t k_first = blockIdx.y * per_split, k_end = PARTIAL ? min(p.K, k_first + per_split) : p.K;
-  float acc[TM][TM], ra[NV], rb[NV];
+  float acc[TM][TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = 0.f;
   pdl_wait();
   pdl_trigger();
-  auto load = [&](int64_t k0) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int q = v * 256 + tid;
-      fetch(p.a, p.a_k, i0, p.M, k0, k_end, p.a_k ? q / BK : q % BM, p.a_k ? q % BK : q / BM, ra[v]);
-      fetch(p.b, p.b_k, j0, p.N, k0, k_end, p.b_k ? q / BK : q % BM, p.b_k ? q % BK : q / BM, rb[v]);
-    }
+  auto copy = [&](int buf, int64_t k0) {
+    A::copy(s_a[buf], p.a, vec_a, i0, p.M, k0, k_end);
+    B::copy(s_b[buf], p.b, vec_b, j0, p.N, k0, k_end);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto put = [&](int buf) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int q = v * 256 + tid;
-      s_a[buf][p.a_k ? q % BK : q / BM][p.a_k ? q / BK : q % BM] = ra[v];
-      s_b[buf][p.b_k ? q % BK : q / BM][p.b_k ? q / BK : q % BM] = rb[v];
-    }
-  };
-  load(k_first);
-  put(0);
-  __syncthreads();
+  for (int i = 0; i < kStages - 1; ++i) copy(i, k_first + i * BK);      // past the end: zeros, which nothing reads
   int buf = 0;
   for (int64_t k0 = k_first; k0 < k_end; k0 += BK) {
-    const bool more = k0 + BK < k_end;
-    if (more) load(k0 + BK);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();                                         // this step's operands are there, and the last one's have been read
+    copy(buf == 0 ? kStages - 1 : buf - 1, k0 + (kStages - 1) * BK);
 #pragma unroll
-    for (int k = 0; k < BK; ++k) {
-      float a[TM], b[TM];
+    for (int k = 0; k < BK; k += 4) {
+      float a[4][TM], b[4][TM];
+      A::read(s_a[buf], ty, k, a);
+      B::read(s_b[buf], tx, k, b);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        a[i] = s_a[buf][k][(i / (TM / 2)) * (BM / 2) + ty * (TM / 2) + i % (TM / 2)];
-        b[i] = s_b[buf][k][(i / (TM / 2)) * (BM / 2) + tx * (TM / 2) + i % (TM / 2)];
-      }
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+          for (int j = 0; j < TM; ++j) acc[i][j] = fmaf(a[q][i], b[q][j], acc[i][j]);
     }
-    if (more) {
-      put(buf ^ 1);
-      __syncthreads();
-      buf ^= 1;
-    }
+    if (++buf == kStages) buf = 0;
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int64_t r = i0 + (i / (TM / 2)) * (BM / 2) + ty * (TM / 2) + i % (TM / 2);
+    const int64_t r = i0 + A::row(ty, i);
     if (r >= p.M) continue;
     const int64_t sample = !PARTIAL && e.gate.p ? (uint32_t) r / e.rows_per_gate : 0;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      const int64_t c = j0 + (j / (TM / 2)) * (BM / 2) + tx * (TM / 2) + j % (TM / 2);
+      const int64_t c = j0 + B::row(tx, j);
       if (c >= p.N) continue;
       if constexpr (PARTIAL) {
         partial[(blockIdx.y * p.M + r) * partial_ld + c] = acc[i][j];
@@ -104,18 +138,20 @@ product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial,
   }
 }
 
-template <bool PARTIAL>
+template <bool A_K, bool B_K, bool PARTIAL>
 int launch_product(const Product<float>& p, const Epilogue<float>& e, float* partial, int64_t ld, cudaStream_t st) {
   const int64_t split = PARTIAL ? p.split : 1;
   auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
   const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
+  auto vec = [](const Mat<const float>& m) { return (uintptr_t) m.p % 16 == 0 && m.ld % 4 == 0; };
   auto go = [&](auto kernel, int64_t b) {
-    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(256), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per);
+    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(256), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per, (int) vec(p.a), (int) vec(p.b));
   };
   LLSA_REQUIRE(tiles(32) <= INT32_MAX, LLSA_ERR_SHAPE, "linear: too many outputs");
-  if (tiles(128) * split >= 148) go(product_kernel<8, PARTIAL>, 128);
-  else if (tiles(64) * split >= 148) go(product_kernel<4, PARTIAL>, 64);
-  else go(product_kernel<2, PARTIAL>, 32);
+  // the largest tile that still gives every SM one
+  if (tiles(128) * split >= 148) go(product_kernel<8, A_K, B_K, PARTIAL>, 128);
+  else if (tiles(64) * split >= 148) go(product_kernel<4, A_K, B_K, PARTIAL>, 64);
+  else go(product_kernel<2, A_K, B_K, PARTIAL>, 32);
   LLSA_LAUNCH_OK("product_kernel");
   return LLSA_OK;
 }
@@ -132,15 +168,11 @@ struct FrontArgs {
   int F, act, tx;              // tx: threads along the columns, a power of two
 };
 template <typename T, int V>
-struct alignas(V * sizeof(T)) Piece {
-  T v[V];
-};
-
-template <typename T, int V>
 __global__ void __launch_bounds__(256)
 linear_dz_kernel(FrontArgs<T> a) {
   constexpr int U = 4;
-  using P = Piece<T, V>;
+  using P = Vec<T, V>;
+  using Raw = typename P::type;
   extern __shared__ float s_part[];                        // [2][256 / tx][tx * V]
   const int tx = a.tx, lanes = 256 / tx, col = threadIdx.x % tx, lane = threadIdx.x / tx, c = (blockIdx.y * tx + col) * V;
   const uint32_t b = blockIdx.x / a.chunks, first = (blockIdx.x - b * a.chunks) * a.per, end = min(a.N, first + a.per);
@@ -153,31 +185,30 @@ linear_dz_kernel(FrontArgs<T> a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) gate[i] = a.gate.p ? to_f32<T>(a.gate.p[b * a.gate.ld + c + i]) : 1.f;
     for (uint32_t n0 = first + lane; n0 < end; n0 += U * lanes) {
-      P dy[U], pre[U];
+      Raw dy[U], pre[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (n0 + u * lanes < end) {
           const int64_t r = (int64_t) b * a.N + n0 + u * lanes;
-          dy[u] = *reinterpret_cast<const P*>(a.dy.p + r * a.dy.ld + c);
-          if (a.pre.p) pre[u] = *reinterpret_cast<const P*>(a.pre.p + r * a.pre.ld + c);
+          dy[u] = *reinterpret_cast<const Raw*>(a.dy.p + r * a.dy.ld + c);
+          if (a.pre.p) pre[u] = *reinterpret_cast<const Raw*>(a.pre.p + r * a.pre.ld + c);
         }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (n0 + u * lanes < end) {
-          P dz;
+          float g[V], z[V], d[V];
+          P::unpack(dy[u], g);
+          if (a.pre.p) P::unpack(pre[u], z);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float g = to_f32<T>(dy[u].v[i]);
-            float d = __fmul_rn(g, gate[i]);      // never contracted: the sums' bits do not depend on what else is asked for
+            d[i] = __fmul_rn(g[i], gate[i]);      // never contracted: the sums' bits do not depend on what else is asked for
             if (a.pre.p) {
-              const float z = to_f32<T>(pre[u].v[i]);
-              p[i] = fmaf(g, z, p[i]);
-              if constexpr (sizeof(T) == 4) d *= activate_grad(z, a.act);
+              p[i] = fmaf(g[i], z[i], p[i]);
+              if constexpr (sizeof(T) == 4) d[i] *= activate_grad(z[i], a.act);
             }
-            s[i] = __fadd_rn(s[i], d);
-            dz.v[i] = from_f32<T>(d);
+            s[i] = __fadd_rn(s[i], d[i]);
           }
-          if (a.dz.p) *reinterpret_cast<P*>(a.dz.p + ((int64_t) b * a.N + n0 + u * lanes) * a.dz.ld + c) = dz;
+          if (a.dz.p) *reinterpret_cast<Raw*>(a.dz.p + ((int64_t) b * a.N + n0 + u * lanes) * a.dz.ld + c) = P::pack(d);
         }
     }
   }
@@ -337,7 +368,7 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   }
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
   p->turned = false;
-  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 255) / 256));
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 127) / 128));
   p->part_ld = ((p->turned ? p->F : p->K) + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -359,12 +390,14 @@ Mat<T> mat(const LlsaTensor* t) {
   return m;
 }
 
-int product(const Product<float>& p, const Epilogue<float>& e, const LlsaLinearArgs*, cudaStream_t st) { return launch_product<false>(p, e, nullptr, 0, st); }
+int product(const Product<float>& p, const Epilogue<float>& e, const LlsaLinearArgs*, cudaStream_t st) {
+  return p.b_k ? launch_product<true, true, false>(p, e, nullptr, 0, st) : launch_product<true, false, false>(p, e, nullptr, 0, st);
+}
 int product(const Product<bf16>& p, const Epilogue<bf16>& e, const LlsaLinearArgs* a, cudaStream_t st) {
   return linear_tc_product(p, e, a->wait_limit, a->status, st);
 }
 int product_parts(const Product<float>& p, float* partial, int64_t ld, const LlsaLinearArgs*, cudaStream_t st) {
-  return launch_product<true>(p, Epilogue<float>{}, partial, ld, st);
+  return launch_product<false, false, true>(p, Epilogue<float>{}, partial, ld, st);
 }
 int product_parts(const Product<bf16>& p, float* partial, int64_t ld, const LlsaLinearArgs* a, cudaStream_t st) {
   return linear_tc_parts(p, partial, ld, a->wait_limit, a->status, st);

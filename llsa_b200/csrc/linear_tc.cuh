@@ -388,14 +388,16 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
           if (!steady_wait(&bars.avail[wg * 2 + b], (uint32_t) (seq >> 1) & 1, ctl)) break;
           if (IN && !out.tma_in) {                             // a warp's own rows, a row at a time
 #pragma unroll 1
-            for (int k = 0; k < 32; ++k) {
-              const int64_t rr = i0 + (warp & 3) * 32 + k;
-              const uint16_t* src = reinterpret_cast<const uint16_t*>(out.in.p + rr * out.in.ld + j0);
+            for (int k = 0; k < 32; k += 8) {                  // eight on their way at once
+              uint16_t u[16];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int x = lane + 32 * h;
-                *element(buf, (warp & 3) * 32 + k, x) = rr < M && x < cols ? src[x] : (uint16_t) 0;
+              for (int i = 0; i < 16; ++i) {
+                const int64_t rr = i0 + (warp & 3) * 32 + k + i / 2;
+                const int x = lane + 32 * (i & 1);
+                u[i] = rr < M && x < cols ? reinterpret_cast<const uint16_t*>(out.in.p + rr * out.in.ld + j0)[x] : (uint16_t) 0;
               }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) *element(buf, (warp & 3) * 32 + k + i / 2, lane + 32 * (i & 1)) = u[i];
             }
             __syncwarp();
           }
@@ -493,13 +495,15 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
           if (!out.tma_y) {
             __syncwarp();
 #pragma unroll 1
-            for (int k = 0; k < 32; ++k) {
-              const int64_t rr = i0 + (warp & 3) * 32 + k;
-              uint16_t* dst = reinterpret_cast<uint16_t*>(e.y.p + rr * e.y.ld + j0);
+            for (int k = 0; k < 32; k += 8) {
+              uint16_t u[16];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int x = lane + 32 * h;
-                if (rr < M && x < cols) dst[x] = *element(buf, (warp & 3) * 32 + k, x);
+              for (int i = 0; i < 16; ++i) u[i] = *element(buf, (warp & 3) * 32 + k + i / 2, lane + 32 * (i & 1));
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int64_t rr = i0 + (warp & 3) * 32 + k + i / 2;
+                const int x = lane + 32 * (i & 1);
+                if (rr < M && x < cols) reinterpret_cast<uint16_t*>(e.y.p + rr * e.y.ld + j0)[x] = u[i];
               }
             }
             tc::fence_async_smem();

@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "vec.cuh"
 
 namespace llsa {
 
@@ -35,37 +36,6 @@ struct Positions {
     if (kind == LLSA_I32) return (double) reinterpret_cast<const int32_t*>(p)[i];
     return (double) reinterpret_cast<const float*>(p)[i];
   }
-};
-
-template <typename T, int N>
-struct Vec;
-template <>
-struct Vec<bf16, 8> {
-  using type = uint4;
-  static __device__ __forceinline__ void unpack(const uint4& x, float* v) {
-    v[0] = bf16_lo(x.x); v[1] = bf16_hi(x.x); v[2] = bf16_lo(x.y); v[3] = bf16_hi(x.y);
-    v[4] = bf16_lo(x.z); v[5] = bf16_hi(x.z); v[6] = bf16_lo(x.w); v[7] = bf16_hi(x.w);
-  }
-  static __device__ __forceinline__ uint4 pack(const float* v) {
-    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-  }
-};
-template <>
-struct Vec<float, 4> {
-  using type = float4;
-  static __device__ __forceinline__ void unpack(const float4& x, float* v) { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
-  static __device__ __forceinline__ float4 pack(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
-};
-// two channels, element by element: rows on no particular boundary
-template <typename T>
-struct Two {
-  T a, b;
-};
-template <typename T>
-struct Vec<T, 2> {
-  using type = Two<T>;
-  static __device__ __forceinline__ void unpack(const Two<T>& x, float* v) { v[0] = to_f32<T>(x.a); v[1] = to_f32<T>(x.b); }
-  static __device__ __forceinline__ Two<T> pack(const float* v) { return Two<T>{from_f32<T>(v[0]), from_f32<T>(v[1])}; }
 };
 
 // Grid: x over (token, 16 bytes), y over parts of the B H rows of a token (per sample: of its H heads, times B).

@@ -183,13 +183,16 @@ def _register_fakes() -> None:
         return [x.new_empty(x.shape)] + [x.new_empty((C,) if i < 2 else (x.shape[0], C), dtype=types[i]) for i in range(4) if want >> i & 1]
 
     @torch.library.register_fake("llsa_b200::linear_fwd")
-    def _(x, weight, bias, residual, gate, activation, want_pre):
-        F = weight.shape[0]
-        y = x.new_empty((*x.shape[:-1], F))
-        return [y, x.new_empty((x.numel() // x.shape[-1], F))] if want_pre else [y]
+    def _(x, weight, bias, residual, gate, activation, want_pre, want_copies):
+        F, K = weight.shape
+        M = x.numel() // K
+        out = [x.new_empty((*x.shape[:-1], F))] + ([x.new_empty((M, F))] if want_pre else [])
+        if want_copies and x.dtype == torch.bfloat16 and K % 8:
+            out += [x.new_empty_strided((n, K), ((K + 7) // 8 * 8, 1)) for n in (M, F)]
+        return out
 
     @torch.library.register_fake("llsa_b200::linear_bwd")
-    def _(dy, x, weight, bias, pre, gate, activation, want):
+    def _(dy, x, weight, bias, pre, gate, x_copy, w_copy, activation, want):
         F = weight.shape[0]
         shapes = (x.shape, weight.shape, (F,), (x.shape[0] if gate is not None else 1, F))
         return [x.new_empty(shapes[i]) for i in range(4) if want >> i & 1]
@@ -501,7 +504,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if activation not in _ACTIVATIONS:
         raise ValueError("llsa_b200: activation must be None, 'gelu_tanh' or 'silu', got %r" % (activation,))
     _ready()
-    return torch.ops.llsa_b200.linear_fwd(x, weight, bias, residual, gate, _ACTIVATIONS[activation], False)[0]
+    return torch.ops.llsa_b200.linear_fwd(x, weight, bias, residual, gate, _ACTIVATIONS[activation], False, False)[0]
 
 
 # ----------------------------------------------------------------------------- selection
