@@ -18,102 +18,127 @@ using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------ scalar products
 // fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of 256 threads owns a tile of
-// 16 TM x 16 TM outputs, a thread TM x TM of them.  Steps of 16 along k are copied ahead into a ring of buffers as they lie in
-// memory: rows of 16 k's (20 apart, so that eight rows' vectors fall into different banks; a thread's rows are then 16 apart), or 16 rows of
-// i's or j's (a thread's are then fours of neighbours).  TM^2 multiply-adds a k against TM / 2 vector loads of shared memory: the FMA pipe is what bounds it.
+// 16 TM x 16 TM outputs, a thread TM x TM of them.  Steps of 16 along k: the next step's operands are on their way in registers while this one's are
+// multiplied from shared memory, where either stands as 16 rows of neighbours in i or j (turned on the way in if memory has it along k), so that a thread's
+// fours are one load.  TM^2 multiply-adds a k against TM / 2 such loads: the FMA pipe is what bounds it, with two CTAs to an SM.
 template <int TM, bool ALONG_K>
 struct Operand {
-  static constexpr int kRows = 16 * TM, kK = 16, kLd = ALONG_K ? kK + 4 : kRows + 4, kFloats = ALONG_K ? kRows * kLd : kK * kLd;
-  static constexpr int kVecs = kRows * kK / 4;
+  static constexpr int kRows = 16 * TM, kK = 16, kLd = kRows + 4, kFloats = kK * kLd;
+  static constexpr int kVecs = kRows * kK / 4, kMine = (kVecs + 255) / 256;
+  float4 x[kMine];
   // The place of the thread's u-th row (t: its number along the tile)
-  static __device__ __forceinline__ int row(int t, int u) { return ALONG_K ? t + 16 * u : TM >= 4 ? (u / 4) * 64 + 4 * t + u % 4 : 2 * t + u; }
-  static __device__ __forceinline__ void copy(float* buf, const Mat<const float>& m, int vec, int64_t row0, int64_t rows, int64_t k0, int64_t k1) {
+  static __device__ __forceinline__ int row(int t, int u) { return TM >= 4 ? (u / 4) * 64 + 4 * t + u % 4 : 2 * t + u; }
+  static __device__ __forceinline__ void place(int v, int& r, int& k) {
+    r = ALONG_K ? v / 4 : v % (kRows / 4) * 4;
+    k = ALONG_K ? v % 4 * 4 : v / (kRows / 4);
+  }
+  const float* src[kMine];      // of the next step
+  int have[kMine];              // rows, or columns of the four, that are there
+  __device__ __forceinline__ void begin(const Mat<const float>& m, int64_t row0, int64_t rows, int64_t k0) {
 #pragma unroll
-    for (int v0 = 0; v0 < kVecs; v0 += 256) {
-      const int v = v0 + threadIdx.x;
-      if (kVecs < 256 && v >= kVecs) break;
-      const int r = ALONG_K ? v / 4 : v % (kRows / 4) * 4, k = ALONG_K ? v % 4 * 4 : v / (kRows / 4);
-      const int64_t i = row0 + r, kk = k0 + k;
-      const float* src = ALONG_K ? m.p + i * m.ld + kk : m.p + kk * m.ld + i;
-      const int n = ALONG_K ? (i < rows ? (int) max((int64_t) 0, min((int64_t) 4, k1 - kk)) : 0) : (kk < k1 ? (int) max((int64_t) 0, min((int64_t) 4, rows - i)) : 0);
-      const uint32_t dst = (uint32_t) __cvta_generic_to_shared(buf + (ALONG_K ? r * kLd + k : k * kLd + r));
-      if (vec) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(n ? src : m.p), "r"(4 * n) : "memory");
+    for (int q = 0; q < kMine; ++q) {
+      const int v = q * 256 + threadIdx.x;
+      int r, k;
+      place(v, r, k);
+      const int64_t i = row0 + r, left = max((int64_t) 0, min((int64_t) 4, rows - i));
+      src[q] = ALONG_K ? m.p + i * m.ld + k0 + k : m.p + (k0 + k) * m.ld + i;
+      have[q] = kVecs < 256 && v >= kVecs ? 0 : ALONG_K ? (left ? 4 : 0) : (int) left;
+    }
+  }
+  // `left` k's are left
+  __device__ __forceinline__ void load(int64_t ld, int vec, int left) {
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) {
+      int r, k;
+      place(q * 256 + threadIdx.x, r, k);
+      const int n = ALONG_K ? min(have[q], left - k) : k < left ? have[q] : 0;
+      x[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (vec && n >= 4) {
+        x[q] = __ldg(reinterpret_cast<const float4*>(src[q]));
       } else {
+        if (n > 0) x[q].x = __ldg(src[q]);
+        if (n > 1) x[q].y = __ldg(src[q] + 1);
+        if (n > 2) x[q].z = __ldg(src[q] + 2);
+        if (n > 3) x[q].w = __ldg(src[q] + 3);
+      }
+      src[q] += ALONG_K ? kK : kK * ld;
+    }
+  }
+  __device__ __forceinline__ void put(float* buf) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * j), "l"(j < n ? src + j : m.p), "r"(j < n ? 4 : 0) : "memory");
+    for (int q = 0; q < kMine; ++q) {
+      const int v = q * 256 + threadIdx.x;
+      if (kVecs < 256 && v >= kVecs) break;
+      int r, k;
+      place(v, r, k);
+      if constexpr (ALONG_K) {
+        float* to = buf + k * kLd + r;
+        to[0] = x[q].x;
+        to[kLd] = x[q].y;
+        to[2 * kLd] = x[q].z;
+        to[3 * kLd] = x[q].w;
+      } else {
+        *reinterpret_cast<float4*>(buf + k * kLd + r) = x[q];
       }
     }
   }
-  // Four k's of the thread's TM rows
-  static __device__ __forceinline__ void read(const float* buf, int t, int k, float (&x)[4][TM]) {
-    if constexpr (ALONG_K) {
+  static __device__ __forceinline__ void read(const float* buf, int t, int k, float (&u)[TM]) {
+    if constexpr (TM >= 4) {
 #pragma unroll
-      for (int u = 0; u < TM; ++u) {
-        const float4 f = *reinterpret_cast<const float4*>(buf + (t + 16 * u) * kLd + k);
-        x[0][u] = f.x; x[1][u] = f.y; x[2][u] = f.z; x[3][u] = f.w;
+      for (int i = 0; i < TM; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(buf + k * kLd + (i / 4) * 64 + 4 * t);
+        u[i] = f.x; u[i + 1] = f.y; u[i + 2] = f.z; u[i + 3] = f.w;
       }
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if constexpr (TM >= 4) {
-#pragma unroll
-          for (int u = 0; u < TM; u += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(buf + (k + j) * kLd + (u / 4) * 64 + 4 * t);
-            x[j][u] = f.x; x[j][u + 1] = f.y; x[j][u + 2] = f.z; x[j][u + 3] = f.w;
-          }
-        } else {
-          const float2 f = *reinterpret_cast<const float2*>(buf + (k + j) * kLd + 2 * t);
-          x[j][0] = f.x; x[j][1] = f.y;
-        }
+      const float2 f = *reinterpret_cast<const float2*>(buf + k * kLd + 2 * t);
+      u[0] = f.x; u[1] = f.y;
     }
   }
 };
 
 template <int TM, bool A_K, bool B_K, bool PARTIAL>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split, int vec_a, int vec_b) {
   using A = Operand<TM, A_K>;
   using B = Operand<TM, B_K>;
   constexpr int BM = 16 * TM, BK = 16;
-  constexpr int kStages = TM >= 8 ? 2 : 4;                 // 41 KB of shared memory at most
-  __shared__ __align__(16) float s_a[kStages][A::kFloats], s_b[kStages][B::kFloats];
+  __shared__ __align__(16) float s_a[2][A::kFloats], s_b[2][B::kFloats];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int64_t i0 = blockIdx.x / tiles_n * BM, j0 = blockIdx.x % tiles_n * BM;
   const int64_t k_first = blockIdx.y * per_split, k_end = PARTIAL ? min(p.K, k_first + per_split) : p.K;
-  float acc[TM][TM];
+  float2 acc[TM][TM / 2];                                    // two neighbours an instruction, the same multiply-adds
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < TM / 2; ++j) acc[i][j] = make_float2(0.f, 0.f);
   pdl_wait();
   pdl_trigger();
-  auto copy = [&](int buf, int64_t k0) {
-    A::copy(s_a[buf], p.a, vec_a, i0, p.M, k0, k_end);
-    B::copy(s_b[buf], p.b, vec_b, j0, p.N, k0, k_end);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) copy(i, k_first + i * BK);      // past the end: zeros, which nothing reads
-  int buf = 0;
-  for (int64_t k0 = k_first; k0 < k_end; k0 += BK) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncthreads();                                         // this step's operands are there, and the last one's have been read
-    copy(buf == 0 ? kStages - 1 : buf - 1, k0 + (kStages - 1) * BK);
-#pragma unroll
-    for (int k = 0; k < BK; k += 4) {
-      float a[4][TM], b[4][TM];
-      A::read(s_a[buf], ty, k, a);
-      B::read(s_b[buf], tx, k, b);
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < TM; ++j) acc[i][j] = fmaf(a[q][i], b[q][j], acc[i][j]);
+  A a;
+  B b;
+  a.begin(p.a, i0, p.M, k_first);
+  b.begin(p.b, j0, p.N, k_first);
+  int buf = 0, left = (int) (k_end - k_first);               // of a part, or of the features: fewer than 2^31
+  a.load(p.a.ld, vec_a, left);
+  b.load(p.b.ld, vec_b, left);
+  for (; left > 0; buf ^= 1) {
+    a.put(s_a[buf]);
+    b.put(s_b[buf]);
+    __syncthreads();                                         // and the other buffer's readers are through
+    left -= BK;
+    if (left > 0) {
+      a.load(p.a.ld, vec_a, left);
+      b.load(p.b.ld, vec_b, left);
     }
-    if (++buf == kStages) buf = 0;
+#pragma unroll
+    for (int k = 0; k < BK; ++k) {
+      float u[TM], v[TM];
+      A::read(s_a[buf], ty, k, u);
+      B::read(s_b[buf], tx, k, v);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TM / 2; ++j) acc[i][j] = __ffma2_rn(make_float2(u[i], u[i]), make_float2(v[2 * j], v[2 * j + 1]), acc[i][j]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
@@ -124,10 +149,11 @@ product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial,
     for (int j = 0; j < TM; ++j) {
       const int64_t c = j0 + B::row(tx, j);
       if (c >= p.N) continue;
+      const float d = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
       if constexpr (PARTIAL) {
-        partial[(blockIdx.y * p.M + r) * partial_ld + c] = acc[i][j];
+        partial[(blockIdx.y * p.M + r) * partial_ld + c] = d;
       } else {
-        float z = acc[i][j] + (e.bias ? e.bias[c] : 0.f);
+        float z = d + (e.bias ? e.bias[c] : 0.f);
         if (e.pre.p) e.pre.p[r * e.pre.ld + c] = z;
         z = activate(z, e.act);
         if (e.gate.p) z *= e.gate.p[sample * e.gate.ld + c];
@@ -368,7 +394,7 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   }
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
   p->turned = false;
-  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min((148 * 2 + tiles - 1) / tiles, (p->M + 127) / 128));
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min(148 * 2 / tiles, (p->M + 127) / 128));      // one wave of two CTAs to an SM
   p->part_ld = ((p->turned ? p->F : p->K) + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {
