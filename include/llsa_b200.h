@@ -162,11 +162,12 @@ typedef struct LlsaLinearArgs {
   const LlsaTensor* gate;      /* [B,F], any row stride, or NULL: row b stands for rows [b M/B, (b+1) M/B); with a residual and no activation */
   const LlsaTensor* y;         /* [M,F] out, any row stride */
   const LlsaTensor* pre;       /* x weight^T + bias, [M,F] of x's type, contiguous: written by the forward if given (bf16: only with a gate), read by the
-                                  backward for dgate and, F32, through an activation; bf16 data compute it again there (bias as in the forward) */
+                                  backward for dgate or, F32, through an activation, where llsa_linear_keeps_product() is 1.  bf16 data compute it
+                                  again behind an activation, and do without it for a gate of long samples; both read bias, as in the forward */
   int32_t activation;          /* LlsaActivation */
   /* backward: dy in, those of the others that are not NULL out */
-  const LlsaTensor* dy;        /* [M,F], any row stride */
-  const LlsaTensor* dx;        /* [M,K], any row stride */
+  const LlsaTensor* dy;        /* [M,F], any row stride; for a gate of long bf16 samples (llsa_linear_keeps_product() is 0) rows on 16-byte boundaries */
+  const LlsaTensor* dx;        /* [M,K], likewise */
   const LlsaTensor* dweight;   /* [F,K] contiguous, x's type */
   const LlsaTensor* dbias;     /* [F] contiguous, F32 or x's type */
   const LlsaTensor* dgate;     /* [B,F] contiguous, F32 or x's type */
@@ -176,6 +177,8 @@ typedef struct LlsaLinearArgs {
   int32_t* status;
 } LlsaLinearArgs;
 int llsa_linear_fwd(const LlsaLinearArgs* args, void* stream);
+/* 1 where the backward reads `pre`, 0 where it does without, from the shapes of x, weight and gate and the activation; -1 where these are refused */
+int llsa_linear_keeps_product(const LlsaLinearArgs* args);
 /* Read from the shapes of x, weight and gate, dy, the activation and which results are wanted; -1 where these are refused */
 int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* args);
 int llsa_linear_bwd(const LlsaLinearArgs* args, void* stream);

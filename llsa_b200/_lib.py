@@ -58,7 +58,7 @@ EXPORTS = [
     "llsa_transpose_indices", "llsa_transpose_indices_pairs", "llsa_transpose_range_entries", "llsa_transpose_indices_noalloc", "llsa_attn_fwd", "llsa_attn_bwd",
     "llsa_attn_bwd_partial_elems", "llsa_attn_bwd_pds_elems", "llsa_attn_remainder_elems", "llsa_attn_fwd_redo_elems", "llsa_status_check",
     "llsa_rope_axes", "llsa_layer_norm_fwd", "llsa_layer_norm_bwd", "llsa_layer_norm_bwd_partial_elems",
-    "llsa_linear_fwd", "llsa_linear_bwd", "llsa_linear_bwd_workspace_bytes",
+    "llsa_linear_fwd", "llsa_linear_bwd", "llsa_linear_bwd_workspace_bytes", "llsa_linear_keeps_product",
 ]
 
 _lib: Optional[C.CDLL] = None
@@ -109,6 +109,7 @@ def _declare(lib: C.CDLL) -> None:
     lib.llsa_layer_norm_bwd.argtypes = [TP] * 12 + [C.c_void_p]
     lib.llsa_linear_fwd.argtypes = [C.POINTER(LlsaLinearArgs), C.c_void_p]
     lib.llsa_linear_bwd.argtypes = [C.POINTER(LlsaLinearArgs), C.c_void_p]
+    lib.llsa_linear_keeps_product.argtypes = [C.POINTER(LlsaLinearArgs)]
     lib.llsa_linear_bwd_workspace_bytes.argtypes = [C.POINTER(LlsaLinearArgs)]
     lib.llsa_linear_bwd_workspace_bytes.restype = C.c_int64
     for name in EXPORTS:

@@ -10,23 +10,26 @@ constexpr int kCols = 32, kLanes = 32;
 // blockIdx.y: 32 columns; blockIdx.x: a sample, or (the last one, with `overall`) all of them.  Thread (column, lane) adds every 32nd part;
 // the lanes are added in order through shared memory.
 __global__ void __launch_bounds__(kCols * kLanes)
-column_grads_kernel(const float* __restrict__ partial, int64_t B, int64_t chunks, int C, ParamView w, ParamView bias, ParamView s, ColumnGrads g,
-                    int overall) {
+column_grads_kernel(ColumnParts P, ColumnParts S, int64_t B, int C, ParamView w, ParamView bias, ParamView s, float plus, ColumnGrads g, int overall) {
   __shared__ float s_sum[2][kLanes][kCols + 1];
   const int col = threadIdx.x % kCols, lane = threadIdx.x / kCols, c = blockIdx.y * kCols + col;
   const bool all = overall && blockIdx.x == gridDim.x - 1;
-  const int64_t b = blockIdx.x, n = all ? B * chunks : chunks;
-  const float* p = partial + (all ? 0 : b * chunks * 2 * C) + c;
+  const int64_t b = blockIdx.x;
   float u = 0.f, v = 0.f;
+  auto add = [&](const ColumnParts& parts, int which, float& to) {
+    const int64_t n = all ? B * parts.chunks : parts.chunks;
+    const float* p = parts.p + (all ? 0 : b * parts.chunks * 2 * C) + which * C + c;
+#pragma unroll 4
+    for (int64_t i = lane; i < n; i += kLanes) {
+      const float f = all && s.p ? plus + s.at((uint32_t) (i / parts.chunks), c, 0.f) : 1.f;
+      to = fmaf(f, p[i * 2 * C], to);
+    }
+  };
   pdl_wait();
   pdl_trigger();
   if (c < C) {
-#pragma unroll 4
-    for (int64_t i = lane; i < n; i += kLanes) {
-      const float f = all && s.p ? 1.f + s.at((uint32_t) (i / chunks), c, 0.f) : 1.f;
-      u = fmaf(f, p[i * 2 * C], u);
-      v = fmaf(f, p[i * 2 * C + C], v);
-    }
+    if (all ? g.weight.p : g.scale.p) add(P, 0, u);
+    if (all ? g.bias.p != nullptr : g.shift.p || (g.scale.p && bias.p)) add(S, 1, v);
   }
   s_sum[0][lane][col] = u;
   s_sum[1][lane][col] = v;
@@ -71,13 +74,13 @@ int check_grad(const LlsaTensor* t, const char* name, int dtype, int ndim, const
   return check_contig(t, name, t->dtype, ndim, shape);
 }
 
-int finish_column_grads(const float* partial, int64_t B, int64_t chunks, int64_t C, const ParamView& w, const ParamView& bias, const ParamView& s,
+int finish_column_grads(const ColumnParts& P, const ColumnParts& S, int64_t B, int64_t C, const ParamView& w, const ParamView& bias, const ParamView& s, float plus,
                         const ColumnGrads& g, cudaStream_t st) {
   const int per_sample = g.scale.p || g.shift.p, overall = g.weight.p || g.bias.p;
   const int64_t slots = (per_sample ? B : 0) + overall;
   if (slots == 0) return LLSA_OK;
-  launch_pdl(column_grads_kernel, dim3((unsigned) slots, (unsigned) ((C + kCols - 1) / kCols)), dim3(kCols * kLanes), 0, st, partial, B, chunks, (int) C, w,
-             bias, s, g, overall);
+  launch_pdl(column_grads_kernel, dim3((unsigned) slots, (unsigned) ((C + kCols - 1) / kCols)), dim3(kCols * kLanes), 0, st, P, S, B, (int) C, w, bias,
+             s, plus, g, overall);
   LLSA_LAUNCH_OK("column_grads_kernel");
   return LLSA_OK;
 }

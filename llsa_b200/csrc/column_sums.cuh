@@ -41,9 +41,15 @@ inline GradView make_grad(const LlsaTensor* t) {
   return g;
 }
 
-// partial: [B * chunks][2][C], the sums P and S of a part of a sample's rows.  With P_b, S_b the sums of a sample's parts, added in order:
-//   scale_b = w P_b + bias S_b,  shift_b = S_b,  weight = sum_b (1 + s_b) P_b,  bias = sum_b (1 + s_b) S_b          (those that are wanted)
-int finish_column_grads(const float* partial, int64_t B, int64_t chunks, int64_t C, const ParamView& w, const ParamView& bias, const ParamView& s,
+// The sums P and S of parts of a sample's rows: P in partial[B * chunks][0][C] of one array, S in [B * chunks][1][C] of the same or another one
+struct ColumnParts {
+  const float* p;
+  int64_t chunks;
+};
+// With P_b, S_b the sums of a sample's parts, added in order:
+//   scale_b = w P_b + bias S_b,  shift_b = S_b,  weight = sum_b f_b P_b,  bias = sum_b f_b S_b          (those that are wanted)
+// f_b = plus + s_b, 1 where there is no s
+int finish_column_grads(const ColumnParts& P, const ColumnParts& S, int64_t B, int64_t C, const ParamView& w, const ParamView& bias, const ParamView& s, float plus,
                         const ColumnGrads& grads, cudaStream_t st);
 // The same of no rows at all
 int clear_column_grads(const ColumnGrads& grads, int64_t B, int64_t C, cudaStream_t st);

@@ -191,6 +191,22 @@ struct Shape {
                 "llsa_b200: gate must be [B, F] with x [B, ..., K]");
   }
 };
+// What the library says (llsa_linear_keeps_product), from sizes alone
+bool keeps_product(const Shape& s, at::ScalarType type, int64_t act, bool gate) {
+  if (s.M == 0) return false;
+  const int t = dtype_code(type);
+  char* at = (char*) 256;      // no memory is looked at
+  const LlsaTensor x = packed(at, t, {s.M, (s.K + 7) / 8 * 8}), w = packed(at, t, {s.F, (s.K + 7) / 8 * 8}), g = packed(at, t, {s.B, s.F});
+  LlsaTensor xk = x, wk = w;
+  xk.shape[1] = wk.shape[1] = s.K;
+  LlsaLinearArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = &xk; a.weight = &wk; a.activation = (int32_t) act;
+  if (gate) a.gate = &g;
+  const int keeps = llsa_linear_keeps_product(&a);
+  TORCH_CHECK(keeps >= 0, "llsa_b200.linear_fwd failed: ", llsa_last_error_string());
+  return keeps;
+}
 std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
   std::vector<int64_t> s = x.sizes().vec();
   s.back() = n;
@@ -224,7 +240,8 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
   TORCH_CHECK(!g_.defined() || act == LLSA_ACT_NONE, "llsa_b200: a gate goes with no activation");
   const c10::cuda::CUDAGuard guard(x_.device());
   std::vector<Tensor> out = {at::empty(shape, x_.options())};
-  if (want_pre) out.push_back(at::empty({s.M, s.F}, x_.options()));
+  const bool keep = want_pre && keeps_product(s, x_.scalar_type(), act, g_.defined());
+  if (want_pre) out.push_back(at::empty({keep ? s.M : 0, s.F}, x_.options()));
   if (s.M == 0) {
     if (want_copies && rows_want_copies(x_, s.K)) {
       out.push_back(padded({s.M, s.K}, x_));
@@ -242,7 +259,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x_, const Tensor& w_, const OptTens
   if (b_.defined()) { b = aligned_vector(b_); bd = desc(b); a.bias = &bd; }
   if (r_.defined()) { r = matrix(r_, s.M, s.F, false); rd = desc(r); a.residual = &rd; }
   if (g_.defined()) { g = unit_columns(g_); gd = desc(g); a.gate = &gd; }
-  if (want_pre) { pd = desc(out[1]); a.pre = &pd; }
+  if (keep) { pd = desc(out[1]); a.pre = &pd; }
   mark("linear");
   ok(llsa_linear_fwd(&a, at::cuda::getCurrentCUDAStream(x.device().index())), "linear_fwd");
   mark("end");
@@ -275,7 +292,9 @@ std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor
   if (want & 4) out.push_back(db = room({s.F}));
   if (want & 8) out.push_back(dg = room({s.B, s.F}));
   if (s.M == 0 || !want) return out;
-  const Tensor x = matrix(x_copy ? *x_copy : x_, s.M, s.K, true), w = matrix(w_copy ? *w_copy : w_, s.F, s.K, true), dy = matrix(dy_, s.M, s.F, false);
+  const Tensor x = matrix(x_copy ? *x_copy : x_, s.M, s.K, true), w = matrix(w_copy ? *w_copy : w_, s.F, s.K, true);
+  const bool long_samples = g_.defined() && !keeps_product(s, x_.scalar_type(), act, true);
+  const Tensor dy = matrix(dy_, s.M, s.F, long_samples);
   const Status status(x);
   LlsaLinearArgs a = linear_args(act, status);
   const LlsaTensor xd = desc(x), wd = desc(w), dyd = desc(dy);
@@ -289,7 +308,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy_, const Tensor& x_, const Tensor
     a.bias = &bd;
   }
   if (g_.defined()) { g = unit_columns(g_); gd = desc(g); a.gate = &gd; }
-  if (p_.defined()) {
+  if (p_.defined() && p_.numel()) {
     TORCH_CHECK(p_.dim() == 2 && p_.size(0) == s.M && p_.size(1) == s.F && p_.is_contiguous(), "llsa_b200.linear_bwd: `pre` is not from the matching linear_fwd");
     pd = desc(p_);
     a.pre = &pd;

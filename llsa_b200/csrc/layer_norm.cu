@@ -535,5 +535,5 @@ extern "C" int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, co
   else
     rc = launch_bwd<bf16>(&f[0], &f[1], par, sv, &f[2], part, ch, st);
   if (rc || !sums) return rc;
-  return finish_column_grads(part, ch.B, ch.chunks, C, par.w, par.bias, par.scale, grads, st);
+  return finish_column_grads({part, ch.chunks}, {part, ch.chunks}, ch.B, C, par.w, par.bias, par.scale, 1.f, grads, st);
 }

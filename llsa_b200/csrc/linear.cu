@@ -194,9 +194,9 @@ struct FrontArgs {
   int F, act, tx;              // tx: threads along the columns, a power of two
 };
 template <typename T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 linear_dz_kernel(FrontArgs<T> a) {
-  constexpr int U = 4;
+  constexpr int U = 8;
   using P = Vec<T, V>;
   using Raw = typename P::type;
   extern __shared__ float s_part[];                        // [2][256 / tx][tx * V]
@@ -308,6 +308,94 @@ int sum_parts(const float* partial, int64_t ld, int split, bool turned, int64_t 
   return LLSA_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ a gate by samples
+// Of long samples the gate is applied to what is small instead of to dy.  With G_b = dy_b^T x_b (the parts of dw, taken sample by sample) and S_b = sum_n dy:
+//   dx_b = dy_b (gate_b w),   dw = sum_b gate_b G_b,   dgate_b = rowsum(w G_b) + bias S_b,   dbias = sum_b gate_b S_b
+// so that the product of the forward is not kept, dz is neither written nor rounded, and what passes through memory for it is B weights and parts.
+// us, 131072 rows in 8 samples, 1536 -> 384, forward and backward: 562 with z kept and dz written.
+__global__ void __launch_bounds__(256)
+gated_weight_kernel(Mat<const bf16> w, Mat<const bf16> gate, bf16* __restrict__ out, int F, int K) {      // out [B][F][K]; K a multiple of 8
+  const int64_t i = blockIdx.x * (int64_t) blockDim.x + threadIdx.x, b = blockIdx.y;
+  const int per = K / 8;
+  pdl_wait();
+  pdl_trigger();
+  if (i >= (int64_t) F * per) return;
+  const int f = (int) (i / per), k = (int) (i % per) * 8;
+  float v[8];
+  Vec<bf16, 8>::unpack(*reinterpret_cast<const uint4*>(w.p + f * w.ld + k), v);
+  const float g = __bfloat162float(gate.p[b * gate.ld + f]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= g;
+  *reinterpret_cast<uint4*>(out + (b * F + f) * K + k) = Vec<bf16, 8>::pack(v);
+}
+
+// As sum_parts_kernel, `per_sample` parts of each of B samples weighed with its gate; and rowsum(w G_b) of the CTA's 32 columns in pg[B][columns / 32][0][F].
+// out, pg: NULL where not wanted.
+template <bool TURNED>
+__global__ void __launch_bounds__(256)
+gated_parts_kernel(const float* __restrict__ partial, int64_t ld, int per_sample, int B, int64_t F, int64_t K, Mat<const bf16> gate, Mat<const bf16> w,
+                   bf16* __restrict__ out, float* __restrict__ pg) {
+  __shared__ float s_tile[32][33];
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const int64_t f0 = blockIdx.y * (int64_t) 32, k0 = blockIdx.x * (int64_t) 32, part = (TURNED ? K : F) * ld;
+  pdl_wait();
+  pdl_trigger();
+  int64_t f[4], k[4];
+  bool there[4];
+  float wv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = f0 + (TURNED ? x : y + 8 * i);
+    k[i] = k0 + (TURNED ? y + 8 * i : x);
+    there[i] = f[i] < F && k[i] < K;
+    wv[i] = pg && there[i] ? __bfloat162float(w.p[f[i] * w.ld + k[i]]) : 0.f;
+  }
+  for (int b = 0; b < B; ++b) {
+    float u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < per_sample; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (there[i]) u[i] += partial[((int64_t) b * per_sample + s) * part + (TURNED ? k[i] * ld + f[i] : f[i] * ld + k[i])];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (there[i]) acc[i] = fmaf(__bfloat162float(gate.p[b * gate.ld + f[i]]), u[i], acc[i]);
+    if (pg) {
+      float* to = pg + ((int64_t) b * gridDim.x + blockIdx.x) * 2 * F;
+      if constexpr (TURNED) {
+        s_tile[y][x] = (wv[0] * u[0] + wv[1] * u[1]) + (wv[2] * u[2] + wv[3] * u[3]);
+        __syncthreads();
+        if (y == 0 && f[0] < F) {
+          float t = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t += s_tile[j][x];
+          to[f[0]] = t;
+        }
+        __syncthreads();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float t = wv[i] * u[i];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+          if (x == 0 && f[i] < F) to[f[i]] = t;
+        }
+      }
+    }
+  }
+  if (!out) return;
+  if constexpr (TURNED) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_tile[y + 8 * i][x] = acc[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = s_tile[x][y + 8 * i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (f0 + y + 8 * i < F && k0 + x < K) out[(f0 + y + 8 * i) * K + k0 + x] = __float2bfloat16_rn(acc[i]);
+}
+
 // ------------------------------------------------------------------------------------------------ checks and plan
 // A matrix with unit column stride
 int check_matrix(const LlsaTensor* t, const char* name, int dtype, int64_t rows, int64_t cols) {
@@ -330,8 +418,15 @@ struct Plan {
   int split;                   // dw: parts of the sum over the rows, of [F][part_ld], or turned [K][part_ld]
   bool turned;
   int64_t part_ld;
-  size_t o_dz, o_cols, o_parts, bytes;
+  bool by_sample;              // the gate is applied to the weight and to the parts of dw
+  int64_t k_tiles;
+  size_t o_dz, o_cols, o_parts, o_wg, o_pg, bytes;
 };
+
+// Long samples: twice as many rows as input features, what the B weights and parts cost beside z and dz; rows on 16-byte boundaries throughout
+bool by_sample(const LlsaLinearArgs* a, const Plan& p) {
+  return p.dtype == LLSA_BF16 && a->gate && p.N >= 512 && p.N >= 2 * p.K && p.K % 8 == 0 && p.F % 8 == 0;
+}
 
 int check_common(const LlsaLinearArgs* a, Plan* p) {
   LLSA_REQUIRE(a && a->x && a->x->ptr && a->weight && a->weight->ptr, LLSA_ERR_NULL, "linear: null argument");
@@ -371,13 +466,16 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   const int es = (int) dtype_size(p->dtype);
   // dy itself is dz without an activation and a gate, where the tensor cores can read it
   p->write_dz = a->activation != kActNone || a->gate || (p->dtype == LLSA_BF16 && !(a->dy && rows16(a->dy)));
-  p->sums = a->dbias || a->dgate;
+  p->by_sample = by_sample(a, *p);
+  if (p->by_sample) p->write_dz = false;
+  p->sums = p->by_sample ? a->dbias || (a->dgate && a->bias) : a->dbias || a->dgate;
   p->dz_ld = (p->F + 7) / 8 * 8;
   p->slope = p->dtype == LLSA_BF16 && a->activation != kActNone;
   if (p->slope) {
     p->chunks = linear_tc_slope_groups(p->M, p->F, p->K);
   } else {
-    // a CTA: tx threads along the columns, the width of 16, 32 or 64 that leaves the fewest idle; enough CTAs along the rows for 148 x 6, 16 rows a thread or more
+    // a CTA: tx threads along the columns, the width of 16, 32 or 64 that leaves the fewest idle; along the rows as many CTAs as the SMs hold at once, two,
+    // or of 16 rows a thread at least (U = 8 loads on their way a thread; 131072 x 384 sums in 26 us, with four and six CTAs and U = 4 51 and 54)
     p->vec = p->F % 8 == 0 && a->dy && rows16(a->dy) ? 16 / es : 1;
     int64_t idle = INT64_MAX;
     for (int tx : {64, 32, 16}) {
@@ -388,13 +486,13 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
       }
     }
     const int64_t cols = (p->F + p->tx * p->vec - 1) / (p->tx * p->vec), lanes = 256 / p->tx;
-    p->chunks = std::max<int64_t>(1, std::min((148 * 6 + cols * p->B - 1) / (cols * p->B), (p->N + 16 * lanes - 1) / (16 * lanes)));
+    p->chunks = std::max<int64_t>(1, std::min(148 * 2 / (cols * p->B), (p->N + 16 * lanes - 1) / (16 * lanes)));
     p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
     p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
   }
   const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
   p->turned = false;
-  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->M, &p->turned) : (int) std::max<int64_t>(1, std::min(148 * 2 / tiles, (p->M + 127) / 128));      // one wave of two CTAs to an SM
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->by_sample ? p->N : p->M, p->by_sample ? p->B : 0, &p->turned) : (int) std::max<int64_t>(1, std::min(148 * 2 / tiles, (p->M + 127) / 128));      // one wave of two CTAs to an SM
   p->part_ld = ((p->turned ? p->F : p->K) + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -404,7 +502,11 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   };
   p->o_dz = take(p->write_dz ? (size_t) (p->M * p->dz_ld * es) : 0);
   p->o_cols = take(p->sums ? (size_t) (p->B * p->chunks * 2 * p->F * 4) : 0);
-  p->o_parts = take(a->dweight ? (size_t) (p->split * (p->turned ? p->K : p->F) * p->part_ld * 4) : 0);
+  const bool parts = a->dweight || (p->by_sample && a->dgate);
+  p->o_parts = take(parts ? (size_t) ((p->by_sample ? p->B : 1) * p->split * (p->turned ? p->K : p->F) * p->part_ld * 4) : 0);
+  p->k_tiles = (p->K + 31) / 32;
+  p->o_wg = take(p->by_sample && a->dx ? (size_t) (p->B * p->F * p->K * es) : 0);
+  p->o_pg = take(p->by_sample && a->dgate ? (size_t) (p->B * p->k_tiles * 2 * p->F * 4) : 0);
   p->bytes = at;
 }
 
@@ -452,6 +554,55 @@ int slope(const LlsaLinearArgs* a, const Plan& p, const Mat<bf16>& dz, float* su
 }
 int slope(const LlsaLinearArgs*, const Plan&, const Mat<float>&, float*, cudaStream_t) { return LLSA_ERR_ARG; }      // not asked for
 
+int backward_by_sample(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
+  char* ws = (char*) a->workspace;
+  const Mat<const bf16> dy = mat<const bf16>(a->dy), x = mat<const bf16>(a->x), w = mat<const bf16>(a->weight), gate = mat<const bf16>(a->gate);
+  float* cols = p.sums ? (float*) (ws + p.o_cols) : nullptr;
+  int rc;
+  if (p.sums) {
+    FrontArgs<bf16> f = {};
+    f.dy = dy;
+    f.partial = cols;
+    f.N = (uint32_t) p.N; f.chunks = (uint32_t) p.chunks; f.per = (uint32_t) p.per;
+    f.F = (int) p.F;
+    rc = p.vec > 1 ? launch_dz<bf16, 8>(f, p.B * p.chunks, p.tx, st) : launch_dz<bf16, 1>(f, p.B * p.chunks, p.tx, st);
+    if (rc) return rc;
+  }
+  if (a->dx) {
+    bf16* wg = (bf16*) (ws + p.o_wg);
+    LLSA_REQUIRE(p.B <= 65535, LLSA_ERR_SHAPE, "linear_bwd: too many samples");
+    launch_pdl(gated_weight_kernel, dim3((unsigned) ((p.F * (p.K / 8) + 255) / 256), (unsigned) p.B), dim3(256), 0, st, w, gate, wg, (int) p.F, (int) p.K);
+    LLSA_LAUNCH_OK("gated_weight_kernel");
+    Epilogue<bf16> e = {};
+    e.y = mat<bf16>(a->dx);
+    Product<bf16> d = {dy, {wg, p.K}, 1, 0, p.N, p.K, p.F, 1};
+    d.samples = p.B;
+    if ((rc = product(d, e, a, st))) return rc;
+  }
+  if (a->dweight || a->dgate) {
+    float* parts = (float*) (ws + p.o_parts);
+    float* pg = a->dgate ? (float*) (ws + p.o_pg) : nullptr;
+    Product<bf16> d = p.turned ? Product<bf16>{x, dy, 0, 0, p.K, p.F, p.N, p.split} : Product<bf16>{dy, x, 0, 0, p.F, p.K, p.N, p.split};
+    d.samples = p.B;
+    if ((rc = product_parts(d, parts, p.part_ld, a, st))) return rc;
+    const dim3 grid((unsigned) p.k_tiles, (unsigned) ((p.F + 31) / 32));
+    bf16* dw = a->dweight ? (bf16*) a->dweight->ptr : nullptr;
+    launch_pdl(p.turned ? gated_parts_kernel<true> : gated_parts_kernel<false>, grid, dim3(256), 0, st, (const float*) parts, p.part_ld, p.split, (int) p.B, p.F, p.K,
+               gate, w, dw, pg);
+    LLSA_LAUNCH_OK("gated_parts_kernel");
+    if (pg) {
+      const ParamView none = {nullptr, 0, 0};
+      ParamView bias;
+      if ((rc = make_param(&bias, a->bias, "bias", p.dtype, 0, p.F))) return rc;
+      rc = finish_column_grads({pg, p.k_tiles}, {cols, p.chunks}, p.B, p.F, none, bias, none, 1.f, {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(nullptr)}, st);
+      if (rc) return rc;
+    }
+  }
+  if (!a->dbias) return LLSA_OK;
+  const ParamView none = {nullptr, 0, 0}, factor = {a->gate->ptr, gate.ld, 1};
+  return finish_column_grads({nullptr, 0}, {cols, p.chunks}, p.B, p.F, none, none, factor, 0.f, {make_grad(nullptr), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
+}
+
 template <typename T>
 int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
   char* ws = (char*) a->workspace;
@@ -480,7 +631,7 @@ int backward(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) {
     if (rc) return rc;
     if (p.sums) {
       const ParamView none = {nullptr, 0, 0};
-      rc = finish_column_grads(f.partial, p.B, p.chunks, p.F, none, none, none,
+      rc = finish_column_grads({f.partial, p.chunks}, {f.partial, p.chunks}, p.B, p.F, none, none, none, 1.f,
                                {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
       if (rc) return rc;
     }
@@ -519,6 +670,12 @@ extern "C" int llsa_linear_fwd(const LlsaLinearArgs* a, void* stream) {
   return p.dtype == LLSA_F32 ? forward<float>(a, p, (cudaStream_t) stream) : forward<bf16>(a, p, (cudaStream_t) stream);
 }
 
+extern "C" int llsa_linear_keeps_product(const LlsaLinearArgs* a) {
+  Plan p;
+  if (check_common(a, &p)) return -1;
+  return p.dtype == LLSA_F32 ? a->activation != kActNone || a->gate : a->gate && !by_sample(a, p);
+}
+
 extern "C" int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* a) {
   Plan p;
   if (check_common(a, &p)) return -1;
@@ -532,7 +689,9 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
   if (rc) return rc;
   plan_bwd(a, &p);
   if ((rc = check_matrix(a->dy, "dy", p.dtype, p.M, p.F))) return rc;
-  LLSA_REQUIRE(a->pre || !(a->dgate || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
+  LLSA_REQUIRE(!p.by_sample || rows16(a->dy), LLSA_ERR_STRIDE, "dy: rows must start on 16-byte boundaries for a gate of long samples");
+  LLSA_REQUIRE(!p.by_sample || !a->dx || rows16(a->dx), LLSA_ERR_STRIDE, "dx: rows must start on 16-byte boundaries for a gate of long samples");
+  LLSA_REQUIRE(a->pre || !((a->dgate && !p.by_sample) || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
   if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;
   const int64_t ws[2] = {p.F, p.K}, gs[2] = {p.B, p.F}, bs[1] = {p.F};
   if (a->dweight && (rc = check_contig(a->dweight, "dweight", p.dtype, 2, ws))) return rc;
@@ -548,5 +707,6 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
     return clear_column_grads({make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, a->gate ? a->gate->shape[0] : 0, p.F,
                               (cudaStream_t) stream);
   }
+  if (p.by_sample) return backward_by_sample(a, p, (cudaStream_t) stream);
   return p.dtype == LLSA_F32 ? backward<float>(a, p, (cudaStream_t) stream) : backward<bf16>(a, p, (cudaStream_t) stream);
 }

@@ -51,11 +51,13 @@ struct Product {
   Mat<const T> a, b;
   int a_k, b_k;
   int64_t M, N, K;
-  int split;                   // parts of the sum over k, one after another in `partial` (linear_sum_parts adds them); 1: none
+  int split;                   // parts of the sum over k, one after another in `partial`; 1: none
+  int64_t samples = 0;         // bf16: that many products of these sizes, their operands and results one behind the other (parts: `split` of each)
 };
 
 // bf16, on tcgen05 (linear_tc.cu).  Operands: rows on 16-byte boundaries.  The forward and the input's gradient (A along k), with their epilogue;
 int linear_tc_product(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, int wait_limit, int32_t* status, cudaStream_t st);
+// (with samples: the input's gradient alone, B along i or j).
 // dz = dy act'(z) with z computed once more, e.y = dz (rows on 16-byte boundaries), and the column sums of dz: sums[group][1][N], linear_tc_slope_groups of them;
 int linear_tc_slope(const Product<__nv_bfloat16>& p, const Epilogue<__nv_bfloat16>& e, const Mat<const __nv_bfloat16>& dy, float* sums, int wait_limit,
                     int32_t* status, cudaStream_t st);
@@ -63,6 +65,6 @@ int64_t linear_tc_slope_groups(int64_t M, int64_t N, int64_t K);
 // the weight's gradient (both operands across), in p.split parts of [M][ld], ld a multiple of 8; the number of parts to take
 int linear_tc_parts(const Product<__nv_bfloat16>& p, float* partial, int64_t ld, int wait_limit, int32_t* status, cudaStream_t st);
 // `turned`: the parts are better taken of the transposed result, A and B changing places
-int linear_tc_split(int64_t M, int64_t N, int64_t K, bool* turned);
+int linear_tc_split(int64_t M, int64_t N, int64_t K, int64_t samples, bool* turned);
 
 }  // namespace llsa

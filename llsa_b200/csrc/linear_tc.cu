@@ -31,13 +31,14 @@ namespace {
 int64_t step_cycles(int bn, bool pair) { return std::max(2 * bn, 256 + (pair ? bn : 2 * bn)); }
 
 // The tile, and with `parts` the number of parts, that a count of waves over 148 SMs says is the fastest.  in: the epilogue reads a tile as well
-Choice choose(int64_t M, int64_t N, int64_t k_blocks, int kind, bool in, bool act) {
+// samples: that many products of these sizes
+Choice choose(int64_t M, int64_t N, int64_t k_blocks, int kind, bool in, bool act, int64_t samples = 1) {
   Choice best = {128, false, 1, INT64_MAX};
   int64_t least = INT64_MAX;
   for (const Choice c : {Choice{64, false}, Choice{128, false}, Choice{192, true}, Choice{256, true}}) {
     if (kind == kSlope && c.bn != 128 && c.bn != 192) continue;
-    const int64_t units = c.pair ? 74 : 148, rows = c.pair ? 2 * kBM : kBM, tiles = (M + rows - 1) / rows * ((N + c.bn - 1) / c.bn);
-    const int64_t most = kind == kParts ? std::max<int64_t>(1, std::min<int64_t>(k_blocks / 4, units / std::min<int64_t>(tiles, units))) : 1;
+    const int64_t units = c.pair ? 74 : 148, rows = c.pair ? 2 * kBM : kBM, tiles = (M + rows - 1) / rows * ((N + c.bn - 1) / c.bn) * samples;
+    const int64_t most = kind == kParts ? std::max<int64_t>(1, std::min<int64_t>(k_blocks / 4, 4 * units / tiles)) : 1;
     for (int64_t s = 1; s <= most; ++s) {
       const int64_t waves = (tiles * s + units - 1) / units, steps = (k_blocks + s - 1) / s;
       // beside the steps: the epilogue's tile through the same port, a part written and read again (about 40 bytes a cycle of the SM); an activation takes two of
@@ -67,7 +68,8 @@ Outputs outputs(const Product<bf16>& p, const Epilogue<bf16>& e, const Mat<const
 
 int linear_tc_product(const Product<bf16>& p, const Epilogue<bf16>& e, int wait_limit, int32_t* status, cudaStream_t st) {
   Outputs out = outputs(p, e, e.residual);
-  const Choice c = choose(p.M, p.N, (p.K + kBK - 1) / kBK, kForward, e.residual.p != nullptr, e.act != kActNone);
+  const Choice c = choose(p.M, p.N, (p.K + kBK - 1) / kBK, kForward, e.residual.p != nullptr, e.act != kActNone, std::max<int64_t>(1, p.samples));
+  if (p.samples) return launch_choice<false, true, kForward, kActNone, false, false, 2, true>(c, p, out, wait_limit, status, st);
   if (!p.b_k) return launch_choice<false, true, kForward, kActNone, false, false, 2>(c, p, out, wait_limit, status, st);
   return launch_forward(c, p, out, wait_limit, status, st);
 }
@@ -85,9 +87,9 @@ int linear_tc_slope(const Product<bf16>& p, const Epilogue<bf16>& e, const Mat<c
                                : launch_choice<false, false, kSlope, kActSilu, true, false, 3>(c, p, out, wait_limit, status, st);
 }
 
-int linear_tc_split(int64_t M, int64_t N, int64_t K, bool* turned) {
-  const int64_t k_blocks = (K + kBK - 1) / kBK;
-  const Choice c = choose(M, N, k_blocks, kParts, false, false), d = choose(N, M, k_blocks, kParts, false, false);
+int linear_tc_split(int64_t M, int64_t N, int64_t K, int64_t samples, bool* turned) {
+  const int64_t k_blocks = (K + kBK - 1) / kBK, n = std::max<int64_t>(1, samples);
+  const Choice c = choose(M, N, k_blocks, kParts, false, false, n), d = choose(N, M, k_blocks, kParts, false, false, n);
   *turned = d.cost < c.cost;
   const int s = *turned ? d.split : c.split;
   const int64_t per = (k_blocks + s - 1) / s;
@@ -98,7 +100,9 @@ int linear_tc_parts(const Product<bf16>& p, float* partial, int64_t ld, int wait
   Outputs out = outputs(p, {}, {});
   out.partial = partial;
   out.ld = ld;
-  return launch_choice<true, true, kParts, kActNone, false, false, 2>(choose(p.M, p.N, (p.K + kBK - 1) / kBK, kParts, false, false), p, out, wait_limit, status, st);
+  const Choice c = choose(p.M, p.N, (p.K + kBK - 1) / kBK, kParts, false, false, std::max<int64_t>(1, p.samples));
+  return p.samples ? launch_choice<true, true, kParts, kActNone, false, false, 2, true>(c, p, out, wait_limit, status, st)
+                   : launch_choice<true, true, kParts, kActNone, false, false, 2>(c, p, out, wait_limit, status, st);
 }
 
 }  // namespace llsa

@@ -49,8 +49,8 @@ struct Outputs {
   Mat<const bf16> in;        // residual or dy
   float* partial;            // parts: [part][M][ld]; slope: [CTAs of a column][2][N], the sums in the second row
   int64_t ld;
-  int64_t M, N;
-  int tma_in, tma_y, vec_pre;
+  int64_t M, N;              // M: of a sample, where there are several
+  int vec_pre;
 };
 
 __device__ __forceinline__ void stg256(void* p, const uint32_t* r) {
@@ -71,8 +71,9 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float min_nan(float x, float m) {      // NaN stays
+__device__ __forceinline__ float clamp_nan(float x, float m) {      // to [-m, m]; NaN stays
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(m));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-m));
   return x;
 }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -89,14 +90,19 @@ __device__ __forceinline__ float2 activate2(float2 z) {
   else t = __fmul2_rn(z, two(-kLog2e));
   return __fmul2_rn(z, logistic2(t));
 }
+// s + z s (1 - s) u'(z).  Beyond +-7 (SiLU: +-30) the slope is 1 or within 4e-14 (3e-12) of 0, and z stays there: 2^t then stays below 2^52 and both of a pair's
+// reciprocals come from one.  The special functions, 16 a cycle, are what paces the kernel: three for two values instead of four.
 template <int ACT>
-__device__ __forceinline__ float2 slope2(float2 z) {      // s + z s (1 - s) u'(z)
-  float2 q = __fmul2_rn(z, z);
-  if constexpr (ACT == kActGeluTanh) q = make_float2(min_nan(q.x, 1e30f), min_nan(q.y, 1e30f));      // finite beside an s (1 - s) of 0
+__device__ __forceinline__ float2 slope2(float2 z) {
+  constexpr float kFar = ACT == kActGeluTanh ? 7.f : 30.f;
+  z = make_float2(clamp_nan(z.x, kFar), clamp_nan(z.y, kFar));
+  const float2 q = __fmul2_rn(z, z);
   float2 t;
   if constexpr (ACT == kActGeluTanh) t = __fmul2_rn(z, __ffma2_rn(q, two(-kGelu2 * kGelu3 * kLog2e), two(-kGelu2 * kLog2e)));
   else t = __fmul2_rn(z, two(-kLog2e));
-  const float2 s = logistic2(t);
+  const float2 d = __fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), two(1.f));
+  const float r = rcp(d.x * d.y);
+  const float2 s = make_float2(r * d.y, r * d.x);
   float2 w = __fmul2_rn(__fmul2_rn(z, s), __ffma2_rn(s, two(-1.f), two(1.f)));
   if constexpr (ACT == kActGeluTanh) w = __fmul2_rn(w, __ffma2_rn(q, two(3.f * kGelu3 * kGelu2), two(kGelu2)));
   return __fadd2_rn(w, s);
@@ -174,10 +180,12 @@ struct Chunks {
 // ------------------------------------------------------------------------------------------------ kernel
 // items: (part, row tile, column tile), columns fastest.  k_blocks: steps of 64; per_split: those of a part.
 // IN: the epilogue reads a tile (residual, dy); GATED: it multiplies by a gate and may keep z
-template <int BN, bool PAIR, bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G>
+// TMA: the movers bring and store the epilogue's tiles; else the epilogue's warps do, for rows that are on no 16-byte boundary.
+// SAMPLES: the maps have a third dimension, the sample; row tiles, or the parts of a sum over rows, are a sample's each, `per_sample` of them
+template <int BN, bool PAIR, bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES, bool TMA>
 __global__ void __launch_bounds__(Roles<G>::kThreads, 1)
 product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constant__ Outputs out, int k_blocks, int per_split, int tiles_n, int tiles, int items,
-                  int wait_limit, int32_t* status) {
+                  int per_sample, int wait_limit, int32_t* status) {
   using T = Tile<BN, PAIR, B_MN, KIND, G>;
   using R = Roles<G>;
   extern __shared__ unsigned char smem_dyn[];
@@ -218,9 +226,10 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
     uint32_t ph = 1;
     bool ok = true;
     for (Walk w(unit, units, tiles_n); ok && w.item < items; w.step()) {
-      const int split = KIND == kParts ? w.item / tiles : 0, i0 = (w.i - split * rows_m) * (kBM << PAIR) + row0, j0 = w.j * BN + rank * T::kBCols;
-      const int k_end = min(k_blocks, (split + 1) * per_split);
-      for (int kb = split * per_split; kb < k_end; ++kb) {
+      const int split = KIND == kParts ? w.item / tiles : 0, sample = SAMPLES ? (KIND == kParts ? split : w.i) / per_sample : 0;
+      const int i0 = (w.i - (KIND == kParts ? split * rows_m : sample * per_sample)) * (kBM << PAIR) + row0, j0 = w.j * BN + rank * T::kBCols;
+      const int part = KIND == kParts ? split - sample * per_sample : 0, k_end = min(k_blocks, (part + 1) * per_split);
+      for (int kb = part * per_split; kb < k_end; ++kb) {
         if (!(ok = tc::warp_wait(&bars.empty[st], ph, ctl))) break;
         bf16* a = ring + st * T::kStageElems;
         bf16* b = a + kBM * kBK;
@@ -228,7 +237,9 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
         if (rank == 0) tma::expect_tx_w(bar, (T::kStageElems * 2) << PAIR);
         const uint32_t to = PAIR ? tc::at_rank(bar, 0) : 0;
         auto load = [&](bf16* dst, const CUtensorMap* map, int c0, int c1) {
-          if constexpr (PAIR) tma::load_2d_pair_w(dst, map, to, c0, c1);
+          if constexpr (SAMPLES && PAIR) tma::load_3d_pair_w(dst, map, to, c0, c1, sample);
+          else if constexpr (SAMPLES) tma::load_3d_w(dst, map, bar, c0, c1, sample);
+          else if constexpr (PAIR) tma::load_2d_pair_w(dst, map, to, c0, c1);
           else tma::load_2d_w(dst, map, bar, c0, c1);
         };
         if constexpr (A_MN) {
@@ -262,7 +273,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
     uint32_t ph = 0, acc_ph = 1;
     bool ok = true;
     for (int item = unit; ok && rank == 0 && item < items; item += units) {
-      const int split = KIND == kParts ? item / tiles : 0, first = split * per_split, k_end = min(k_blocks, first + per_split);
+      const int split = KIND == kParts ? item / tiles : 0, first = (SAMPLES && KIND == kParts ? split % per_sample : split) * per_split, k_end = min(k_blocks, first + per_split);
       if (!(ok = tc::warp_wait(&bars.free_[acc], acc_ph, ctl))) break;
       for (int kb = first; kb < k_end; ++kb) {
         if (!(ok = tc::warp_wait(&bars.full[st], ph, ctl))) break;
@@ -284,7 +295,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
       Chunks<BN, KIND, G> head(Walk(unit, units, tiles_n), wg, items, (int) out.N), tail(head);
       auto prepare = [&](int b) {                              // the buffer for the chunk at `head`
         uint64_t* bar = &bars.avail[wg * 2 + b];
-        if (IN && out.tma_in) {
+        if (IN && TMA) {
           tma::expect_tx_w(bar, kChunkElems * 2);
           tma::load_2d_w(buffers + (wg * 2 + b) * kChunkElems, &maps.in, bar, head.j0(), head.w.i * (kBM << PAIR) + row0);
         } else if (lane == 0) {
@@ -298,10 +309,11 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
       for (int b = 0; tail.find(); ph ^= b, b ^= 1, tail.take()) {
         if (!steady_wait(&bars.done[wg * 2 + b], ph, ctl)) break;
         const bf16* buf = buffers + (wg * 2 + b) * kChunkElems;
-        const int i0 = tail.w.i * (kBM << PAIR) + row0;
-        const bool store = out.tma_y && i0 < out.M;
+        const int sample = SAMPLES ? tail.w.i / per_sample : 0, i0 = (tail.w.i - sample * per_sample) * (kBM << PAIR) + row0;
+        const bool store = TMA && i0 < out.M;
         if (store) {
-          tma::store_2d_w(&maps.y, tail.j0(), i0, tc::smem_u32(buf));
+          if constexpr (SAMPLES) tma::store_3d_w(&maps.y, tail.j0(), i0, sample, tc::smem_u32(buf));
+          else tma::store_2d_w(&maps.y, tail.j0(), i0, tc::smem_u32(buf));
           tma::reduce_commit_w();
         }
         if (store) tma::reduce_wait_read();
@@ -355,9 +367,9 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
     } else {
       const Epilogue<bf16>& e = out.e;
       const int t = tid & 127, M = (int) out.M, N = (int) out.N;
-      float sums[KIND == kSlope ? 16 : 1];                     // slope: of this thread's 16 columns and its rows, before they are rounded
+      float2 sums[KIND == kSlope ? 8 : 1];                     // slope: of this thread's 16 columns and its rows, before they are rounded
 #pragma unroll
-      for (int i = 0; i < (KIND == kSlope ? 16 : 1); ++i) sums[i] = 0.f;
+      for (int i = 0; i < (KIND == kSlope ? 8 : 1); ++i) sums[i] = two(0.f);
       int seq = 0;
       for (Chunks<BN, KIND, G> own(Walk(unit, units, tiles_n), wg, items, N); own.w.item < items; own.next_tile()) {
         const int i0 = own.w.i * (kBM << PAIR) + row0, r = i0 + row;
@@ -386,7 +398,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
           s_col[b][wg][t] = col[k0];
           asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
           if (!steady_wait(&bars.avail[wg * 2 + b], (uint32_t) (seq >> 1) & 1, ctl)) break;
-          if (IN && !out.tma_in) {                             // a warp's own rows, a row at a time
+          if constexpr (IN && !TMA) {                             // a warp's own rows, a row at a time
 #pragma unroll 1
             for (int k = 0; k < 32; k += 8) {                  // eight on their way at once
               uint16_t u[16];
@@ -406,7 +418,6 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
           if (!ok) {                                           // the products never came
 #pragma unroll
             for (int g = 0; g < 8; ++g) sts128(at ^ (g << 4), make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu));
-            sums[0] = __uint_as_float(0x7fffffffu);
           } else if constexpr (KIND == kSlope) {
             // Spread as the accumulators of small products are (tc05.cuh: tmem_ld_16x64), not a row to a thread: a thread then has 16 columns and not 64, whose
             // sums fit its registers and whose bias it unpacks once for four rows.  The buffer's 8 x 8 pieces go through ldmatrix and stmatrix
@@ -432,8 +443,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
                   const int jj = j + i / 2;
                   const float2 z = __fadd2_rn(make_float2(v[4 * jj + 2 * (i & 1)], v[4 * jj + 2 * (i & 1) + 1]), make_float2(bf16_lo(bias[jj]), bf16_hi(bias[jj])));
                   const float2 dz = __fmul2_rn(make_float2(bf16_lo(d[i]), bf16_hi(d[i])), slope2<ACT>(z));
-                  sums[2 * jj] += dz.x;
-                  sums[2 * jj + 1] += dz.y;
+                  sums[jj] = __fadd2_rn(sums[jj], dz);
                   d[i] = pack_bf16(dz.x, dz.y);
                 }
                 asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(d[0]), "r"(d[1]), "r"(d[2]), "r"(d[3]) : "memory");
@@ -492,7 +502,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
             read = last;
           }
           tc::fence_async_smem();                              // what TMA stores from here, and loads into here next
-          if (!out.tma_y) {
+          if constexpr (!TMA) {
             __syncwarp();
 #pragma unroll 1
             for (int k = 0; k < 32; k += 8) {
@@ -519,16 +529,19 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
       if constexpr (KIND == kSlope) {
         // the columns of a CTA stay the same (its units are a multiple of tiles_n): one sum over its rows.  Lanes 4 apart have the same columns
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sums[i] += ok ? 0.f : __uint_as_float(0x7fffffffu);
+        for (int i = 0; i < 8; ++i) {
+          if (!ok) sums[i] = two(__uint_as_float(0x7fffffffu));
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], o);
+          for (int o = 4; o < 32; o <<= 1) {
+            sums[i].x += __shfl_xor_sync(0xffffffffu, sums[i].x, o);
+            sums[i].y += __shfl_xor_sync(0xffffffffu, sums[i].y, o);
+          }
         }
         float* s_sum = reinterpret_cast<float*>(ring);         // the last product has read the ring
         asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (lane < 4) s_sum[warp * kChunk + 8 * (i / 2) + 2 * lane + (i & 1)] = sums[i];
+        for (int i = 0; i < 8; ++i)
+          if (lane < 4) *reinterpret_cast<float2*>(s_sum + warp * kChunk + 8 * i + 2 * lane) = sums[i];
         asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
         const int j = unit % tiles_n * BN + wg * kChunk + row;
         if (out.partial && wg < BN / kChunk && row < kChunk && j < N) {
@@ -566,55 +579,62 @@ inline int64_t slope_rows(int64_t M, int64_t N, int bn, bool pair) {
   return std::max<int64_t>(1, std::min((M + rows - 1) / rows, (pair ? 74 : 148) / tiles_n));
 }
 
-inline int matrix_map(CUtensorMap* m, const void* base, int64_t ld, int64_t rows, int64_t cols, uint32_t box_rows) {
-  const uint64_t dims[2] = {(uint64_t) cols, (uint64_t) rows}, strides[1] = {(uint64_t) ld * 2};
-  return tma::make_map(m, base, 2, dims, strides, box_rows);
+// samples: 0 for a matrix, else that many of them, `apart` elements from one to the next
+inline int matrix_map(CUtensorMap* m, const void* base, int64_t ld, int64_t rows, int64_t cols, uint32_t box_rows, int64_t samples, int64_t apart) {
+  const uint64_t dims[3] = {(uint64_t) cols, (uint64_t) rows, (uint64_t) samples}, strides[2] = {(uint64_t) ld * 2, (uint64_t) apart * 2};
+  return tma::make_map(m, base, samples ? 3 : 2, dims, strides, box_rows);
 }
 template <typename T>
 inline bool rows16(const Mat<T>& m) { return m.p && ((uintptr_t) m.p & 15) == 0 && m.ld % 8 == 0; }
 
-template <int BN, bool PAIR, bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G>
+template <int BN, bool PAIR, bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES, bool TMA>
 int launch(const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
   using T = Tile<BN, PAIR, B_MN, KIND, G>;
   using R = Roles<G>;
   ProductMaps maps;
-  int rc = A_MN ? matrix_map(&maps.a, p.a.p, p.a.ld, p.K, p.M, kBK) : matrix_map(&maps.a, p.a.p, p.a.ld, p.M, p.K, kBM);
+  int rc = A_MN ? matrix_map(&maps.a, p.a.p, p.a.ld, p.K, p.M, kBK, p.samples, p.K * p.a.ld) : matrix_map(&maps.a, p.a.p, p.a.ld, p.M, p.K, kBM, p.samples, p.M * p.a.ld);
   if (rc) return rc;
-  rc = B_MN ? matrix_map(&maps.b, p.b.p, p.b.ld, p.K, p.N, kBK) : matrix_map(&maps.b, p.b.p, p.b.ld, p.N, p.K, T::kBCols);
+  rc = B_MN ? matrix_map(&maps.b, p.b.p, p.b.ld, p.K, p.N, kBK, p.samples, p.K * p.b.ld) : matrix_map(&maps.b, p.b.p, p.b.ld, p.N, p.K, T::kBCols, 0, 0);
   if (rc) return rc;
   maps.in = maps.y = maps.a;
   if (KIND != kParts) {
-    out.tma_in = rows16(out.in);
-    out.tma_y = rows16(out.e.y);
     out.vec_pre = rows16(out.e.pre);
-    if (out.tma_in && (rc = matrix_map(&maps.in, out.in.p, out.in.ld, p.M, p.N, kBM))) return rc;
-    if (out.tma_y && (rc = matrix_map(&maps.y, out.e.y.p, out.e.y.ld, p.M, p.N, kBM))) return rc;
+    if (IN && TMA && (rc = matrix_map(&maps.in, out.in.p, out.in.ld, p.M, p.N, kBM, 0, 0))) return rc;
+    if (TMA && (rc = matrix_map(&maps.y, out.e.y.p, out.e.y.ld, p.M, p.N, kBM, p.samples, p.M * out.e.y.ld))) return rc;
   }
-  const auto kernel = product_tc_kernel<BN, PAIR, A_MN, B_MN, KIND, ACT, IN, GATED, G>;
+  const auto kernel = product_tc_kernel<BN, PAIR, A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, TMA>;
   LLSA_SMEM_LIMIT(kernel, T::kSmem);
   constexpr int64_t kRows = kBM << PAIR, kUnits = PAIR ? 74 : 148;
-  const int64_t tiles_n = (p.N + BN - 1) / BN, tiles = (p.M + kRows - 1) / kRows * tiles_n, k_blocks = (p.K + kBK - 1) / kBK;
+  const int64_t tiles_n = (p.N + BN - 1) / BN, k_blocks = (p.K + kBK - 1) / kBK, tiles_m = (p.M + kRows - 1) / kRows;
+  // samples: of their own row tiles, or (parts) of their own parts of the sum
+  const int64_t tiles = tiles_m * tiles_n * (SAMPLES && KIND != kParts ? p.samples : 1), parts = p.split * (SAMPLES && KIND == kParts ? p.samples : 1);
   LLSA_REQUIRE(p.N <= INT32_MAX / 2, LLSA_ERR_SHAPE, "linear: too many features");
-  const int64_t per = (k_blocks + p.split - 1) / p.split, items = tiles * p.split;
+  const int64_t per = (k_blocks + p.split - 1) / p.split, items = tiles * parts;
   LLSA_REQUIRE(items <= INT32_MAX / 4 && p.M <= INT32_MAX - 2 * kBM && p.N <= INT32_MAX - BN && p.K <= INT32_MAX - kBK, LLSA_ERR_SHAPE, "linear: too many outputs");
   const int64_t units = KIND == kSlope ? tiles_n * slope_rows(p.M, p.N, BN, PAIR) : std::min(items, kUnits);
   launch_pdl_cluster(kernel, dim3((unsigned) (units << PAIR)), dim3(R::kThreads), PAIR ? 2u : 1u, T::kSmem, st, maps, out, (int) k_blocks, (int) per, (int) tiles_n,
-                     (int) tiles, (int) items, wait_limit, status);
+                     (int) tiles, (int) items, (int) (KIND == kParts ? p.split : tiles_m), wait_limit, status);
   LLSA_LAUNCH_OK("product_tc_kernel");
   return LLSA_OK;
 }
 
 // The tiles that are built: 128 x 64 (not slope) and 128 x 128 of one CTA, 256 x 192 and 256 x 256 (not slope) of a pair
-template <bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G>
-int launch_choice(const Choice& c, const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
+template <bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES, bool TMA>
+int launch_tile(const Choice& c, const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
   if (c.pair) {
     if constexpr (KIND != kSlope)
-      if (c.bn == 256) return launch<256, true, A_MN, B_MN, KIND, ACT, IN, GATED, G>(p, out, wait_limit, status, st);
-    return launch<192, true, A_MN, B_MN, KIND, ACT, IN, GATED, G>(p, out, wait_limit, status, st);
+      if (c.bn == 256) return launch<256, true, A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, TMA>(p, out, wait_limit, status, st);
+    return launch<192, true, A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, TMA>(p, out, wait_limit, status, st);
   }
   if constexpr (KIND != kSlope)
-    if (c.bn == 64) return launch<64, false, A_MN, B_MN, KIND, ACT, IN, GATED, G>(p, out, wait_limit, status, st);
-  return launch<128, false, A_MN, B_MN, KIND, ACT, IN, GATED, G>(p, out, wait_limit, status, st);
+    if (c.bn == 64) return launch<64, false, A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, TMA>(p, out, wait_limit, status, st);
+  return launch<128, false, A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, TMA>(p, out, wait_limit, status, st);
+}
+template <bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES = false>
+int launch_choice(const Choice& c, const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
+  if constexpr (KIND == kParts || SAMPLES) return launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, true>(c, p, out, wait_limit, status, st);
+  return (!IN || rows16(out.in)) && rows16(out.e.y) ? launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, true>(c, p, out, wait_limit, status, st)
+                                                    : launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, false>(c, p, out, wait_limit, status, st);
 }
 // A forward with a long epilogue: by the length of its sums
 template <int ACT, bool IN, bool GATED>

@@ -96,6 +96,20 @@ __device__ __forceinline__ void load_2d_w(void* smem_dst, const CUtensorMap* map
                "l"(map), "r"((uint32_t) __cvta_generic_to_shared(mbar)), "r"(c0), "r"(c1)
                : "memory");
 }
+__device__ __forceinline__ void load_3d_w(void* smem_dst, const CUtensorMap* map, uint64_t* mbar, int c0, int c1, int c2) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(
+                   (uint32_t) __cvta_generic_to_shared(smem_dst)),
+               "l"(map), "r"((uint32_t) __cvta_generic_to_shared(mbar)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+__device__ __forceinline__ void load_3d_pair_w(void* smem_dst, const CUtensorMap* map, uint32_t mbar, int c0, int c1, int c2) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(
+                   (uint32_t) __cvta_generic_to_shared(smem_dst)),
+               "l"(map), "r"(mbar), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
 // A copy into this CTA's shared memory that completes on a barrier of the pair's other CTA, or of this one: `mbar` is its address in the cluster
 __device__ __forceinline__ void load_2d_pair_w(void* smem_dst, const CUtensorMap* map, uint32_t mbar, int c0, int c1) {
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
@@ -136,6 +150,11 @@ __device__ __forceinline__ void store_4d_w(const CUtensorMap* map, int c0, int c
 __device__ __forceinline__ void store_2d_w(const CUtensorMap* map, int c0, int c1, uint32_t smem_src) {
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
                "@e cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(smem_src)
+               : "memory");
+}
+__device__ __forceinline__ void store_3d_w(const CUtensorMap* map, int c0, int c1, int c2, uint32_t smem_src) {
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+               "@e cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\t}" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_src)
                : "memory");
 }
 __device__ __forceinline__ void reduce_commit_w() {

@@ -186,7 +186,11 @@ def _register_fakes() -> None:
     def _(x, weight, bias, residual, gate, activation, want_pre, want_copies):
         F, K = weight.shape
         M = x.numel() // K
-        out = [x.new_empty((*x.shape[:-1], F))] + ([x.new_empty((M, F))] if want_pre else [])
+        out = [x.new_empty((*x.shape[:-1], F))]
+        if want_pre:      # not kept for a gate of long samples (csrc/linear.cu: by_sample)
+            N = M // x.shape[0] if gate is not None and x.shape[0] else M
+            kept = not (x.dtype == torch.bfloat16 and gate is not None and N >= 512 and N >= 2 * K and K % 8 == 0 and F % 8 == 0) and M > 0
+            out.append(x.new_empty((M if kept else 0, F)))
         if want_copies and x.dtype == torch.bfloat16 and K % 8:
             out += [x.new_empty_strided((n, K), ((K + 7) // 8 * 8, 1)) for n in (M, F)]
         return out
@@ -500,7 +504,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x: [..., K]; weight: [F, K]; bias: [F]; activation: None, "gelu_tanh" or "silu"; residual: of y's shape [..., F]; gate: [B, F], a sample's
     factors for all of its tokens (x is then [B, ..., K]), with a residual and without an activation.  All of one type, float32 or
     bfloat16; sums are fp32.  Differentiable in all five.  For the gradient of a gate, and of float32 data through an activation, the product
-    is kept between the passes; bfloat16 data compute it again for an activation.  Rows that are no multiple of 16 bytes cost bfloat16 operands a copy."""
+    is kept between the passes; bfloat16 data compute it again for an activation and do without it for a gate of long samples.  Rows that are no multiple of 16 bytes cost bfloat16 operands a copy."""
     if activation not in _ACTIVATIONS:
         raise ValueError("llsa_b200: activation must be None, 'gelu_tanh' or 'silu', got %r" % (activation,))
     _ready()

@@ -183,7 +183,7 @@ def linear_reference(x, w, b, act, r, gate, dy=None):
 
 
 LINEAR_SHAPES = [(1, 1, 1, 1), (1, 1, 16, 16), (8, 1, 256, 384), (1, 5, 3, 7), (2, 65, 64, 64), (1, 128, 128, 192), (2, 130, 72, 200), (3, 77, 389, 133), (1, 300, 384, 3),
-                 (2, 100, 390, 256), (1, 257, 520, 1032), (5, 60, 1536, 384), (2, 1000, 384, 1152), (1, 2049, 40, 8)]
+                 (2, 100, 390, 256), (1, 257, 520, 1032), (5, 60, 1536, 384), (2, 1000, 384, 1152), (3, 777, 384, 200), (2, 600, 64, 320), (1, 1100, 520, 72), (5, 513, 256, 136), (1, 2049, 40, 8)]
 FORMS = [("plain", None, False, False), ("gelu", "gelu_tanh", False, False), ("silu", "silu", False, False), ("residual", None, True, False),
          ("gated", None, True, True), ("gelu residual", "gelu_tanh", True, False)]
 
