@@ -117,6 +117,15 @@ __device__ __forceinline__ void load_param(float (&v)[S::E], const ParamView& p,
     for (int e = 0; e < S::E; ++e) v[e] = absent;
   }
 }
+// Four channels of one
+__device__ __forceinline__ void load_param4(float (&v)[4], const ParamView& p, uint32_t b, float absent, int c, int C) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = absent;
+  if (!p.p || c >= C) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = p.is_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(p.p)[b * p.ld + c + j]) : reinterpret_cast<const float*>(p.p)[b * p.ld + c + j];
+}
 template <typename T>
 __device__ __forceinline__ int shift_of(const T* row) { return (int) ((uintptr_t) row / sizeof(T) & 3); }
 
@@ -143,18 +152,26 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], 
   }
 }
 
-// CTAs that an SM should hold, by threads and by values of a thread: registers are what decides
-constexpr int fwd_ctas(int tpb, int e) { return tpb > 256 ? 1 : e <= 12 ? 4 : 3; }
+// CTAs that an SM should hold, by threads, by values of a thread and their type: registers are what decides (fp32, 12 values: four CTAs 75 us, three 71.5)
+constexpr int fwd_ctas(int tpb, int form, int e, int bytes) {
+  return tpb > 256 ? 1 : form == kWhole ? (bytes == 2 || e <= 8 ? 4 : 3) : e <= 12 ? 4 : 3;
+}
 constexpr int bwd_ctas(int tpb) { return tpb > 256 ? 1 : 2; }
 
 // TPB: threads of a CTA; MULTI: more than one warp to a row.  A CTA takes rows [blockIdx.x * per, + per): neighbours, so that a group's sample, and with it A and
 // T, changes rarely.  (Rows a grid apart had them loaded for nearly every row: 8 x 16384 rows of 384 channels 77 us, 44 so.)
+// Measured (bf16 unless said): 8 x 16384 rows of 384 channels 39.6 us (5.1 TB/s), in fp32 71.5 (5.6); 8 x 16384 of 768 92.7; 2 x 8192 of 2048 35.6; with A and T
+// in registers, which spill, 43.6, 81.7, 105 and 40.6.  Two rows on their way are worth 1 us of the first and cost 12 of the 768 channels' 93.
 template <typename T, int FORM, int R, bool MULTI, int TPB>
-__global__ void __launch_bounds__(TPB, fwd_ctas(TPB, R * (FORM == kSingle ? 1 : 4)))
+__global__ void __launch_bounds__(TPB, fwd_ctas(TPB, FORM, R * (FORM == kSingle ? 1 : 4), sizeof(T)))
 layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, float2* __restrict__ stats, uint32_t M, uint32_t N, uint32_t per, int C, int warps) {
   using S = Slice<T, FORM, R>;
   constexpr int E = S::E;
+  // whole vectors: A and T lie in shared memory, each thread's own, and leave their registers to the rows; rows of one warp have two on their way
+  constexpr bool KEEP = FORM == kWhole;
+  constexpr int DEPTH = FORM == kWhole && R <= 3 && !MULTI && sizeof(T) == 2 ? 2 : 1;
   __shared__ float s_red[2][32][2];
+  __shared__ float4 s_par[KEEP ? 2 * R * TPB : 1];
   const int threads = MULTI ? 32 * warps : 32, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = TPB / threads;
   const float inv_c = 1.f / (float) C;
   const uint32_t end = min(M, (blockIdx.x + 1) * per);
@@ -163,16 +180,11 @@ layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, flo
   pdl_trigger();
   float2 a[E / 2], sh[E / 2];
   uint32_t cur = ~0u, r = blockIdx.x * per + group, b = r / N, n = r - b * N;
-  S raw;
-  if (r < end) {
-    const T* row = x.row(b, n);
-    if (FORM == kShifted) m = shift_of(row);                   // of all the group's rows: they are a multiple of four apart
-    raw.load(row, t, threads, C, m);
-  }
-  while (r < end) {
-    const uint32_t rb = b, rn = n, rr = r;
-    float2 v[E / 2];
-    raw.values(v, t, threads, C, m);
+  S raw[DEPTH];
+  uint32_t sb[DEPTH], sn[DEPTH];                               // whose they are
+  const auto fetch = [&](int d) {                              // the next row into place d
+    sb[d] = b, sn[d] = n;
+    if (r < end) raw[d].load(x.row(b, n), t, threads, C, m);
     r += groups;
     n += groups;
     if (n >= N) {
@@ -180,54 +192,98 @@ layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, flo
       b += q;
       n -= q * N;
     }
-    if (r < end) raw.load(x.row(b, n), t, threads, C, m);
-    if (rb != cur) {
-      cur = rb;
-      float u[E], w[E];
-      load_param<S>(u, par.scale, rb, 0.f, t, threads, C, m);
-      load_param<S>(w, par.w, 0, 1.f, t, threads, C, m);
+  };
+  if (FORM == kShifted && r < end) m = shift_of(x.row(b, n));  // of all the group's rows: they are a multiple of four apart
+  const uint32_t mine = r < end ? (end - r + groups - 1) / groups : 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(a)[e] = w[e] * (1.f + u[e]);
-      load_param<S>(w, par.bias, 0, 0.f, t, threads, C, m);
+  for (int d = 0; d < DEPTH; ++d) fetch(d);
+  for (uint32_t i0 = 0; i0 < mine; i0 += DEPTH) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] = w[e] * (1.f + u[e]);
-      load_param<S>(u, par.shift, rb, 0.f, t, threads, C, m);
+    for (int d = 0; d < DEPTH; ++d) {
+      if (d && i0 + d >= mine) break;
+      const uint32_t rb = sb[d], rn = sn[d];
+      float2 v[E / 2];
+      raw[d].values(v, t, threads, C, m);
+      fetch(d);
+      if (rb != cur) {
+        cur = rb;
+        if constexpr (KEEP) {
+#pragma unroll 1
+          for (int i = 0; i < R; ++i) {
+            const int c = (i * threads + t) * 4;
+            float u[4], w[4], bias[4], shift[4];
+            load_param4(u, par.scale, rb, 0.f, c, C);
+            load_param4(w, par.w, 0, 1.f, c, C);
+            load_param4(bias, par.bias, 0, 0.f, c, C);
+            load_param4(shift, par.shift, rb, 0.f, c, C);
 #pragma unroll
-      for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] += u[e];
+            for (int j = 0; j < 4; ++j) {
+              w[j] *= 1.f + u[j];
+              bias[j] = fmaf(bias[j], 1.f + u[j], shift[j]);
+            }
+            s_par[2 * i * TPB + threadIdx.x] = make_float4(w[0], w[1], w[2], w[3]);
+            s_par[(2 * i + 1) * TPB + threadIdx.x] = make_float4(bias[0], bias[1], bias[2], bias[3]);
+          }
+        } else {
+          float u[E], w[E];
+          load_param<S>(u, par.scale, rb, 0.f, t, threads, C, m);
+          load_param<S>(w, par.w, 0, 1.f, t, threads, C, m);
+#pragma unroll
+          for (int e = 0; e < E; ++e) reinterpret_cast<float*>(a)[e] = w[e] * (1.f + u[e]);
+          load_param<S>(w, par.bias, 0, 0.f, t, threads, C, m);
+#pragma unroll
+          for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] = w[e] * (1.f + u[e]);
+          load_param<S>(u, par.shift, rb, 0.f, t, threads, C, m);
+#pragma unroll
+          for (int e = 0; e < E; ++e) reinterpret_cast<float*>(sh)[e] += u[e];
+        }
+      }
+      float2 s2 = v[0];
+#pragma unroll
+      for (int i = 1; i < E / 2; ++i) s2 = __fadd2_rn(s2, v[i]);
+      float s[1] = {s2.x + s2.y};
+      group_sum<MULTI>(s, s_red, turn, warps, group);
+      const float mean = s[0] * inv_c;
+      float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        v[i] = __fadd2_rn(v[i], make_float2(-mean, -mean));
+        float2 u = v[i];                                         // what is not there stays out of the squares
+        if (!S::there(2 * i, S::channel(2 * i, t, threads, m), C)) u.x = 0.f;
+        if (!S::there(2 * i + 1, S::channel(2 * i + 1, t, threads, m), C)) u.y = 0.f;
+        q2 = __ffma2_rn(u, u, q2);
+      }
+      float q[1] = {q2.x + q2.y};
+      group_sum<MULTI>(q, s_red, turn, warps, group);
+      const float rstd = rsqrtf(fmaf(q[0], inv_c, eps));
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        float2 ai = a[i], ti = sh[i];
+        if constexpr (KEEP) {
+          const float4 pa = s_par[i / 2 * 2 * TPB + threadIdx.x], pt = s_par[(i / 2 * 2 + 1) * TPB + threadIdx.x];
+          ai = i & 1 ? make_float2(pa.z, pa.w) : make_float2(pa.x, pa.y);
+          ti = i & 1 ? make_float2(pt.z, pt.w) : make_float2(pt.x, pt.y);
+        }
+        v[i] = __ffma2_rn(__fmul2_rn(v[i], make_float2(rstd, rstd)), ai, ti);
+      }
+      S::store(y.row(rb, rn), v, t, threads, C, m);
+      if (stats && t == 0) stats[(uint64_t) rb * N + rn] = make_float2(mean, rstd);
     }
-    float2 s2 = v[0];
-#pragma unroll
-    for (int i = 1; i < E / 2; ++i) s2 = __fadd2_rn(s2, v[i]);
-    float s[1] = {s2.x + s2.y};
-    group_sum<MULTI>(s, s_red, turn, warps, group);
-    const float mean = s[0] * inv_c;
-    float2 q2 = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      v[i] = __fadd2_rn(v[i], make_float2(-mean, -mean));
-      float2 u = v[i];                                         // what is not there stays out of the squares
-      if (!S::there(2 * i, S::channel(2 * i, t, threads, m), C)) u.x = 0.f;
-      if (!S::there(2 * i + 1, S::channel(2 * i + 1, t, threads, m), C)) u.y = 0.f;
-      q2 = __ffma2_rn(u, u, q2);
-    }
-    float q[1] = {q2.x + q2.y};
-    group_sum<MULTI>(q, s_red, turn, warps, group);
-    const float rstd = rsqrtf(fmaf(q[0], inv_c, eps));
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) v[i] = __ffma2_rn(__fmul2_rn(v[i], make_float2(rstd, rstd)), a[i], sh[i]);
-    S::store(y.row(rb, rn), v, t, threads, C, m);
-    if (stats && t == 0) stats[rr] = make_float2(mean, rstd);
   }
 }
 
 // A CTA takes rows [s * per, (s + 1) * per) of sample b, chunk = b * chunks + s, and leaves its two column sums in partial[chunk][2][C] (NULL: none are wanted).
 // Of shifted rows every group holds other channels in a thread than its neighbour: the sums meet by channel in shared memory.
+// Measured, the parameters' gradients included (bf16 unless said): 8 x 16384 rows of 384 channels 58.4 us (5.2 TB/s), in fp32 99.6 (6.1); 8 x 16384 of 768 123.6;
+// 2 x 8192 of 2048 53.5; 3 x 5377 of 1155 in fp32, shifted, 56.  With one row on its way instead of two 68.3 and 131.5 (384 and 768); of 16 values to a
+// thread, or of fp32, two rows spill (2048: 84.7, fp32 115).
 template <typename T, int FORM, int R, bool MULTI, int TPB>
 __global__ void __launch_bounds__(TPB, bwd_ctas(TPB))
 layer_norm_bwd_kernel(Rows<const T> dy, Rows<const T> x, NormParams par, const float2* __restrict__ stats, Rows<T> dx, float* __restrict__ partial,
                       uint32_t N, uint32_t chunks, uint32_t per, int C, int warps) {
   using S = Slice<T, FORM, R>;
   constexpr int E = S::E;
+  constexpr int DEPTH = FORM == kWhole && R <= 3 && sizeof(T) == 2 ? 2 : 1;       // rows on their way
   __shared__ float s_red[2][32][2];
   __shared__ float s_col[TPB > 512 ? 1 : 16 * TPB];
   const int threads = MULTI ? 32 * warps : 32, group = threadIdx.x / threads, t = threadIdx.x - group * threads, groups = TPB / threads;
@@ -248,41 +304,48 @@ layer_norm_bwd_kernel(Rows<const T> dy, Rows<const T> x, NormParams par, const f
   }
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) p[i] = sum[i] = make_float2(0.f, 0.f);
-  S rx, rg;
-  float2 rs = make_float2(0.f, 0.f);
-  if (n < end) {
-    rx.load(x.row(b, n), t, threads, C, m);
-    rg.load(dy.row(b, n), t, threads, C, m);
-    rs = stats[(uint64_t) b * N + n];
-  }
+  S rx[DEPTH], rg[DEPTH];
+  float2 rst[DEPTH];
+  uint32_t ahead = n;
+  const auto fetch = [&](int d) {                              // the next row into place d
+    if (ahead < end) {
+      rx[d].load(x.row(b, ahead), t, threads, C, m);
+      rg[d].load(dy.row(b, ahead), t, threads, C, m);
+      rst[d] = stats[(uint64_t) b * N + ahead];
+    }
+    ahead += groups;
+  };
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) fetch(d);
   while (n < end) {
-    const uint32_t rn = n;
-    float2 h[E / 2], g[E / 2];
-    rx.values(h, t, threads, C, m);
-    rg.values(g, t, threads, C, m);
-    const float2 minus = make_float2(-rs.x, -rs.x), r2 = make_float2(rs.y, rs.y);
-    n += groups;
-    if (n < end) {
-      rx.load(x.row(b, n), t, threads, C, m);
-      rg.load(dy.row(b, n), t, threads, C, m);
-      rs = stats[(uint64_t) b * N + n];
-    }
-    float2 m1 = make_float2(0.f, 0.f), m2 = m1;
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      h[i] = __fmul2_rn(__fadd2_rn(h[i], minus), r2);
-      p[i] = __ffma2_rn(g[i], h[i], p[i]);
-      sum[i] = __fadd2_rn(sum[i], g[i]);
-      g[i] = __fmul2_rn(g[i], a[i]);                           // 0 where nothing is there
-      m1 = __fadd2_rn(m1, g[i]);
-      m2 = __ffma2_rn(g[i], h[i], m2);
-    }
-    float s[2] = {m1.x + m1.y, m2.x + m2.y};
-    group_sum<MULTI>(s, s_red, turn, warps, group);
-    const float2 k1 = make_float2(-s[0] * inv_c, -s[0] * inv_c), k2 = make_float2(-s[1] * inv_c, -s[1] * inv_c);
+    for (int d = 0; d < DEPTH; ++d) {
+      if (d && n >= end) break;
+      const uint32_t rn = n;
+      const float2 rs = rst[d];
+      float2 h[E / 2], g[E / 2];
+      rx[d].values(h, t, threads, C, m);
+      rg[d].values(g, t, threads, C, m);
+      const float2 minus = make_float2(-rs.x, -rs.x), r2 = make_float2(rs.y, rs.y);
+      n += groups;
+      fetch(d);
+      float2 m1 = make_float2(0.f, 0.f), m2 = m1;
 #pragma unroll
-    for (int i = 0; i < E / 2; ++i) g[i] = __fmul2_rn(r2, __ffma2_rn(h[i], k2, __fadd2_rn(g[i], k1)));
-    S::store(dx.row(b, rn), g, t, threads, C, m);
+      for (int i = 0; i < E / 2; ++i) {
+        h[i] = __fmul2_rn(__fadd2_rn(h[i], minus), r2);
+        p[i] = __ffma2_rn(g[i], h[i], p[i]);
+        sum[i] = __fadd2_rn(sum[i], g[i]);
+        g[i] = __fmul2_rn(g[i], a[i]);                           // 0 where nothing is there
+        m1 = __fadd2_rn(m1, g[i]);
+        m2 = __ffma2_rn(g[i], h[i], m2);
+      }
+      float s[2] = {m1.x + m1.y, m2.x + m2.y};
+      group_sum<MULTI>(s, s_red, turn, warps, group);
+      const float2 k1 = make_float2(-s[0] * inv_c, -s[0] * inv_c), k2 = make_float2(-s[1] * inv_c, -s[1] * inv_c);
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) g[i] = __fmul2_rn(r2, __ffma2_rn(h[i], k2, __fadd2_rn(g[i], k1)));
+      S::store(dx.row(b, rn), g, t, threads, C, m);
+    }
   }
   if (!partial) return;
   float* out = partial + (int64_t) blockIdx.x * 2 * C;
@@ -427,7 +490,7 @@ int launch_fwd(const LlsaTensor* x, const NormParams& par, float eps, const Llsa
   const Rows<T> yr = make_rows<T>(y);
   LLSA_NORM_KERNEL({
     // as many CTAs as the SMs hold at once, an equal share of rows each
-    const int64_t most = 148 * fwd_ctas(TPB, R * (FORM == kSingle ? 1 : 4)), per = ((M + most - 1) / most + groups - 1) / groups * groups, grid = (M + per - 1) / per;
+    const int64_t most = 148 * fwd_ctas(TPB, FORM, R * (FORM == kSingle ? 1 : 4), sizeof(T)), per = ((M + most - 1) / most + groups - 1) / groups * groups, grid = (M + per - 1) / per;
     launch_pdl(layer_norm_fwd_kernel<T, FORM, R, MULTI, TPB>, dim3((unsigned) grid), dim3(TPB), 0, st, xr, par, eps, yr, stats, M, N, (uint32_t) per, C, sp.warps);
   })
   LLSA_LAUNCH_OK("layer_norm_fwd_kernel");
