@@ -480,6 +480,16 @@ Chunks chunks_of(int64_t B, int64_t N, int64_t C) {
   else LLSA_NORM_R(kSingle, 16, true, 1024, __VA_ARGS__)                                                        \
   else LLSA_REQUIRE(false, LLSA_ERR_SHAPE, "layer_norm: no kernel for %d channels", C);
 
+// Rows that follow one another as one sample: where nothing is per sample, A and T are loaded once
+bool flatten(LlsaTensor* t) {
+  const int64_t B = t->shape[0], N = t->shape[1];
+  if (B > 1 && N > 1 && t->stride[0] != N * t->stride[1]) return false;
+  if (N == 1) t->stride[1] = t->stride[0];
+  t->shape[0] = 1;
+  t->shape[1] = B * N;
+  return true;
+}
+
 template <typename T>
 int launch_fwd(const LlsaTensor* x, const NormParams& par, float eps, const LlsaTensor* y, float2* stats, cudaStream_t st) {
   const uint32_t M = (uint32_t) (x->shape[0] * x->shape[1]), N = (uint32_t) x->shape[1];
@@ -537,6 +547,8 @@ extern "C" int llsa_layer_norm_fwd(const LlsaTensor* x, const LlsaTensor* weight
   LLSA_REQUIRE(eps >= 0.f, LLSA_ERR_ARG, "layer_norm: eps %g is negative or not a number", (double) eps);
   if (shape[0] * shape[1] == 0) return LLSA_OK;
   float2* st = stats ? (float2*) stats->ptr : nullptr;
+  LlsaTensor fx = *x, fy = *y;
+  if (!scale && !shift && flatten(&fx) && flatten(&fy)) x = &fx, y = &fy;
   return x->dtype == LLSA_F32 ? launch_fwd<float>(x, par, eps, y, st, (cudaStream_t) stream)
                               : launch_fwd<bf16>(x, par, eps, y, st, (cudaStream_t) stream);
 }
@@ -584,12 +596,8 @@ extern "C" int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, co
   // one sample of all rows: needs rows that follow one another
   LlsaTensor f[3] = {*dy, *x, *dx};
   if (!per_sample && B > 1)
-    for (LlsaTensor& t : f) {
-      LLSA_REQUIRE(N == 1 || t.stride[0] == N * t.stride[1], LLSA_ERR_STRIDE, "layer_norm_bwd: samples must follow one another where nothing is per sample");
-      if (N == 1) t.stride[1] = t.stride[0];
-      t.shape[1] = B * N;
-      t.shape[0] = 1;
-    }
+    for (LlsaTensor& t : f)
+      LLSA_REQUIRE(flatten(&t), LLSA_ERR_STRIDE, "layer_norm_bwd: samples must follow one another where nothing is per sample");
   float* part = sums ? (float*) partial->ptr : nullptr;
   const float2* sv = (const float2*) stats->ptr;
   const cudaStream_t st = (cudaStream_t) stream;

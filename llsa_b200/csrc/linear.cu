@@ -423,9 +423,10 @@ struct Plan {
   size_t o_dz, o_cols, o_parts, o_wg, o_pg, bytes;
 };
 
-// Long samples: twice as many rows as input features, what the B weights and parts cost beside z and dz; rows on 16-byte boundaries throughout
+// Long samples: twice as many rows as input features, what the B weights and parts cost beside z and dz; rows on 16-byte boundaries throughout;
+// samples that a grid's second dimension takes
 bool by_sample(const LlsaLinearArgs* a, const Plan& p) {
-  return p.dtype == LLSA_BF16 && a->gate && p.N >= 512 && p.N >= 2 * p.K && p.K % 8 == 0 && p.F % 8 == 0;
+  return p.dtype == LLSA_BF16 && a->gate && p.N >= 512 && p.N >= 2 * p.K && p.K % 8 == 0 && p.F % 8 == 0 && p.B <= 65535;
 }
 
 int check_common(const LlsaLinearArgs* a, Plan* p) {
@@ -570,7 +571,6 @@ int backward_by_sample(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) 
   }
   if (a->dx) {
     bf16* wg = (bf16*) (ws + p.o_wg);
-    LLSA_REQUIRE(p.B <= 65535, LLSA_ERR_SHAPE, "linear_bwd: too many samples");
     launch_pdl(gated_weight_kernel, dim3((unsigned) ((p.F * (p.K / 8) + 255) / 256), (unsigned) p.B), dim3(256), 0, st, w, gate, wg, (int) p.F, (int) p.K);
     LLSA_LAUNCH_OK("gated_weight_kernel");
     Epilogue<bf16> e = {};

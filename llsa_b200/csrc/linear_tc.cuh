@@ -91,15 +91,16 @@ __device__ __forceinline__ float2 activate2(float2 z) {
   return __fmul2_rn(z, logistic2(t));
 }
 // s + z s (1 - s) u'(z).  Beyond +-7 (SiLU: +-30) the slope is 1 or within 4e-14 (3e-12) of 0, and z stays there: 2^t then stays below 2^52 and both of a pair's
-// reciprocals come from one.  The special functions, 16 a cycle, are what paces the kernel: three for two values instead of four.
+// reciprocals come from one.  The special functions, 16 a cycle, are what paces the kernel: three for two values instead of four.  A NaN stands in for itself
+// alone: it goes in with the last factor, and the shared reciprocal sees a number in its place.
 template <int ACT>
 __device__ __forceinline__ float2 slope2(float2 z) {
   constexpr float kFar = ACT == kActGeluTanh ? 7.f : 30.f;
   z = make_float2(clamp_nan(z.x, kFar), clamp_nan(z.y, kFar));
-  const float2 q = __fmul2_rn(z, z);
+  const float2 c = make_float2(fmaxf(z.x, -kFar), fmaxf(z.y, -kFar)), q = __fmul2_rn(c, c);
   float2 t;
-  if constexpr (ACT == kActGeluTanh) t = __fmul2_rn(z, __ffma2_rn(q, two(-kGelu2 * kGelu3 * kLog2e), two(-kGelu2 * kLog2e)));
-  else t = __fmul2_rn(z, two(-kLog2e));
+  if constexpr (ACT == kActGeluTanh) t = __fmul2_rn(c, __ffma2_rn(q, two(-kGelu2 * kGelu3 * kLog2e), two(-kGelu2 * kLog2e)));
+  else t = __fmul2_rn(c, two(-kLog2e));
   const float2 d = __fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), two(1.f));
   const float r = rcp(d.x * d.y);
   const float2 s = make_float2(r * d.y, r * d.x);
@@ -530,7 +531,6 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
         // the columns of a CTA stay the same (its units are a multiple of tiles_n): one sum over its rows.  Lanes 4 apart have the same columns
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (!ok) sums[i] = two(__uint_as_float(0x7fffffffu));
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             sums[i].x += __shfl_xor_sync(0xffffffffu, sums[i].x, o);
@@ -548,6 +548,7 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
           float u = 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) u += s_sum[(wg * 4 + k) * kChunk + row];
+          if (ctl->abort) u = __uint_as_float(0x7fffffffu);      // tiles are missing, and copies may still land in the ring
           out.partial[((int64_t) ((unit / tiles_n) << PAIR | rank) * 2 + 1) * N + j] = u;
         }
       }

@@ -189,7 +189,7 @@ def _register_fakes() -> None:
         out = [x.new_empty((*x.shape[:-1], F))]
         if want_pre:      # not kept for a gate of long samples (csrc/linear.cu: by_sample)
             N = M // x.shape[0] if gate is not None and x.shape[0] else M
-            kept = not (x.dtype == torch.bfloat16 and gate is not None and N >= 512 and N >= 2 * K and K % 8 == 0 and F % 8 == 0) and M > 0
+            kept = M > 0 and not (x.dtype == torch.bfloat16 and gate is not None and N >= 512 and N >= 2 * K and K % 8 == 0 and F % 8 == 0 and x.shape[0] <= 65535)
             out.append(x.new_empty((M if kept else 0, F)))
         if want_copies and x.dtype == torch.bfloat16 and K % 8:
             out += [x.new_empty_strided((n, K), ((K + 7) // 8 * 8, 1)) for n in (M, F)]

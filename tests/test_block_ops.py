@@ -577,6 +577,208 @@ def test_refusals():
         llsa_b200.layer_norm(fwd.make_dual(x.detach(), torch.ones_like(x)))
 
 
+# ------------------------------------------------------------------------------------------------------ unusual calls
+def test_a_bad_value_stays_where_the_formula_puts_it():
+    """NaN in one row of the weight, in the bias, in one row of x: what does not depend on it is what it is without."""
+    g = gen(71)
+    x, w, b = normal(g, 2, 300, 64, dtype=BF16), normal(g, 72, 64, dtype=BF16, std=0.2), normal(g, 72, dtype=BF16)
+    dy = normal(g, 2, 300, 72, dtype=BF16)
+    for act in ("gelu_tanh", "silu"):
+        def grads(x, w, b):
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+            y = llsa_b200.linear(leaves[0], leaves[1], leaves[2], activation=act)
+            return y.detach(), *torch.autograd.grad(y, leaves, dy)
+        want = grads(x, w, b)
+        for f in (0, 7, 40, 71):
+            others = [i for i in range(72) if i != f]
+            for bad_w in (True, False):
+                w2, b2 = w.clone(), b.clone()
+                if bad_w:
+                    w2[f, 3] = float("nan")
+                else:
+                    b2[f] = float("nan")
+                y, dx, dw, db = grads(x, w2, b2)
+                assert y[..., f].isnan().all() and dw[f].isnan().all() and db[f].isnan() and dx.isnan().all()
+                assert torch.equal(y[..., others], want[0][..., others]) and torch.equal(dw[others], want[2][others]) and torch.equal(db[others], want[3][others])
+        x2 = x.clone()
+        x2[1, 77, 5] = float("nan")
+        y, dx, dw, db = grads(x2, w, b)
+        assert y[1, 77].isnan().all() and dx[1, 77].isnan().all() and dw.isnan().all() and db.isnan().all()
+        y[1, 77], dx[1, 77] = want[0][1, 77], want[1][1, 77]
+        assert torch.equal(y, want[0]) and torch.equal(dx, want[1])
+
+
+def _long_samples(seed, B=3, N=1030, K=96, F=136):
+    g = gen(seed)
+    leaves = [normal(g, B, N, K, dtype=BF16), normal(g, F, K, dtype=BF16, std=K ** -0.5), normal(g, F, dtype=BF16, std=0.1), normal(g, B, N, F, dtype=BF16),
+              normal(g, B, F, dtype=BF16)]
+    return [t.requires_grad_(True) for t in leaves], normal(g, B, N, F, dtype=BF16)
+
+
+def _gated(x, w, b, r, gate):
+    return llsa_b200.linear(x, w, b, residual=r, gate=gate)
+
+
+def test_gate_of_long_samples_in_parts_in_graphs_and_traced():
+    """Any of the gradients alone has the bits that it has among all of them; so it has captured, replayed and traced."""
+    leaves, dy = _long_samples(81)
+    want = torch.autograd.grad(_gated(*leaves), leaves, dy)
+    for mask in range(1, 32):
+        some = [t.detach().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate(leaves)]
+        wanted = [i for i in range(5) if mask >> i & 1]
+        got = torch.autograd.grad(_gated(*some), [some[i] for i in wanted], dy)
+        for i, d in zip(wanted, got):
+            assert torch.equal(d, want[i]), (mask, i)
+    other, dy2 = _long_samples(82)
+    want2 = torch.autograd.grad(_gated(*other), other, dy2)
+    ins, dyc = [t.detach().clone().requires_grad_(True) for t in leaves], dy.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(_gated(*ins), ins, dyc)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = torch.autograd.grad(_gated(*ins), ins, dyc)
+    for src, d, expect in ((leaves, dy, want), (other, dy2, want2), (leaves, dy, want)):
+        with torch.no_grad():
+            for t, v in zip(ins, src):
+                t.copy_(v)
+            dyc.copy_(d)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, expect))
+    y = torch.compile(_gated, backend="aot_eager", fullgraph=True)(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
+# a gate of long samples; of short ones; products, slope, both tiles of one CTA and of a pair
+@pytest.mark.parametrize("M,K,F,act,gate", [(4096, 384, 1536, "gelu_tanh", 0), (4096, 1536, 384, None, 2), (300, 100, 72, "silu", 0), (1200, 256, 512, None, 12),
+                                            (128, 64, 64, None, 0), (16384, 64, 64, "silu", 0)])
+@pytest.mark.parametrize("limit", [1, 2, 8, 32])
+def test_every_value_behind_an_expired_wait_is_nan(M, K, F, act, gate, limit, monkeypatch):
+    """Under a poll limit of a few looks results are final or NaN, the status word says so under set_device_checks, and the next call is right."""
+    from llsa_b200 import ops
+    g = gen(M + K + F)
+    x, w, b = normal(g, gate or 1, M // (gate or 1), K, dtype=BF16), normal(g, F, K, dtype=BF16, std=K ** -0.5), normal(g, F, dtype=BF16)
+    r, gt, dy = normal(g, *x.shape[:2], F, dtype=BF16), normal(g, gate, F, dtype=BF16) if gate else None, normal(g, *x.shape[:2], F, dtype=BF16)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, gt) if t is not None]
+
+    def run():
+        y = llsa_b200.linear(x, w, b, activation=act, residual=r if gate else None, gate=gt)
+        return y.detach(), *torch.autograd.grad(y, leaves, dy)
+
+    want = run()
+    for t in run():                                               # so that what a limited call finds in memory is not the answer
+        t.fill_(3.0)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(ops, "_wait_limit", limit)
+    ops._native()
+    got = run()
+    torch.cuda.synchronize()
+    try:
+        llsa_b200.set_device_checks(True)
+        ops._native()
+        if limit == 1:
+            with pytest.raises(RuntimeError, match="bounded wait"):
+                llsa_b200.linear(x, w, b)
+    finally:
+        monkeypatch.setattr(ops, "_wait_limit", 0)
+        llsa_b200.set_device_checks(False)
+        ops._native()
+    for a, c in zip(got, want):
+        assert bool((a.isnan() | (a == c)).all()), int((~a.isnan() & (a != c)).sum())
+    if limit == 1:
+        assert got[0].isnan().any()
+    assert all(torch.equal(a, c) for a, c in zip(run(), want))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last rows have the bits that a call of them alone has, and no others."""
+    g = gen(91)
+    M, C = 2_200_000, 1024
+    x = torch.empty(M, C, device=DEV, dtype=BF16)
+    tail = normal(g, 1000, C, dtype=BF16)
+    x.zero_()[-1000:] = tail
+    w, b = normal(g, C, dtype=BF16), normal(g, C, dtype=BF16)
+    y = llsa_b200.layer_norm(x, w, b)
+    assert torch.equal(y[-1000:], llsa_b200.layer_norm(tail, w, b)) and torch.equal(y[:5], b.expand(5, C))
+    xg, wg = x.requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(llsa_b200.layer_norm(xg, wg, b), (xg, wg), y)
+    tg = tail.clone().requires_grad_(True)
+    (dt,) = torch.autograd.grad(llsa_b200.layer_norm(tg, w, b), tg, y[-1000:].contiguous())
+    zg = torch.zeros(5, C, device=DEV, dtype=BF16, requires_grad=True)
+    (d0,) = torch.autograd.grad(llsa_b200.layer_norm(zg, w, b), zg, y[:5].contiguous())
+    assert torch.equal(dx[-1000:], dt) and torch.equal(dx[:5], d0) and torch.isfinite(dw).all()
+    del dx, y, xg
+    x = x.detach()
+    rows = x.view(1, M // 1000, 1000, C)
+    pos = torch.arange(1000, device=DEV)[:, None]
+    turned = llsa_b200.rope_axes(rows[..., :512], pos, (512,))
+    assert torch.equal(turned[:, -1:], llsa_b200.rope_axes(rows[:, -1:, :, :512], pos, (512,))) and not turned[:, 0].any()
+    del turned, rows
+    w1, b1 = normal(g, 1024, 64, dtype=BF16), normal(g, 1024, dtype=BF16)
+    small = x[:, :64]                                             # rows 2 KB apart
+    y = llsa_b200.linear(small, w1, b1, activation="silu")
+    near = llsa_b200.linear(tail[:, :64], w1, b1, activation="silu")
+    zero = llsa_b200.linear(torch.zeros(8, 64, device=DEV, dtype=BF16), w1, b1, activation="silu")
+    assert torch.equal(y[-1000:], near) and torch.equal(y[:8], zero)
+    xg, wg = small.requires_grad_(True), w1.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(llsa_b200.linear(xg, wg, b1, activation="silu"), (xg, wg), y)
+    tg = tail[:, :64].clone().requires_grad_(True)
+    wt = w1.clone().requires_grad_(True)
+    dt, dwt = torch.autograd.grad(llsa_b200.linear(tg, wt, b1, activation="silu"), (tg, wt), near)
+    # dx of a row: sums over 1024 features, of the same bf16 terms, in fp32: 1024 roundings of what may stand in any order, and one to bf16
+    mag = (near.double().abs() * 2) @ w1.double().abs()
+    within("dx", dx[-1000:], dt.double(), 2 * 1024 * U * mag, 2.0)
+    # rows of zeros add nothing to dw; what is left are sums over 1000 rows
+    mag = (near.double().abs() * 2).t() @ tail[:, :64].double().abs()
+    within("dw", dw, dwt.double(), 2 * 1000 * U * mag, 2.0)
+
+
+def test_outputs_of_the_c_entries_leave_their_surroundings_alone():
+    """Rows of y, dx and z inside larger matrices: nothing between or behind them is written."""
+    import ctypes as C
+    from llsa_b200 import _lib
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for dtype in (BF16, F32):
+        for M, K, F in ((130, 64, 72), (257, 40, 200), (1, 8, 8), (300, 64, 66)):
+            g = gen(M + F)
+            x, w, dy = normal(g, M, K, dtype=dtype), normal(g, F, K, dtype=dtype), normal(g, M, F, dtype=dtype)
+            want = llsa_b200.linear(x, w)
+            for pad in (8, 16, 3):
+                big = torch.full((M + 4, F + pad), 7.0, device=DEV, dtype=dtype)
+                a = _lib.LlsaLinearArgs()
+                keep = [_lib.desc(t) for t in (x, w, big[2:-2, :F])]
+                a.x, a.weight, a.y = [C.pointer(d) for d in keep]
+                assert lib.llsa_linear_fwd(C.byref(a), stream) == 0, lib.llsa_last_error_string()
+                assert torch.equal(big[2:-2, :F], want), (dtype, M, K, F, pad)
+                big[2:-2, :F] = 7.0
+                assert bool((big == 7.0).all())
+                big = torch.full((M + 4, K + pad), 7.0, device=DEV, dtype=dtype)
+                b = _lib.LlsaLinearArgs()
+                keep = [_lib.desc(t) for t in (x, w, dy, big[2:-2, :K])]
+                b.x, b.weight, b.dy, b.dx = [C.pointer(d) for d in keep]
+                ws = torch.empty(max(1, lib.llsa_linear_bwd_workspace_bytes(C.byref(b))) + 256, device=DEV, dtype=torch.uint8)
+                b.workspace, b.workspace_bytes = (ws.data_ptr() + 255) // 256 * 256, ws.numel() - 256
+                assert lib.llsa_linear_bwd(C.byref(b), stream) == 0, lib.llsa_last_error_string()
+                xg = x.clone().requires_grad_(True)
+                (dx,) = torch.autograd.grad(llsa_b200.linear(xg, w), xg, dy)
+                assert torch.equal(big[2:-2, :K], dx), (dtype, M, K, F, pad)
+                big[2:-2, :K] = 7.0
+                assert bool((big == 7.0).all())
+        for B, N, Ch in ((2, 9, 64), (3, 5, 130), (1, 4, 384)):
+            x = normal(gen(Ch), B, N, Ch, dtype=dtype)
+            for pad in (4, 8, 3):
+                big = torch.full((B + 2, N + 2, Ch + pad), 7.0, device=DEV, dtype=dtype)
+                out = big[1:-1, 1:-1, :Ch]
+                keep = [_lib.desc(x), _lib.desc(out)]
+                assert lib.llsa_layer_norm_fwd(C.byref(keep[0]), None, None, None, None, 1e-5, C.byref(keep[1]), None, stream) == 0, lib.llsa_last_error_string()
+                want = norm_reference(x, None, None, None, None, 1e-5)["y"]
+                within("y", out, want[0], (Ch + 16) * U * want[1])
+                out.fill_(7.0)
+                assert bool((big == 7.0).all())
+
+
 # ------------------------------------------------------------------------------------------------------ the model
 @pytest.mark.parametrize("attn,fused_rope,side", [("sparse_l2", True, 128), ("sparse_l1", False, 32), ("pixel", True, 16)])
 def test_model_on_the_fused_block_agrees_with_the_eager_block(attn, fused_rope, side):
