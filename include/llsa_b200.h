@@ -168,7 +168,7 @@ typedef struct LlsaLinearArgs {
   /* backward: dy in, those of the others that are not NULL out */
   const LlsaTensor* dy;        /* [M,F], any row stride; for a gate of long bf16 samples (llsa_linear_keeps_product() is 0) rows on 16-byte boundaries */
   const LlsaTensor* dx;        /* [M,K], likewise */
-  const LlsaTensor* dweight;   /* [F,K] contiguous, x's type */
+  const LlsaTensor* dweight;   /* [F,K] contiguous, x's type; for such a gate on a 16-byte boundary */
   const LlsaTensor* dbias;     /* [F] contiguous, F32 or x's type */
   const LlsaTensor* dgate;     /* [B,F] contiguous, F32 or x's type */
   void* workspace;             /* backward: llsa_linear_bwd_workspace_bytes() bytes on a 256-byte boundary, not read before they are written */

@@ -117,14 +117,16 @@ __device__ __forceinline__ void load_param(float (&v)[S::E], const ParamView& p,
     for (int e = 0; e < S::E; ++e) v[e] = absent;
   }
 }
-// Four channels of one
+// Four channels of one, of which those of a shifted vector are there or not one by one
+template <int FORM>
 __device__ __forceinline__ void load_param4(float (&v)[4], const ParamView& p, uint32_t b, float absent, int c, int C) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = absent;
   if (!p.p || c >= C) return;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    v[j] = p.is_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(p.p)[b * p.ld + c + j]) : reinterpret_cast<const float*>(p.p)[b * p.ld + c + j];
+    if (FORM == kWhole || (unsigned) (c + j) < (unsigned) C)
+      v[j] = p.is_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(p.p)[b * p.ld + c + j]) : reinterpret_cast<const float*>(p.p)[b * p.ld + c + j];
 }
 template <typename T>
 __device__ __forceinline__ int shift_of(const T* row) { return (int) ((uintptr_t) row / sizeof(T) & 3); }
@@ -152,23 +154,25 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], 
   }
 }
 
-// CTAs that an SM should hold, by threads, by values of a thread and their type: registers are what decides (fp32, 12 values: four CTAs 75 us, three 71.5)
+// CTAs that an SM should hold, by threads, by values of a thread and their type: registers are what decides (fp32, 12 values: four CTAs 75 us, three 71.5;
+// shifted, 16 values: bf16 three 87.5 us, two 100, fp32 49.5 and 45.6)
 constexpr int fwd_ctas(int tpb, int form, int e, int bytes) {
-  return tpb > 256 ? 1 : form == kWhole ? (bytes == 2 || e <= 8 ? 4 : 3) : e <= 12 ? 4 : 3;
+  return tpb > 256 ? 1 : form == kWhole ? (bytes == 2 || e <= 8 ? 4 : 3) : form == kShifted ? (e <= 8 ? 4 : bytes == 2 ? 3 : 2) : e <= 12 ? 4 : 3;
 }
 constexpr int bwd_ctas(int tpb) { return tpb > 256 ? 1 : 2; }
 
 // TPB: threads of a CTA; MULTI: more than one warp to a row.  A CTA takes rows [blockIdx.x * per, + per): neighbours, so that a group's sample, and with it A and
 // T, changes rarely.  (Rows a grid apart had them loaded for nearly every row: 8 x 16384 rows of 384 channels 77 us, 44 so.)
 // Measured (bf16 unless said): 8 x 16384 rows of 384 channels 39.6 us (5.1 TB/s), in fp32 71.5 (5.6); 8 x 16384 of 768 92.7; 2 x 8192 of 2048 35.6; with A and T
-// in registers, which spill, 43.6, 81.7, 105 and 40.6.  Two rows on their way are worth 1 us of the first and cost 12 of the 768 channels' 93.
+// in registers, which spill, 43.6, 81.7, 105 and 40.6.  Shifted, 8 x 16384 rows of 390: 87.5 (104 in registers); 4 x 4096 of 770: 28.2 (53).  Two rows on their way are worth 1 us of the first and cost 12 of the 768 channels' 93.
 template <typename T, int FORM, int R, bool MULTI, int TPB>
 __global__ void __launch_bounds__(TPB, fwd_ctas(TPB, FORM, R * (FORM == kSingle ? 1 : 4), sizeof(T)))
 layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, float2* __restrict__ stats, uint32_t M, uint32_t N, uint32_t per, int C, int warps) {
   using S = Slice<T, FORM, R>;
   constexpr int E = S::E;
-  // whole vectors: A and T lie in shared memory, each thread's own, and leave their registers to the rows; rows of one warp have two on their way
-  constexpr bool KEEP = FORM == kWhole;
+  // vectors: A and T lie in shared memory, each thread's own, and leave their registers to the rows (512 threads have the registers, and would need more than
+  // 48 KB); rows of one warp have two on their way
+  constexpr bool KEEP = FORM == kWhole || (FORM == kShifted && TPB == 256);
   constexpr int DEPTH = FORM == kWhole && R <= 3 && !MULTI && sizeof(T) == 2 ? 2 : 1;
   __shared__ float s_red[2][32][2];
   __shared__ float4 s_par[KEEP ? 2 * R * TPB : 1];
@@ -210,12 +214,12 @@ layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, flo
         if constexpr (KEEP) {
 #pragma unroll 1
           for (int i = 0; i < R; ++i) {
-            const int c = (i * threads + t) * 4;
+            const int c = S::channel(4 * i, t, threads, m);
             float u[4], w[4], bias[4], shift[4];
-            load_param4(u, par.scale, rb, 0.f, c, C);
-            load_param4(w, par.w, 0, 1.f, c, C);
-            load_param4(bias, par.bias, 0, 0.f, c, C);
-            load_param4(shift, par.shift, rb, 0.f, c, C);
+            load_param4<FORM>(u, par.scale, rb, 0.f, c, C);
+            load_param4<FORM>(w, par.w, 0, 1.f, c, C);
+            load_param4<FORM>(bias, par.bias, 0, 0.f, c, C);
+            load_param4<FORM>(shift, par.shift, rb, 0.f, c, C);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               w[j] *= 1.f + u[j];

@@ -329,71 +329,116 @@ gated_weight_kernel(Mat<const bf16> w, Mat<const bf16> gate, bf16* __restrict__ 
   *reinterpret_cast<uint4*>(out + (b * F + f) * K + k) = Vec<bf16, 8>::pack(v);
 }
 
-// As sum_parts_kernel, `per_sample` parts of each of B samples weighed with its gate; and rowsum(w G_b) of the CTA's 32 columns in pg[B][columns / 32][0][F].
-// out, pg: NULL where not wanted.
+// dw = sum_b gate_b (sum of sample b's parts), and of each CTA's share of the input features rowsum(w G_b) in pg[B][share][0][F].  out, pg: NULL where not wanted.
+// A CTA takes 16 rows of 128 columns of the parts ([F][K], or TURNED [K][F]), 512 bytes of a row to a warp; its threads hold 2 x 4 values, and two samples' parts
+// are on their way at once, in order.  (57 MB of parts, 1536 x 384 in 24: 31 us in tiles of 32 x 32, 62 and more with more of those 128-byte pieces on their
+// way; so AFTER_US.)  F and K are multiples of 8.
+constexpr int kPartRows = 16, kPartCols = 128;
 template <bool TURNED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 gated_parts_kernel(const float* __restrict__ partial, int64_t ld, int per_sample, int B, int64_t F, int64_t K, Mat<const bf16> gate, Mat<const bf16> w,
                    bf16* __restrict__ out, float* __restrict__ pg) {
-  __shared__ float s_tile[32][33];
+  constexpr int kAtOnce = 2, kAhead = 4;
+  __shared__ float4 s_sum[kAtOnce][8][kPartCols / 4];
+  __shared__ float s_out[TURNED ? kPartCols : 1][kPartRows + 1];
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-  const int64_t f0 = blockIdx.y * (int64_t) 32, k0 = blockIdx.x * (int64_t) 32, part = (TURNED ? K : F) * ld;
+  const int64_t rows = TURNED ? K : F, cols = TURNED ? F : K, part = rows * ld, r0 = blockIdx.x * (int64_t) kPartRows, c0 = blockIdx.y * (int64_t) kPartCols,
+                c = c0 + 4 * x, share = TURNED ? blockIdx.x : blockIdx.y, shares = TURNED ? gridDim.x : gridDim.y;
+  const bool there[2] = {r0 + y < rows && c < cols, r0 + y + 8 < rows && c < cols};
   pdl_wait();
   pdl_trigger();
-  int64_t f[4], k[4];
-  bool there[4];
-  float wv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+  float wv[2][4], acc[2][4] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = f0 + (TURNED ? x : y + 8 * i);
-    k[i] = k0 + (TURNED ? y + 8 * i : x);
-    there[i] = f[i] < F && k[i] < K;
-    wv[i] = pg && there[i] ? __bfloat162float(w.p[f[i] * w.ld + k[i]]) : 0.f;
-  }
-  for (int b = 0; b < B; ++b) {
-    float u[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < per_sample; ++s)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (there[i]) u[i] += partial[((int64_t) b * per_sample + s) * part + (TURNED ? k[i] * ld + f[i] : f[i] * ld + k[i])];
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = r0 + y + 8 * i;
+      wv[i][j] = pg && there[i] ? __bfloat162float(TURNED ? w.p[(c + j) * w.ld + r] : w.p[r * w.ld + c + j]) : 0.f;
+    }
+  for (int b0 = 0; b0 < B; b0 += kAtOnce) {
+    float u[kAtOnce][2][4] = {}, g[kAtOnce][TURNED ? 4 : 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (there[i]) acc[i] = fmaf(__bfloat162float(gate.p[b * gate.ld + f[i]]), u[i], acc[i]);
-    if (pg) {
-      float* to = pg + ((int64_t) b * gridDim.x + blockIdx.x) * 2 * F;
-      if constexpr (TURNED) {
-        s_tile[y][x] = (wv[0] * u[0] + wv[1] * u[1]) + (wv[2] * u[2] + wv[3] * u[3]);
-        __syncthreads();
-        if (y == 0 && f[0] < F) {
+    for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+      for (int j = 0; j < (TURNED ? 4 : 2); ++j)
+        g[q][j] = b0 + q < B && there[TURNED ? 0 : j] ? __bfloat162float(gate.p[(b0 + q) * gate.ld + (TURNED ? c + j : r0 + y + 8 * j)]) : 0.f;
+    for (int s = 0; s < per_sample; s += kAhead) {
+      float4 v[kAtOnce][kAhead][2];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const float* p = partial + ((int64_t) (b0 + q) * per_sample + s + j) * part + (r0 + y) * ld + c;
+          const bool some = b0 + q < B && s + j < per_sample;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) v[q][j][i] = some && there[i] ? *reinterpret_cast<const float4*>(p + 8 * i * ld) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            u[q][i][0] += v[q][j][i].x;
+            u[q][i][1] += v[q][j][i].y;
+            u[q][i][2] += v[q][j][i].z;
+            u[q][i][3] += v[q][j][i].w;
+          }
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (b0 + q < B && there[i]) acc[i][j] = fmaf(g[q][TURNED ? j : i], u[q][i][j], acc[i][j]);
+    if (!pg) continue;
+    if constexpr (TURNED) {
+      if (b0) __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = fmaf(wv[1][j], u[q][1][j], wv[0][j] * u[q][0][j]);
+        s_sum[q][y][x] = make_float4(t[0], t[1], t[2], t[3]);
+      }
+      __syncthreads();
+      const int q = threadIdx.x / kPartCols, col = threadIdx.x % kPartCols;
+      if (b0 + q < B && c0 + col < F) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += reinterpret_cast<const float*>(&s_sum[q][k][0])[col];
+        pg[((int64_t) (b0 + q) * shares + share) * 2 * F + c0 + col] = t;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           float t = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) t += s_tile[j][x];
-          to[f[0]] = t;
-        }
-        __syncthreads();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float t = wv[i] * u[i];
+          for (int j = 0; j < 4; ++j) t = fmaf(wv[i][j], u[q][i][j], t);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-          if (x == 0 && f[i] < F) to[f[i]] = t;
+          const int64_t f = r0 + y + 8 * i;
+          if (x == 0 && b0 + q < B && f < F) pg[((int64_t) (b0 + q) * shares + share) * 2 * F + f] = t;
         }
-      }
     }
   }
   if (!out) return;
   if constexpr (TURNED) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s_tile[y + 8 * i][x] = acc[i];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_out[4 * x + j][y + 8 * i] = acc[i][j];
     __syncthreads();
+    const int64_t f = c0 + threadIdx.x / 2, k = r0 + threadIdx.x % 2 * 8;
+    if (f < F && k < K) *reinterpret_cast<uint4*>(out + f * K + k) = Vec<bf16, 8>::pack(&s_out[threadIdx.x / 2][threadIdx.x % 2 * 8]);
+  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = s_tile[x][y + 8 * i];
+    for (int i = 0; i < 2; ++i)
+      if (there[i]) *reinterpret_cast<uint2*>(out + (r0 + y + 8 * i) * K + c) = Vec<bf16, 4>::pack(acc[i]);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (f0 + y + 8 * i < F && k0 + x < K) out[(f0 + y + 8 * i) * K + k0 + x] = __float2bfloat16_rn(acc[i]);
 }
 
 // ------------------------------------------------------------------------------------------------ checks and plan
@@ -505,7 +550,7 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   p->o_cols = take(p->sums ? (size_t) (p->B * p->chunks * 2 * p->F * 4) : 0);
   const bool parts = a->dweight || (p->by_sample && a->dgate);
   p->o_parts = take(parts ? (size_t) ((p->by_sample ? p->B : 1) * p->split * (p->turned ? p->K : p->F) * p->part_ld * 4) : 0);
-  p->k_tiles = (p->K + 31) / 32;
+  p->k_tiles = p->turned ? (p->K + kPartRows - 1) / kPartRows : (p->K + kPartCols - 1) / kPartCols;
   p->o_wg = take(p->by_sample && a->dx ? (size_t) (p->B * p->F * p->K * es) : 0);
   p->o_pg = take(p->by_sample && a->dgate ? (size_t) (p->B * p->k_tiles * 2 * p->F * 4) : 0);
   p->bytes = at;
@@ -579,28 +624,25 @@ int backward_by_sample(const LlsaLinearArgs* a, const Plan& p, cudaStream_t st) 
     d.samples = p.B;
     if ((rc = product(d, e, a, st))) return rc;
   }
+  float* pg = a->dgate ? (float*) (ws + p.o_pg) : nullptr;
   if (a->dweight || a->dgate) {
     float* parts = (float*) (ws + p.o_parts);
-    float* pg = a->dgate ? (float*) (ws + p.o_pg) : nullptr;
     Product<bf16> d = p.turned ? Product<bf16>{x, dy, 0, 0, p.K, p.F, p.N, p.split} : Product<bf16>{dy, x, 0, 0, p.F, p.K, p.N, p.split};
     d.samples = p.B;
     if ((rc = product_parts(d, parts, p.part_ld, a, st))) return rc;
-    const dim3 grid((unsigned) p.k_tiles, (unsigned) ((p.F + 31) / 32));
+    const int64_t height = p.turned ? p.K : p.F, width = p.turned ? p.F : p.K;
+    const dim3 grid((unsigned) ((height + kPartRows - 1) / kPartRows), (unsigned) ((width + kPartCols - 1) / kPartCols));
     bf16* dw = a->dweight ? (bf16*) a->dweight->ptr : nullptr;
     launch_pdl(p.turned ? gated_parts_kernel<true> : gated_parts_kernel<false>, grid, dim3(256), 0, st, (const float*) parts, p.part_ld, p.split, (int) p.B, p.F, p.K,
                gate, w, dw, pg);
     LLSA_LAUNCH_OK("gated_parts_kernel");
-    if (pg) {
-      const ParamView none = {nullptr, 0, 0};
-      ParamView bias;
-      if ((rc = make_param(&bias, a->bias, "bias", p.dtype, 0, p.F))) return rc;
-      rc = finish_column_grads({pg, p.k_tiles}, {cols, p.chunks}, p.B, p.F, none, bias, none, 1.f, {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(nullptr)}, st);
-      if (rc) return rc;
-    }
   }
-  if (!a->dbias) return LLSA_OK;
+  if (!a->dgate && !a->dbias) return LLSA_OK;
   const ParamView none = {nullptr, 0, 0}, factor = {a->gate->ptr, gate.ld, 1};
-  return finish_column_grads({nullptr, 0}, {cols, p.chunks}, p.B, p.F, none, none, factor, 0.f, {make_grad(nullptr), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
+  ParamView bias;
+  if ((rc = make_param(&bias, a->bias, "bias", p.dtype, 0, p.F))) return rc;
+  return finish_column_grads({pg, p.k_tiles}, {cols, p.chunks}, p.B, p.F, none, bias, factor, 0.f,
+                             {make_grad(a->dgate), make_grad(nullptr), make_grad(nullptr), make_grad(a->dbias)}, st);
 }
 
 template <typename T>
@@ -691,6 +733,7 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
   if ((rc = check_matrix(a->dy, "dy", p.dtype, p.M, p.F))) return rc;
   LLSA_REQUIRE(!p.by_sample || rows16(a->dy), LLSA_ERR_STRIDE, "dy: rows must start on 16-byte boundaries for a gate of long samples");
   LLSA_REQUIRE(!p.by_sample || !a->dx || rows16(a->dx), LLSA_ERR_STRIDE, "dx: rows must start on 16-byte boundaries for a gate of long samples");
+  LLSA_REQUIRE(!p.by_sample || !a->dweight || (uintptr_t) a->dweight->ptr % 16 == 0, LLSA_ERR_STRIDE, "dweight: must start on a 16-byte boundary for a gate of long samples");
   LLSA_REQUIRE(a->pre || !((a->dgate && !p.by_sample) || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
   if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;
   const int64_t ws[2] = {p.F, p.K}, gs[2] = {p.B, p.F}, bs[1] = {p.F};
