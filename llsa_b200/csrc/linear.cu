@@ -17,17 +17,19 @@ namespace {
 using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------ scalar products
-// fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of 256 threads owns a tile of
-// 16 TM x 16 TM outputs, a thread TM x TM of them.  Steps of 16 along k: the next step's operands are on their way in registers while this one's are
-// multiplied from shared memory, where either stands as 16 rows of neighbours in i or j (turned on the way in if memory has it along k), so that a thread's
-// fours are one load.  TM^2 multiply-adds a k against TM / 2 such loads: the FMA pipe is what bounds it, with two CTAs to an SM.
-template <int TM, bool ALONG_K>
+// fp32 data: one multiply-add per product, as fp32 asks; the tensor cores round their operands to fewer bits.  A CTA of TH x TH threads owns a tile of
+// TH TM x TH TM outputs (TH = 16, or 8 for CTAs of two warps), a thread TM x TM of them.  Steps of 16 along k: the next step's operands are on their way in
+// registers while this one's are multiplied from shared memory, where either stands as 16 rows of neighbours in i or j (turned on the way in if memory has it
+// along k), so that a thread's fours are one load.  TM^2 multiply-adds a k against TM / 2 such loads: the FMA pipe is what bounds it, with two CTAs to an SM.
+// 16384 x 384 -> 1536: 437 us forward, 469 dx, 407 dw (44, 41 and 47 TFLOP/s; cuBLAS 500 forward, 406 dw).  2048 x 384 -> 384: 31 us, 192 tiles of 64 x 64 on
+// 148 SMs, of which 44 have two, and there shared memory is the pace (cuBLAS 27); operands four steps ahead instead of one change nothing.
+template <int TM, int TH, bool ALONG_K>
 struct Operand {
-  static constexpr int kRows = 16 * TM, kK = 16, kLd = kRows + 4, kFloats = kK * kLd;
-  static constexpr int kVecs = kRows * kK / 4, kMine = (kVecs + 255) / 256;
+  static constexpr int kRows = TH * TM, kK = 16, kLd = kRows + 4, kFloats = kK * kLd, kThreads = TH * TH;
+  static constexpr int kVecs = kRows * kK / 4, kMine = (kVecs + kThreads - 1) / kThreads;
   float4 x[kMine];
   // The place of the thread's u-th row (t: its number along the tile)
-  static __device__ __forceinline__ int row(int t, int u) { return TM >= 4 ? (u / 4) * 64 + 4 * t + u % 4 : 2 * t + u; }
+  static __device__ __forceinline__ int row(int t, int u) { return TM >= 4 ? (u / 4) * 4 * TH + 4 * t + u % 4 : 2 * t + u; }
   static __device__ __forceinline__ void place(int v, int& r, int& k) {
     r = ALONG_K ? v / 4 : v % (kRows / 4) * 4;
     k = ALONG_K ? v % 4 * 4 : v / (kRows / 4);
@@ -37,12 +39,12 @@ struct Operand {
   __device__ __forceinline__ void begin(const Mat<const float>& m, int64_t row0, int64_t rows, int64_t k0) {
 #pragma unroll
     for (int q = 0; q < kMine; ++q) {
-      const int v = q * 256 + threadIdx.x;
+      const int v = q * kThreads + threadIdx.x;
       int r, k;
       place(v, r, k);
       const int64_t i = row0 + r, left = max((int64_t) 0, min((int64_t) 4, rows - i));
       src[q] = ALONG_K ? m.p + i * m.ld + k0 + k : m.p + (k0 + k) * m.ld + i;
-      have[q] = kVecs < 256 && v >= kVecs ? 0 : ALONG_K ? (left ? 4 : 0) : (int) left;
+      have[q] = kVecs % kThreads && v >= kVecs ? 0 : ALONG_K ? (left ? 4 : 0) : (int) left;
     }
   }
   // `left` k's are left
@@ -50,7 +52,7 @@ struct Operand {
 #pragma unroll
     for (int q = 0; q < kMine; ++q) {
       int r, k;
-      place(q * 256 + threadIdx.x, r, k);
+      place(q * kThreads + threadIdx.x, r, k);
       const int n = ALONG_K ? min(have[q], left - k) : k < left ? have[q] : 0;
       x[q] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (vec && n >= 4) {
@@ -67,8 +69,8 @@ struct Operand {
   __device__ __forceinline__ void put(float* buf) const {
 #pragma unroll
     for (int q = 0; q < kMine; ++q) {
-      const int v = q * 256 + threadIdx.x;
-      if (kVecs < 256 && v >= kVecs) break;
+      const int v = q * kThreads + threadIdx.x;
+      if (kVecs % kThreads && v >= kVecs) break;
       int r, k;
       place(v, r, k);
       if constexpr (ALONG_K) {
@@ -86,7 +88,7 @@ struct Operand {
     if constexpr (TM >= 4) {
 #pragma unroll
       for (int i = 0; i < TM; i += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(buf + k * kLd + (i / 4) * 64 + 4 * t);
+        const float4 f = *reinterpret_cast<const float4*>(buf + k * kLd + i * TH + 4 * t);
         u[i] = f.x; u[i + 1] = f.y; u[i + 2] = f.z; u[i + 3] = f.w;
       }
     } else {
@@ -96,14 +98,14 @@ struct Operand {
   }
 };
 
-template <int TM, bool A_K, bool B_K, bool PARTIAL>
-__global__ void __launch_bounds__(256, 2)
+template <int TM, int TH, bool A_K, bool B_K, bool PARTIAL>
+__global__ void __launch_bounds__(TH * TH, TH == 16 ? 2 : 4)
 product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split, int vec_a, int vec_b) {
-  using A = Operand<TM, A_K>;
-  using B = Operand<TM, B_K>;
-  constexpr int BM = 16 * TM, BK = 16;
+  using A = Operand<TM, TH, A_K>;
+  using B = Operand<TM, TH, B_K>;
+  constexpr int BM = TH * TM, BK = 16;
   __shared__ __align__(16) float s_a[2][A::kFloats], s_b[2][B::kFloats];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int tx = threadIdx.x % TH, ty = threadIdx.x / TH;
   const int64_t i0 = blockIdx.x / tiles_n * BM, j0 = blockIdx.x % tiles_n * BM;
   const int64_t k_first = blockIdx.y * per_split, k_end = PARTIAL ? min(p.K, k_first + per_split) : p.K;
   float2 acc[TM][TM / 2];                                    // two neighbours an instruction, the same multiply-adds
@@ -170,14 +172,21 @@ int launch_product(const Product<float>& p, const Epilogue<float>& e, float* par
   auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
   const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
   auto vec = [](const Mat<const float>& m) { return (uintptr_t) m.p % 16 == 0 && m.ld % 4 == 0; };
-  auto go = [&](auto kernel, int64_t b) {
-    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(256), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per, (int) vec(p.a), (int) vec(p.b));
+  auto go = [&](auto kernel, int64_t b, unsigned threads) {
+    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(threads), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per, (int) vec(p.a), (int) vec(p.b));
   };
   LLSA_REQUIRE(tiles(32) <= INT32_MAX, LLSA_ERR_SHAPE, "linear: too many outputs");
-  // the largest tile that still gives every SM one
-  if (tiles(128) * split >= 148) go(product_kernel<8, A_K, B_K, PARTIAL>, 128);
-  else if (tiles(64) * split >= 148) go(product_kernel<4, A_K, B_K, PARTIAL>, 64);
-  else go(product_kernel<2, A_K, B_K, PARTIAL>, 32);
+  // the largest tile that still gives every SM one; parts in tiles of 64 x 64 that two warps hold, which fill four to an SM evenly (dw of 16384 x 384 -> 1536
+  // 407 us, in tiles of 128 x 128 446; of 2048 x 384 -> 384 24.4 and 28.9.  Forward 469 and 437: their operands are turned on the way in)
+  const bool large = tiles(128) >= 148, middle = tiles(64) * split >= 148;
+  if constexpr (PARTIAL) {
+    if (middle) go(product_kernel<8, 8, A_K, B_K, true>, 64, 64);
+  } else if (large) {
+    go(product_kernel<8, 16, A_K, B_K, false>, 128, 256);
+  } else if (middle) {
+    go(product_kernel<4, 16, A_K, B_K, false>, 64, 256);
+  }
+  if (!middle && (PARTIAL || !large)) go(product_kernel<2, 16, A_K, B_K, PARTIAL>, 32, 256);
   LLSA_LAUNCH_OK("product_kernel");
   return LLSA_OK;
 }
@@ -312,7 +321,7 @@ int sum_parts(const float* partial, int64_t ld, int split, bool turned, int64_t 
 // Of long samples the gate is applied to what is small instead of to dy.  With G_b = dy_b^T x_b (the parts of dw, taken sample by sample) and S_b = sum_n dy:
 //   dx_b = dy_b (gate_b w),   dw = sum_b gate_b G_b,   dgate_b = rowsum(w G_b) + bias S_b,   dbias = sum_b gate_b S_b
 // so that the product of the forward is not kept, dz is neither written nor rounded, and what passes through memory for it is B weights and parts.
-// us, 131072 rows in 8 samples, 1536 -> 384, forward and backward: 562 with z kept and dz written.
+// us, 131072 rows in 8 samples, 1536 -> 384, forward and backward: 490 with z kept and dz written, 465 so.
 __global__ void __launch_bounds__(256)
 gated_weight_kernel(Mat<const bf16> w, Mat<const bf16> gate, bf16* __restrict__ out, int F, int K) {      // out [B][F][K]; K a multiple of 8
   const int64_t i = blockIdx.x * (int64_t) blockDim.x + threadIdx.x, b = blockIdx.y;
@@ -332,7 +341,7 @@ gated_weight_kernel(Mat<const bf16> w, Mat<const bf16> gate, bf16* __restrict__ 
 // dw = sum_b gate_b (sum of sample b's parts), and of each CTA's share of the input features rowsum(w G_b) in pg[B][share][0][F].  out, pg: NULL where not wanted.
 // A CTA takes 16 rows of 128 columns of the parts ([F][K], or TURNED [K][F]), 512 bytes of a row to a warp; its threads hold 2 x 4 values, and two samples' parts
 // are on their way at once, in order.  (57 MB of parts, 1536 x 384 in 24: 31 us in tiles of 32 x 32, 62 and more with more of those 128-byte pieces on their
-// way; so AFTER_US.)  F and K are multiples of 8.
+// way; so 18.)  F and K are multiples of 8.
 constexpr int kPartRows = 16, kPartCols = 128;
 template <bool TURNED>
 __global__ void __launch_bounds__(256, 2)
@@ -536,9 +545,9 @@ void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
     p->per = std::max<int64_t>(1, (p->N + p->chunks - 1) / p->chunks);
     p->chunks = std::max<int64_t>(1, (p->N + p->per - 1) / p->per);
   }
-  const int64_t tiles = (p->F + 127) / 128 * ((p->K + 127) / 128);
+  const int64_t tiles = (p->F + 63) / 64 * ((p->K + 63) / 64);
   p->turned = false;
-  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->by_sample ? p->N : p->M, p->by_sample ? p->B : 0, &p->turned) : (int) std::max<int64_t>(1, std::min(148 * 2 / tiles, (p->M + 127) / 128));      // one wave of two CTAs to an SM
+  p->split = p->dtype == LLSA_BF16 ? linear_tc_split(p->F, p->K, p->by_sample ? p->N : p->M, p->by_sample ? p->B : 0, &p->turned) : (int) std::max<int64_t>(1, std::min(148 * 4 / tiles, (p->M + 127) / 128));      // one wave of four CTAs to an SM
   p->part_ld = ((p->turned ? p->F : p->K) + 7) / 8 * 8;
   size_t at = 0;
   auto take = [&](size_t bytes) {

@@ -1,8 +1,8 @@
 // The projection's matrix products on tcgen05 (bf16): D[i, j] = sum_k A(i, k) B(j, k), fp32 sums in tensor memory, and what stands behind them.
 //
 //   forward   A = x, B = w, both along k in memory:  y = residual + gate act(D + bias)
-//   slope     the same product again:                dz = dy act'(D + bias), and its column sums.  z is not kept between the passes: writing it and
-//             reading it back costs 4 bytes a value, computing it again K / 750 ns a value and SM; it is never rounded
+//   slope     the same product again:                dz = dy act'(D + bias), and its column sums.  z is not kept between the passes: that would cost 4 bytes a
+//             value of memory traffic and 2 of storage (123 us and 400 MB at 131072 x 1536), and z would be rounded
 //   forward   A = dz, B = w taken across:            dx
 //   parts     A = dz, B = x, both taken across:      dw, in parts of the sum over the tokens, which a second kernel adds in order
 //
@@ -10,12 +10,16 @@
 // matrix with 128-byte swizzled rows of 64 (tc05.cuh).  Ragged edges are zeros that TMA fills in.
 // A persistent CTA per SM walks tiles of 128 x BN, or a pair of them (a cluster of two) tiles of 256 x BN, columns fastest (neighbours in time share rows of A in
 // L2).  The SM takes 64 bytes a cycle from L2, which is the pace of a 128 x 128 tile twice over; a pair keeps half of B in either CTA and multiplies both
-// halves, 256 x 256 at the pace of the tensor cores.  Warp 8 keeps a ring of k-steps of 64 filled; warp 9 (of a pair, rank 0's) issues the products
-// into one of two accumulators in tensor memory; warps 0-7 empty the other one, so that a tile's epilogue runs under the
-// next tile's products.  The epilogue goes in chunks of 64 columns, alternate chunks to either warpgroup, thread = row: a chunk is finished in
-// a 128 x 64 buffer of shared memory (two per warpgroup), which a warp of movers (10, 11) has filled with the residual or dy by TMA beforehand and stores
-// by TMA afterwards.  Written straight from the registers, 32 bytes of each of 32 rows an instruction, the stores were the kernel's pace: 590 us
-// for 131072 x 384 -> 1536 with GELU.  Matrices whose rows TMA cannot take go through the same buffers with loads and stores of the warp.
+// halves, 256 x 256 at the pace of the tensor cores.  One warp keeps a ring of k-steps of 64 filled; another (of a pair, rank 0's) issues the products
+// into one of two accumulators in tensor memory; two or three warpgroups empty the other one, so that a tile's epilogue runs under the
+// next tile's products.  The epilogue goes in chunks of 64 columns, dealt out to the warpgroups in turn: a chunk is finished in a 128 x 64 buffer of
+// shared memory (two per warpgroup), which the warpgroup's mover warp has filled with the residual or dy by TMA beforehand and stores by TMA
+// afterwards.  Matrices whose rows TMA cannot take go through the same buffers with loads and stores of the warp.
+//
+// us, 131072 rows, 384 -> 1536 | 1536 -> 384 (cuBLAS: 145 | 142 to 149 forward, 145 | 175 dw): plain 133 | 133, with GELU 167, gated onto a residual 171 | 157,
+// dx 146 | 144, dw 126 | 133, slope with its column sums 241: 1.0 to 1.2 PFLOP/s where there is little epilogue.  An activation's epilogue is paced by the 16
+// special functions a cycle (89 us of GELU's 167; its instructions do not all hide under the products).  With the results stored straight from registers, 32
+// bytes of each of 32 rows an instruction, GELU took 590; with tiles of one CTA instead of pairs 271 (plain 217).
 // Every mbarrier wait is bounded; tiles behind one that ran out are written as NaN (and the status word says so).
 #include "linear_tc.cuh"
 

@@ -14,7 +14,7 @@ using bf16 = __nv_bfloat16;
 constexpr int kBM = 128, kBK = 64;
 // Roles: G warpgroups of epilogue, the producer, the warp that issues the products, a mover to each warpgroup.  Three warpgroups hide the latencies of a long
 // epilogue; two leave 32 KB more to the ring, which a long sum needs.  us, two / three, 131072 rows, tiles of 256 x 256: 384 -> 1536 with GELU 177 / 164, gated
-// onto a residual 203 / 177, plain 136 / 149; 1536 -> 384 plain 150 / 159, gated 157 / 177.
+// onto a residual 203 / 177, plain 136 / 149; 1536 -> 384 plain 150 / 159, gated 157 / 177.  Four leave a ring of three steps: GELU 183 where three take 167.
 template <int G>
 struct Roles {
   static constexpr int kEpilogueWarps = 4 * G, kProducer = kEpilogueWarps, kIssuer = kProducer + 1, kMover = kIssuer + 1, kThreads = 32 * (kMover + G);

@@ -692,6 +692,36 @@ def test_every_value_behind_an_expired_wait_is_nan(M, K, F, act, gate, limit, mo
     assert all(torch.equal(a, c) for a, c in zip(run(), want))
 
 
+def test_broadcast_operands_and_inference_mode():
+    """Expanded inputs count once for every place they stand in, and their gradients are summed back; inference tensors go through."""
+    g = gen(101)
+    x, w = normal(g, 40, 64, dtype=BF16).requires_grad_(True), normal(g, 48, 64, dtype=BF16, std=0.2).requires_grad_(True)
+    row = normal(g, 48, dtype=BF16).requires_grad_(True)
+    mod = normal(g, 64).requires_grad_(True)
+    one = normal(g, 1, dtype=BF16).requires_grad_(True)
+    dy = normal(g, 3, 40, 48, dtype=BF16)
+
+    def wide(x, w, row, mod, one):
+        h = llsa_b200.layer_norm(x.expand(3, 40, 64), one.expand(64), scale=mod.expand(3, 64), shift=mod.expand(3, 64))
+        return llsa_b200.linear(h, w, one.expand(48), residual=row.expand(3, 40, 48), gate=row.expand(3, 48))
+
+    def dense(x, w, row, mod, one):
+        c = lambda t, *shape: t.expand(*shape).contiguous()
+        h = llsa_b200.layer_norm(c(x, 3, 40, 64), c(one, 64), scale=c(mod, 3, 64), shift=c(mod, 3, 64))
+        return llsa_b200.linear(h, w, c(one, 48), residual=c(row, 3, 40, 48), gate=c(row, 3, 48))
+
+    leaves = [x, w, row, mod, one]
+    a, b = wide(*leaves), dense(*leaves)
+    assert torch.equal(a, b)
+    for p, q in zip(torch.autograd.grad(a, leaves, dy), torch.autograd.grad(b, leaves, dy)):
+        assert torch.equal(p, q)
+    with torch.inference_mode():
+        y = wide(*[t.detach() for t in leaves])
+        z = llsa_b200.rope_axes(y.view(3, 1, 40, 48), torch.arange(40, device=DEV)[:, None], (48,))
+    assert torch.equal(y, a) and torch.isfinite(z).all()
+    assert torch.equal(llsa_b200.linear(x[0], w), llsa_b200.linear(x[:1], w)[0]) and torch.equal(llsa_b200.layer_norm(x[0]), llsa_b200.layer_norm(x[:1])[0])
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 elements: the last rows have the bits that a call of them alone has, and no others."""
     g = gen(91)
