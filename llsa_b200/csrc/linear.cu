@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include "linear.cuh"
+#include "tc05.cuh"
 #include "vec.cuh"
 
 namespace llsa {
@@ -21,7 +22,7 @@ using bf16 = __nv_bfloat16;
 // TH TM x TH TM outputs (TH = 16, or 8 for CTAs of two warps), a thread TM x TM of them.  Steps of 16 along k: the next step's operands are on their way in
 // registers while this one's are multiplied from shared memory, where either stands as 16 rows of neighbours in i or j (turned on the way in if memory has it
 // along k), so that a thread's fours are one load.  TM^2 multiply-adds a k against TM / 2 such loads: the FMA pipe is what bounds it, with two CTAs to an SM.
-// 16384 x 384 -> 1536: 437 us forward, 469 dx, 407 dw (44, 41 and 47 TFLOP/s; cuBLAS 500 forward, 406 dw).  2048 x 384 -> 384: 31 us, 192 tiles of 64 x 64 on
+// 16384 x 384 -> 1536: 437 us forward, 468 dx, 390 dw (44, 41 and 50 TFLOP/s; cuBLAS 500 forward, 406 dw).  2048 x 384 -> 384: 31 us, 192 tiles of 64 x 64 on
 // 148 SMs, of which 44 have two, and there shared memory is the pace (cuBLAS 27); operands four steps ahead instead of one change nothing.
 template <int TM, int TH, bool ALONG_K>
 struct Operand {
@@ -98,16 +99,19 @@ struct Operand {
   }
 };
 
-template <int TM, int TH, bool A_K, bool B_K, bool PARTIAL>
+// S > 1: a cluster of S CTAs takes a tile, an S-th of the sum each; they leave their sums in shared memory, and every one adds an S-th of the rows up, in order
+template <int TM, int TH, int S, bool A_K, bool B_K, bool PARTIAL>
 __global__ void __launch_bounds__(TH * TH, TH == 16 ? 2 : 4)
 product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial, int64_t partial_ld, int64_t tiles_n, int64_t per_split, int vec_a, int vec_b) {
   using A = Operand<TM, TH, A_K>;
   using B = Operand<TM, TH, B_K>;
   constexpr int BM = TH * TM, BK = 16;
-  __shared__ __align__(16) float s_a[2][A::kFloats], s_b[2][B::kFloats];
+  __shared__ __align__(16) float s_ab[4][A::kFloats];
+  float(*s_a)[A::kFloats] = s_ab, (*s_b)[A::kFloats] = s_ab + 2;
   const int tx = threadIdx.x % TH, ty = threadIdx.x / TH;
-  const int64_t i0 = blockIdx.x / tiles_n * BM, j0 = blockIdx.x % tiles_n * BM;
-  const int64_t k_first = blockIdx.y * per_split, k_end = PARTIAL ? min(p.K, k_first + per_split) : p.K;
+  const uint32_t tile = blockIdx.x / S, rank = blockIdx.x % S;
+  const int64_t i0 = tile / tiles_n * BM, j0 = tile % tiles_n * BM;
+  const int64_t k_first = (S > 1 ? rank : blockIdx.y) * per_split, k_end = min(p.K, k_first + per_split);
   float2 acc[TM][TM / 2];                                    // two neighbours an instruction, the same multiply-adds
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -142,10 +146,38 @@ product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial,
         for (int j = 0; j < TM / 2; ++j) acc[i][j] = __ffma2_rn(make_float2(u[i], u[i]), make_float2(v[2 * j], v[2 * j + 1]), acc[i][j]);
     }
   }
+  if constexpr (S > 1) {
+    static_assert(TM % S == 0 && 4 * A::kFloats >= BM * A::kLd, "rows of a thread in equal shares; a tile of sums where the operands stood");
+    float* sums = &s_ab[0][0];
+    __syncthreads();                                         // the last step's readers are through
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TM / 2; j += 2)
+        *reinterpret_cast<float4*>(sums + A::row(ty, i) * A::kLd + B::row(tx, 2 * j)) = make_float4(acc[i][j].x, acc[i][j].y, acc[i][j + 1].x, acc[i][j + 1].y);
+    tc::cluster_sync_all();
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      if (i / (TM / S) == rank)
+#pragma unroll
+        for (int j = 0; j < TM / 2; j += 2) {
+          float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (uint32_t q = 0; q < S; ++q) {
+            float4 u;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w)
+                         : "r"(tc::at_rank(sums + A::row(ty, i) * A::kLd + B::row(tx, 2 * j), q)) : "memory");
+            t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+          }
+          acc[i][j] = make_float2(t.x, t.y);
+          acc[i][j + 1] = make_float2(t.z, t.w);
+        }
+    tc::cluster_sync_all();                                  // nobody's sums are read any more
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int64_t r = i0 + A::row(ty, i);
-    if (r >= p.M) continue;
+    if (r >= p.M || (S > 1 && i / (TM / S) != rank)) continue;
     const int64_t sample = !PARTIAL && e.gate.p ? (uint32_t) r / e.rows_per_gate : 0;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
@@ -168,25 +200,35 @@ product_kernel(Product<float> p, Epilogue<float> e, float* __restrict__ partial,
 
 template <bool A_K, bool B_K, bool PARTIAL>
 int launch_product(const Product<float>& p, const Epilogue<float>& e, float* partial, int64_t ld, cudaStream_t st) {
-  const int64_t split = PARTIAL ? p.split : 1;
   auto tiles = [&](int64_t b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); };
-  const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
   auto vec = [](const Mat<const float>& m) { return (uintptr_t) m.p % 16 == 0 && m.ld % 4 == 0; };
-  auto go = [&](auto kernel, int64_t b, unsigned threads) {
-    launch_pdl(kernel, dim3((unsigned) tiles(b), (unsigned) split), dim3(threads), 0, st, p, e, partial, ld, (p.N + b - 1) / b, per, (int) vec(p.a), (int) vec(p.b));
+  // split: parts of the sum, a CTA each: along y in memory, or the `cluster` CTAs of a tile
+  auto go = [&](auto kernel, int64_t b, unsigned threads, int64_t split, unsigned cluster) {
+    const int64_t per = ((p.K + split - 1) / split + 15) / 16 * 16;
+    launch_pdl_cluster(kernel, dim3((unsigned) (tiles(b) * cluster), (unsigned) (PARTIAL ? split : 1)), dim3(threads), cluster, 0, st, p, e, partial, ld,
+                       (p.N + b - 1) / b, per, (int) vec(p.a), (int) vec(p.b));
   };
-  LLSA_REQUIRE(tiles(32) <= INT32_MAX, LLSA_ERR_SHAPE, "linear: too many outputs");
-  // the largest tile that still gives every SM one; parts in tiles of 64 x 64 that two warps hold, which fill four to an SM evenly (dw of 16384 x 384 -> 1536
-  // 407 us, in tiles of 128 x 128 446; of 2048 x 384 -> 384 24.4 and 28.9.  Forward 469 and 437: their operands are turned on the way in)
-  const bool large = tiles(128) >= 148, middle = tiles(64) * split >= 148;
+  LLSA_REQUIRE(tiles(32) <= INT32_MAX / 8, LLSA_ERR_SHAPE, "linear: too many outputs");
+  const int64_t t = tiles(64), steps = (p.K + 15) / 16;
   if constexpr (PARTIAL) {
-    if (middle) go(product_kernel<8, 8, A_K, B_K, true>, 64, 64);
-  } else if (large) {
-    go(product_kernel<8, 16, A_K, B_K, false>, 128, 256);
-  } else if (middle) {
-    go(product_kernel<4, 16, A_K, B_K, false>, 64, 256);
+    // parts in tiles of 64 x 64 that two warps hold, which fill four to an SM evenly (dw of 16384 x 384 -> 1536 390 us, in tiles of 128 x 128 446; of
+    // 2048 x 384 -> 384 24 and 29)
+    if (t * p.split >= 148) go(product_kernel<8, 8, 1, A_K, B_K, true>, 64, 64, p.split, 1);
+    else go(product_kernel<2, 16, 1, A_K, B_K, true>, 32, 256, p.split, 1);
+  } else {
+    // the largest tile that still gives every SM one (forward of 16384 x 384 -> 1536 in tiles of two warps 469 us, 437 so: operands are turned on the way in);
+    // where there are few, their sums in 2 to 8 parts of 16 steps at least, of 4 where not every SM has a tile.  us, without and so: 512 x 1536 -> 384 60 / 28
+    // (cuBLAS 36), 300 x 389 -> 771 28 / 19 (17), dx of 2048 x 384 -> 1536 107 / 79; 2048 x 384 -> 384 would be 31 / 33, 8 x 256 -> 384 8 / 10
+    int64_t S = 1;
+    while (S < 8 && t * S * 2 <= 148 * 6 && steps / (2 * S) >= (t >= 148 ? 16 : 4)) S *= 2;
+    if (t * S < 148 && steps < 32) S = 1;
+    if (tiles(128) >= 148) go(product_kernel<8, 16, 1, A_K, B_K, false>, 128, 256, 1, 1);
+    else if (S == 8) go(product_kernel<8, 8, 8, A_K, B_K, false>, 64, 64, S, 8);
+    else if (S == 4) go(product_kernel<8, 8, 4, A_K, B_K, false>, 64, 64, S, 4);
+    else if (S == 2) go(product_kernel<8, 8, 2, A_K, B_K, false>, 64, 64, S, 2);
+    else if (t >= 148) go(product_kernel<4, 16, 1, A_K, B_K, false>, 64, 256, 1, 1);
+    else go(product_kernel<2, 16, 1, A_K, B_K, false>, 32, 256, 1, 1);
   }
-  if (!middle && (PARTIAL || !large)) go(product_kernel<2, 16, A_K, B_K, PARTIAL>, 32, 256);
   LLSA_LAUNCH_OK("product_kernel");
   return LLSA_OK;
 }

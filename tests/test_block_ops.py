@@ -206,6 +206,13 @@ def test_linear_against_its_formula(B, N, K, F, dtype, form):
     check_linear(t, dy, act, y, grads, dtype)
 
 
+# fp32 products of few tiles: their sums in 2, 4 and 8 parts over a cluster, forward or in dx, with ragged ends of every size
+@pytest.mark.parametrize("B,N,K,F", [(2, 1000, 384, 640), (1, 1999, 660, 380), (2, 150, 389, 771), (4, 130, 1536, 384), (2, 1000, 384, 1152), (1, 70, 4099, 66)])
+@pytest.mark.parametrize("form", FORMS, ids=[f[0] for f in FORMS])
+def test_fp32_sums_over_a_cluster(B, N, K, F, form):
+    test_linear_against_its_formula(B, N, K, F, F32, form)
+
+
 def check_linear(t, dy, act, y, grads, dtype):
     M, K, F = dy.numel() // dy.shape[-1], t["x"].shape[-1], dy.shape[-1]
     ref = linear_reference(t["x"], t["w"], t.get("b"), act, t.get("r"), t.get("g"), dy)
