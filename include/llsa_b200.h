@@ -61,7 +61,7 @@ typedef struct LlsaTensor {
   int64_t stride[4]; /* in elements */
 } LlsaTensor;
 
-int llsa_version(void);
+int llsa_version(void);      /* 103: llsa_layer_norm_*, llsa_linear_*, llsa_rope_axes */
 const char* llsa_last_error_string(void);
 /* LLSA_OK for a status word of 0, else LLSA_ERR_DEVICE_CHECK with the error string naming the bits
  * (`status_word` is the value the caller copied back from the device). */
