@@ -155,9 +155,9 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*s_red)[32][2], 
 }
 
 // CTAs that an SM should hold, by threads, by values of a thread and their type: registers are what decides (fp32, 12 values: four CTAs 75 us, three 71.5;
-// shifted, 16 values: bf16 three 87.5 us, two 100, fp32 49.5 and 45.6)
+// shifted, 16 values: bf16 three 87.5 us, two 100, fp32 49.5 and 45.6; 20 values: fp32 44 and 34)
 constexpr int fwd_ctas(int tpb, int form, int e, int bytes) {
-  return tpb > 256 ? 1 : form == kWhole ? (bytes == 2 || e <= 8 ? 4 : 3) : form == kShifted ? (e <= 8 ? 4 : bytes == 2 ? 3 : 2) : e <= 12 ? 4 : 3;
+  return tpb > 256 ? 1 : form == kWhole ? (bytes == 2 || e <= 8 ? 4 : 3) : form == kShifted ? (e <= 8 ? 4 : e > 16 ? 2 : bytes == 2 ? 3 : 2) : e <= 12 ? 4 : 3;
 }
 constexpr int bwd_ctas(int tpb) { return tpb > 256 ? 1 : 2; }
 
@@ -380,12 +380,12 @@ layer_norm_bwd_kernel(Rows<const T> dy, Rows<const T> x, NormParams par, const f
 }
 
 // ------------------------------------------------------------------------------------------------ choice of the kernel
-// The fewest warps to a row whose threads hold at most 16 channels each.
+// The fewest warps to a row whose threads hold at most 16 channels each, but for one case.
 struct Split {
   int form, r, warps, threads;
 };
 // whole: rows on the boundaries of their vectors; alike: all of a call's rows begin equally far behind one, and four rows on again
-Split split_of(int64_t C, bool whole, bool alike) {
+Split split_of(int64_t C, bool whole, bool alike, bool fwd) {
   Split s;
   s.form = whole ? kWhole : alike && C + 3 <= 2048 ? kShifted : kSingle;
   const int64_t vec = s.form == kSingle ? 1 : 4, span = C + (s.form == kShifted ? 3 : 0);
@@ -394,6 +394,12 @@ Split split_of(int64_t C, bool whole, bool alike) {
   s.r = (int) ((span + vec * 32 * s.warps - 1) / (vec * 32 * s.warps));
   // rows a multiple of four apart begin alike: four groups at least
   s.threads = s.form == kShifted && s.warps == 4 ? 512 : 256;
+  // forward: two warps with 20 values a thread have two CTAs to an SM (3 x 5377 rows of 1155: fp32 34.4 us, four warps of 512 threads 43; bf16 35 and 46)
+  if (fwd && s.threads == 512 && span <= 1280) {
+    s.warps = 2;
+    s.r = 5;
+    s.threads = 256;
+  }
   if (s.warps > 8) {
     s.threads = 1024;
     s.warps = 32;
@@ -402,7 +408,7 @@ Split split_of(int64_t C, bool whole, bool alike) {
   return s;
 }
 template <typename T, typename... Ts>
-Split split_for(const LlsaTensor* x, Ts... others) {
+Split split_for(bool fwd, const LlsaTensor* x, Ts... others) {
   const LlsaTensor* const t[] = {x, others...};
   const int64_t es = sizeof(T);
   bool whole = true, alike = true;
@@ -413,7 +419,7 @@ Split split_for(const LlsaTensor* x, Ts... others) {
     alike = alike && ((uintptr_t) u->ptr / es) % 4 == ((uintptr_t) x->ptr / es) % 4 && sn % 4 == sn0 % 4 && sb % 4 == sb0 % 4 &&
             (x->shape[0] == 1 || sb % 4 == (x->shape[1] * u->stride[1]) % 4) && (x->shape[1] > 1 || sb % 4 == u->stride[1] % 4);
   }
-  return split_of(x->shape[2], whole, alike);
+  return split_of(x->shape[2], whole, alike, fwd);
 }
 template <typename T>
 Rows<T> make_rows(const LlsaTensor* t) {
@@ -477,6 +483,7 @@ Chunks chunks_of(int64_t B, int64_t N, int64_t C) {
   else LLSA_NORM_R(kShifted, 4, false, 256, __VA_ARGS__)                                                        \
   else LLSA_NORM_R(kShifted, 3, true, 256, __VA_ARGS__)                                                         \
   else LLSA_NORM_R(kShifted, 4, true, 256, __VA_ARGS__)                                                         \
+  else LLSA_NORM_R(kShifted, 5, true, 256, __VA_ARGS__)                                                         \
   else LLSA_NORM_R(kShifted, 3, true, 512, __VA_ARGS__)                                                         \
   else LLSA_NORM_R(kShifted, 4, true, 512, __VA_ARGS__)                                                         \
   else LLSA_NORM_R(kSingle, 16, false, 256, __VA_ARGS__)                                                        \
@@ -498,7 +505,7 @@ template <typename T>
 int launch_fwd(const LlsaTensor* x, const NormParams& par, float eps, const LlsaTensor* y, float2* stats, cudaStream_t st) {
   const uint32_t M = (uint32_t) (x->shape[0] * x->shape[1]), N = (uint32_t) x->shape[1];
   const int C = (int) x->shape[2];
-  const Split sp = split_for<T>(x, y);
+  const Split sp = split_for<T>(true, x, y);
   const int64_t groups = sp.threads / (32 * sp.warps);
   const Rows<const T> xr = make_rows<const T>(x);
   const Rows<T> yr = make_rows<T>(y);
@@ -515,7 +522,7 @@ template <typename T>
 int launch_bwd(const LlsaTensor* dy, const LlsaTensor* x, const NormParams& par, const float2* stats, const LlsaTensor* dx, float* partial,
                const Chunks& ch, cudaStream_t st) {
   const int C = (int) x->shape[2];
-  const Split sp = split_for<T>(x, dy, dx);
+  const Split sp = split_for<T>(false, x, dy, dx);
   const Rows<const T> gr = make_rows<const T>(dy), xr = make_rows<const T>(x);
   const Rows<T> dr = make_rows<T>(dx);
   const unsigned grid = (unsigned) (ch.B * ch.chunks);
