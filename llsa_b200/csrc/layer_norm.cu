@@ -37,7 +37,8 @@ struct NormParams {
 // The part of a row that one thread of a group of `threads` holds: R vectors of VEC channels, `threads` vectors apart.
 //   kWhole   vectors of four on their boundaries; R is no larger than C asks for, and only the last one may lie behind the row's end
 //   kLoose   the same, with any of them behind the end
-//   kShifted rows of any length, whose vectors of four begin `m` channels in front of the row, on their boundary; those over the row's ends go element by element
+//   kShifted rows of any length, whose vectors of four begin `m` channels in front of the row, on their boundary; those over the row's ends go element by element.
+//            R is no larger than C + 3 asks for: only the first vector begins in front of the row, only the last two may lie behind its end
 //   kSingle  element by element
 enum Form { kWhole, kLoose, kShifted, kSingle };
 template <typename T, int FORM, int R>
@@ -48,19 +49,22 @@ struct Slice {
   static __device__ __forceinline__ int channel(int e, int t, int threads, int m) { return ((e / VEC) * threads + t) * VEC + e % VEC - (FORM == kShifted ? m : 0); }
   static __device__ __forceinline__ bool there(int e, int c, int C) {
     if (FORM == kWhole) return e / VEC < R - 1 || c < C;
-    return FORM == kShifted ? (unsigned) c < (unsigned) C : c < C;
+    if (FORM == kShifted) return (e / VEC > 0 || c >= 0) && (e / VEC < R - 2 || c < C);
+    return c < C;
   }
+  // All of a shifted vector
+  static __device__ __forceinline__ bool all_there(int i, int c, int C) { return (i > 0 || c >= 0) && (i < R - 2 || c + VEC <= C); }
   __device__ __forceinline__ void load(const T* row, int t, int threads, int C, int m) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int c = channel(i * VEC, t, threads, m);
-      if (FORM != kShifted ? there(i * VEC, c, C) : c >= 0 && c + VEC <= C) {
+      if (FORM != kShifted ? there(i * VEC, c, C) : all_there(i, c, C)) {
         raw[i] = *reinterpret_cast<const typename P::type*>(row + c);
       } else if (FORM == kShifted) {
         T* u = reinterpret_cast<T*>(&raw[i]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          if (there(0, c + j, C)) u[j] = row[c + j];
+          if (there(i * VEC + j, c + j, C)) u[j] = row[c + j];
       }
     }
   }
@@ -84,13 +88,13 @@ struct Slice {
     for (int i = 0; i < R; ++i) {
       const int c = channel(i * VEC, t, threads, m);
       const typename P::type w = P::pack(reinterpret_cast<const float*>(v) + i * VEC);
-      if (FORM != kShifted ? there(i * VEC, c, C) : c >= 0 && c + VEC <= C) {
+      if (FORM != kShifted ? there(i * VEC, c, C) : all_there(i, c, C)) {
         *reinterpret_cast<typename P::type*>(row + c) = w;
       } else if (FORM == kShifted) {
         const T* u = reinterpret_cast<const T*>(&w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          if (there(0, c + j, C)) row[c + j] = u[j];
+          if (there(i * VEC + j, c + j, C)) row[c + j] = u[j];
       }
     }
   }
@@ -164,7 +168,8 @@ constexpr int bwd_ctas(int tpb) { return tpb > 256 ? 1 : 2; }
 // TPB: threads of a CTA; MULTI: more than one warp to a row.  A CTA takes rows [blockIdx.x * per, + per): neighbours, so that a group's sample, and with it A and
 // T, changes rarely.  (Rows a grid apart had them loaded for nearly every row: 8 x 16384 rows of 384 channels 77 us, 44 so.)
 // Measured (bf16 unless said): 8 x 16384 rows of 384 channels 39.6 us (5.1 TB/s), in fp32 71.5 (5.6); 8 x 16384 of 768 92.7; 2 x 8192 of 2048 35.6; with A and T
-// in registers, which spill, 43.6, 81.7, 105 and 40.6.  Shifted, 8 x 16384 rows of 390: 87.5 (104 in registers); 4 x 4096 of 770: 28.2 (53).  Two rows on their way are worth 1 us of the first and cost 12 of the 768 channels' 93.
+// in registers, which spill, 43.6, 81.7, 105 and 40.6.  Shifted, 8 x 16384 rows of 390: 75 (every vector looked at 94); 4 x 4096 of 770: 26 (31).  Two rows on
+// their way are worth 1 us of the first and cost 12 of the 768 channels' 93.
 template <typename T, int FORM, int R, bool MULTI, int TPB>
 __global__ void __launch_bounds__(TPB, fwd_ctas(TPB, FORM, R * (FORM == kSingle ? 1 : 4), sizeof(T)))
 layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, float2* __restrict__ stats, uint32_t M, uint32_t N, uint32_t per, int C, int warps) {
@@ -279,7 +284,7 @@ layer_norm_fwd_kernel(Rows<const T> x, NormParams par, float eps, Rows<T> y, flo
 // A CTA takes rows [s * per, (s + 1) * per) of sample b, chunk = b * chunks + s, and leaves its two column sums in partial[chunk][2][C] (NULL: none are wanted).
 // Of shifted rows every group holds other channels in a thread than its neighbour: the sums meet by channel in shared memory.
 // Measured, the parameters' gradients included (bf16 unless said): 8 x 16384 rows of 384 channels 58.4 us (5.2 TB/s), in fp32 99.6 (6.1); 8 x 16384 of 768 123.6;
-// 2 x 8192 of 2048 53.5; 3 x 5377 of 1155 in fp32, shifted, 56.  With one row on its way instead of two 68.3 and 131.5 (384 and 768); of 16 values to a
+// 2 x 8192 of 2048 53.5; shifted, 3 x 5377 of 1155 in fp32 56, 8 x 16384 of 390 122.  With one row on its way instead of two 68.3 and 131.5 (384 and 768); of 16 values to a
 // thread, or of fp32, two rows spill (2048: 84.7, fp32 115).
 template <typename T, int FORM, int R, bool MULTI, int TPB>
 __global__ void __launch_bounds__(TPB, bwd_ctas(TPB))
@@ -394,7 +399,7 @@ Split split_of(int64_t C, bool whole, bool alike, bool fwd) {
   s.r = (int) ((span + vec * 32 * s.warps - 1) / (vec * 32 * s.warps));
   // rows a multiple of four apart begin alike: four groups at least
   s.threads = s.form == kShifted && s.warps == 4 ? 512 : 256;
-  // forward: two warps with 20 values a thread have two CTAs to an SM (3 x 5377 rows of 1155: fp32 34.4 us, four warps of 512 threads 43; bf16 35 and 46)
+  // forward: two warps with 20 values a thread have two CTAs to an SM (3 x 5377 rows of 1155: fp32 32.5 us, four warps of 512 threads 43; bf16 29.6 and 46)
   if (fwd && s.threads == 512 && span <= 1280) {
     s.warps = 2;
     s.r = 5;
@@ -466,7 +471,7 @@ Chunks chunks_of(int64_t B, int64_t N, int64_t C) {
 
 // The kernel for a split.  Rows of one warp; of several warps of 256 threads; of 512, which has four groups of four; of all of 1024, above 4096 channels.
 #define LLSA_NORM_R(F_, R_, W_, T_, ...)                                                                        \
-  if (sp.form == F_ && sp.r <= R_ && (sp.warps > 1) == W_ && sp.threads == T_) {                                 \
+  if (sp.form == F_ && (F_ == kWhole || F_ == kShifted ? sp.r == R_ : sp.r <= R_) && (sp.warps > 1) == W_ && sp.threads == T_) { \
     constexpr int FORM = F_, R = R_, TPB = T_;                                                                  \
     constexpr bool MULTI = W_;                                                                                  \
     __VA_ARGS__;                                                                                                \
@@ -479,7 +484,9 @@ Chunks chunks_of(int64_t B, int64_t N, int64_t C) {
   else LLSA_NORM_R(kWhole, 3, true, 256, __VA_ARGS__)                                                           \
   else LLSA_NORM_R(kWhole, 4, true, 256, __VA_ARGS__)                                                           \
   else LLSA_NORM_R(kLoose, 4, true, 1024, __VA_ARGS__)                                                          \
+  else LLSA_NORM_R(kShifted, 1, false, 256, __VA_ARGS__)                                                        \
   else LLSA_NORM_R(kShifted, 2, false, 256, __VA_ARGS__)                                                        \
+  else LLSA_NORM_R(kShifted, 3, false, 256, __VA_ARGS__)                                                        \
   else LLSA_NORM_R(kShifted, 4, false, 256, __VA_ARGS__)                                                        \
   else LLSA_NORM_R(kShifted, 3, true, 256, __VA_ARGS__)                                                         \
   else LLSA_NORM_R(kShifted, 4, true, 256, __VA_ARGS__)                                                         \

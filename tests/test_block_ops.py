@@ -87,6 +87,26 @@ def test_layer_norm_against_its_formula(B, N, C, dtype, given):
         within("d" + k, d, ref[k][0], (200 + B * N) * U * ref[k][1])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("C", [121, 125, 126, 127, 129, 130, 253, 254, 255, 257, 258, 381, 382, 383, 385, 386, 509, 510, 511, 513, 514, 765, 767, 769, 1019, 1021, 1022, 1023, 1025, 1026, 1027,
+                               1277, 1278, 1279, 1281, 1533, 1535, 1537, 2043, 2045, 2046])
+def test_layer_norm_rows_that_end_beside_a_vector(C, dtype):
+    """Rows one to three channels around every multiple of what a group's vectors hold, in a tensor that begins on any of the four places beside a boundary."""
+    for start in range(4):
+        g = gen(7 * C + start)
+        x = normal(g, start + 2 * 9 * C, dtype=dtype)[start:].view(2, 9, C)
+        dy = normal(g, start + 2 * 9 * C, dtype=dtype)[start:].view(2, 9, C)
+        w, b, s, t = normal(g, C), normal(g, C), normal(g, 2, C, std=0.3), normal(g, 2, C)
+        leaves = [v.detach().requires_grad_(True) for v in (x, w, b, s, t)]
+        y = llsa_b200.layer_norm(*leaves[:3], 1e-5, scale=leaves[3], shift=leaves[4])
+        grads = torch.autograd.grad(y, leaves, dy)
+        ref = norm_reference(x, w, b, s, t, 1e-5, dy)
+        within("y", y, ref["y"][0], 120 * U * ref["y"][1])
+        within("dx", grads[0], ref["x"][0], 300 * U * ref["x"][1])
+        for k, d in zip("wbst", grads[1:]):
+            within("d" + k, d, ref[k][0], 218 * U * ref[k][1])
+
+
 @pytest.mark.parametrize("param", [BF16, F32])
 def test_layer_norm_takes_parameters_of_either_type(param):
     g = gen(3)
