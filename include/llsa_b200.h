@@ -179,7 +179,7 @@ typedef struct LlsaLinearArgs {
 int llsa_linear_fwd(const LlsaLinearArgs* args, void* stream);
 /* 1 where the backward reads `pre`, 0 where it does without, from the shapes of x, weight and gate and the activation; -1 where these are refused */
 int llsa_linear_keeps_product(const LlsaLinearArgs* args);
-/* Read from the shapes of x, weight and gate, dy, the activation and which results are wanted; -1 where these are refused */
+/* Read from the shapes of x, weight and gate, dy, the activation and which results are wanted; 0 without rows; -1 where these are refused */
 int64_t llsa_linear_bwd_workspace_bytes(const LlsaLinearArgs* args);
 int llsa_linear_bwd(const LlsaLinearArgs* args, void* stream);
 

@@ -561,6 +561,11 @@ int check_common(const LlsaLinearArgs* a, Plan* p) {
 // What the backward does, from the shapes and from which results are asked for
 void plan_bwd(const LlsaLinearArgs* a, Plan* p) {
   const int es = (int) dtype_size(p->dtype);
+  if (p->M == 0) {             // no product to split and nothing to keep
+    p->write_dz = p->sums = p->slope = p->by_sample = false;
+    p->bytes = 0;
+    return;
+  }
   // dy itself is dz without an activation and a gate, where the tensor cores can read it
   p->write_dz = a->activation != kActNone || a->gate || (p->dtype == LLSA_BF16 && !(a->dy && rows16(a->dy)));
   p->by_sample = by_sample(a, *p);
@@ -785,7 +790,7 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
   LLSA_REQUIRE(!p.by_sample || rows16(a->dy), LLSA_ERR_STRIDE, "dy: rows must start on 16-byte boundaries for a gate of long samples");
   LLSA_REQUIRE(!p.by_sample || !a->dx || rows16(a->dx), LLSA_ERR_STRIDE, "dx: rows must start on 16-byte boundaries for a gate of long samples");
   LLSA_REQUIRE(!p.by_sample || !a->dweight || (uintptr_t) a->dweight->ptr % 16 == 0, LLSA_ERR_STRIDE, "dweight: must start on a 16-byte boundary for a gate of long samples");
-  LLSA_REQUIRE(a->pre || !((a->dgate && !p.by_sample) || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
+  LLSA_REQUIRE(p.M == 0 || a->pre || !((a->dgate && !p.by_sample) || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
   if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;
   const int64_t ws[2] = {p.F, p.K}, gs[2] = {p.B, p.F}, bs[1] = {p.F};
   if (a->dweight && (rc = check_contig(a->dweight, "dweight", p.dtype, 2, ws))) return rc;

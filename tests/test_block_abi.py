@@ -3,6 +3,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -93,6 +94,27 @@ def test_linear_backward_wants_its_workspace():
         assert lib.llsa_linear_bwd(ref(a), None) == ERR_WORKSPACE
     bad, keep2 = linear_args(weight=fake((48, 40)))
     assert lib.llsa_linear_bwd_workspace_bytes(ref(bad)) == -1 and lib.llsa_linear_keeps_product(ref(bad)) == -1
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act,gated", [(0, False), (1, False), (2, False), (0, True)])
+def test_linear_backward_without_rows_wants_no_workspace(dtype, act, gated):
+    """In a process of its own: what goes wrong in a plan for no rows may end it."""
+    code = '''
+import ctypes as C, torch
+from test_block_abi import _lib, fake, linear_args
+F = 48
+given = dict(y=None, x=fake((0, 32), {0}), weight=fake((F, 32), {0}), dy=fake((0, F), {0}), dx=fake((0, 32), {0}))
+if {2}:
+    given["gate"] = fake((3, F), {0})
+a, keep = linear_args(M=0, F=F, dtype={0}, act={1}, **given)
+lib = _lib.lib()
+assert lib.llsa_linear_bwd_workspace_bytes(C.byref(a)) == 0
+assert lib.llsa_linear_bwd(C.byref(a), None) == 0, lib.llsa_last_error_string()
+'''.format(dtype, act, gated)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(__file__),
+                       env=dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(os.path.dirname(os.path.abspath(__file__))), os.path.dirname(os.path.abspath(__file__))])))
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
 
 
 # long samples, and one step beside each side of the rule

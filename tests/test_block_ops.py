@@ -572,6 +572,30 @@ def test_nothing_to_do(dtype):
     assert llsa_b200.rope_axes(x, torch.zeros(5, 1, device=DEV), (16,)).shape == x.shape
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act,gated", [(0, False), (1, False), (0, True)])
+def test_c_backward_without_rows_clears_the_parameters_gradients(dtype, act, gated):
+    import ctypes as C
+    from llsa_b200 import _lib
+    K, F = 32, 48
+    room = torch.zeros(1, 64, device=DEV, dtype=dtype)            # rows that begin somewhere
+    outs = dict(dweight=torch.full((F, K), 7.0, device=DEV, dtype=dtype), dbias=torch.full((F,), 7.0, device=DEV, dtype=dtype))
+    given = dict(x=room[:0, :K], weight=torch.ones(F, K, device=DEV, dtype=dtype), dy=room[:0, :F], dx=room[:0, :K], **outs)
+    if gated:
+        given.update(gate=torch.ones(3, F, device=DEV, dtype=dtype), dgate=torch.full((3, F), 7.0, device=DEV, dtype=dtype))
+        outs["dgate"] = given["dgate"]
+    a, keep = _lib.LlsaLinearArgs(), {}
+    for name, t in given.items():
+        keep[name] = _lib.desc(t)
+        keep[name].ptr = keep[name].ptr or room.data_ptr()        # torch gives an empty tensor no address
+        setattr(a, name, C.pointer(keep[name]))
+    a.activation = act
+    assert _lib.lib().llsa_linear_bwd_workspace_bytes(C.byref(a)) == 0
+    assert _lib.lib().llsa_linear_bwd(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0, _lib.lib().llsa_last_error_string()
+    for name, t in outs.items():
+        assert not t.any(), name
+
+
 def test_refusals():
     x, w = torch.zeros(2, 4, 16, device=DEV), torch.zeros(8, 16, device=DEV)
     r, gate = torch.zeros(2, 4, 8, device=DEV), torch.zeros(2, 8, device=DEV)
