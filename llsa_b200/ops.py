@@ -158,8 +158,19 @@ def _saved_specs(B, H, N, D, dtype, topk1, topk2, block_size, levels):
     return specs
 
 
+def _unit_columns(x: torch.Tensor) -> torch.Tensor:
+    """As csrc/host_block.cpp: a dense copy where the channels are apart."""
+    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _like_rows(x: torch.Tensor) -> torch.Tensor:
+    """As csrc/host_block.cpp: a result laid out as x is, where that leaves the last dimension dense."""
+    y = torch.empty_like(x)
+    return y if y.shape[-1] == 1 or y.stride(-1) == 1 else x.new_empty(x.shape)
+
+
 def _register_fakes() -> None:
-    """Shapes of the native operators for tracing."""
+    """Shapes and strides of the native operators' results for tracing."""
     @torch.library.register_fake("llsa_b200::layer_fwd")
     def _(q, k, v, freq, wq, wk, eps, topk1, topk2, block_size, levels):
         specs = _saved_specs(*q.shape, q.dtype, topk1, topk2, block_size, levels)
@@ -173,7 +184,7 @@ def _register_fakes() -> None:
 
     @torch.library.register_fake("llsa_b200::layer_norm_fwd")
     def _(x, weight, bias, scale, shift, eps, want_stats):
-        y = torch.empty_like(x)
+        y = _like_rows(x.contiguous() if x.dim() > 3 else _unit_columns(x))
         return [y, x.new_empty((x.numel() // x.shape[-1] * 2,), dtype=torch.float32)] if want_stats else [y]
 
     @torch.library.register_fake("llsa_b200::layer_norm_bwd")
@@ -203,7 +214,7 @@ def _register_fakes() -> None:
 
     @torch.library.register_fake("llsa_b200::rope_axes")
     def _(x, positions, axes_dims, theta, inverse):
-        return torch.empty_like(x)
+        return _like_rows(_unit_columns(x))
 
     @torch.library.register_fake("llsa_b200::attn_fwd")
     def _(q, k, v, pk, pv, pk2, pv2, indices, p_indices, topk, topk_p, block_size, w1, w2):

@@ -66,3 +66,108 @@ def test_operators_as_torch_library_checks_them(layout):
         torch.library.opcheck(L.attn_fwd.default, args + (dbg["indices"], *lists, 16, 16.0, 256.0), test_utils=which)
         torch.library.opcheck(L.attn_bwd.default, (do, *args, dbg["o"], dbg["lse"], dbg["indices"], *lists, 16, 16.0, 256.0, 16.0, 256.0, False),
                               test_utils=which)
+
+
+# Layouts of x [2, 6, 40, 64] or of three dimensions: dense, channels apart, permuted with dense channels, rows with gaps, samples and rows on top of one another
+_LAYOUTS = {
+    "dense": lambda m: m(2, 6, 40, 64),
+    "channels apart": lambda m: m(2, 6, 64, 40).transpose(2, 3),
+    "tokens in front": lambda m: m(2, 40, 6, 64).transpose(1, 2),
+    "everything permuted": lambda m: m(64, 40, 6, 2).permute(3, 2, 1, 0),
+    "gaps": lambda m: m(2, 6, 40, 80)[..., 3:67],
+    "rows on top of one another": lambda m: m(2, 6, 1, 64).expand(2, 6, 40, 64),
+    "samples on top of one another": lambda m: m(1, 6, 40, 64).expand(2, 6, 40, 64),
+    "one number everywhere": lambda m: m(1, 1, 1, 1).expand(2, 6, 40, 64),
+    "three, dense": lambda m: m(2, 40, 64),
+    "three, channels apart": lambda m: m(2, 64, 40).transpose(1, 2),
+    "three, tokens in front": lambda m: m(40, 2, 64).transpose(0, 1),
+    "two, channels apart": lambda m: m(64, 40).t(),
+    "one channel": lambda m: m(2, 40, 6, 1).transpose(1, 2),
+}
+# y's strides, where y is not laid out as empty_like(x) says: the kernels read a dense copy
+_DENSE = {"channels apart", "everything permuted", "gaps", "rows on top of one another", "samples on top of one another", "one number everywhere",
+          "three, channels apart", "two, channels apart"}
+# (four dimensions that do not follow one another)
+_DENSE_NORM = _DENSE | {"tokens in front", "one channel"}
+
+
+def _strides(shape):
+    out = [1]
+    for n in reversed(shape[1:]):
+        out.insert(0, out[0] * n)
+    return tuple(out)
+
+
+@pytest.mark.parametrize("layout", _LAYOUTS)
+def test_traced_results_are_laid_out_as_the_kernels_lay_them_out(layout):
+    """Strides that the shape functions give, against the rule: y as x is, where its channels are dense, else contiguous."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops._native()
+    with FakeTensorMode():
+        x = _LAYOUTS[layout](lambda *shape: torch.empty(shape, device="cuda"))
+        y = torch.ops.llsa_b200.layer_norm_fwd(x, None, None, None, None, 1e-5, True)[0]
+        assert y.shape == x.shape and y.stride() == (_strides(x.shape) if layout in _DENSE_NORM else x.stride())
+        if x.dim() == 4 and x.shape[-1] > 1:
+            y = torch.ops.llsa_b200.rope_axes(x, torch.empty(40, 1, device="cuda"), (64,), 1e4, False)
+            assert y.shape == x.shape and y.stride() == (_strides(x.shape) if layout in _DENSE else x.stride())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("layout", _LAYOUTS)
+def test_traced_layouts_are_the_real_ones(layout, dtype):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ops._ready()
+    L = torch.ops.llsa_b200
+    x = _LAYOUTS[layout](lambda *shape: torch.randn(shape, device=DEV, dtype=dtype))
+    pos = torch.arange(40, device=DEV)[:, None]
+    calls = [lambda x, pos: L.layer_norm_fwd(x, None, None, None, None, 1e-5, False), lambda x, pos: L.layer_norm_fwd(x, None, None, None, None, 1e-5, True)]
+    if x.dim() == 4 and x.shape[-1] > 1:
+        calls.append(lambda x, pos: [L.rope_axes(x, pos, (64,), 1e4, False)])
+    for call in calls:
+        real = call(x, pos)
+        with FakeTensorMode() as mode:
+            traced = call(mode.from_tensor(x), mode.from_tensor(pos))
+        assert [(t.shape, t.stride(), t.dtype) for t in traced] == [(t.shape, t.stride(), t.dtype) for t in real]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_block_operators_as_torch_library_checks_them(dtype):
+    ops._ready()
+    L = torch.ops.llsa_b200
+    which, both = ("test_schema", "test_faketensor"), ("test_schema", "test_faketensor", "test_autograd_registration", "test_aot_dispatch_static")
+    g = torch.Generator(device=DEV).manual_seed(5)
+    r = lambda *shape: torch.randn(shape, generator=g, device=DEV).to(dtype)
+    for C in (64, 61):
+        x, w, b, s, t = r(2, 40, C), r(C), r(C), r(2, C), r(2, C)
+        for xx in (x, r(2, C, 40).transpose(1, 2), r(2, 5, 8, C + 3)[..., 3:]):
+            torch.library.opcheck(L.layer_norm_fwd.default, tuple(v.detach().requires_grad_(True) for v in (xx, w, b, s, t)) + (1e-5, False), test_utils=both)
+        stats = L.layer_norm_fwd(x, w, b, s, t, 1e-5, True)[1]
+        for want in (0, 3, 15):
+            torch.library.opcheck(L.layer_norm_bwd.default, (r(2, 40, C), x, w, b, s, stats, want, dtype, dtype), test_utils=which)
+    for K, F, N in ((64, 48, 40), (61, 47, 40), (64, 48, 600)):
+        x, w, b, res, gate, dy = r(2, N, K), r(F, K), r(F), r(2, N, F), r(2, F), r(2, N, F)
+        for act, rr, gg in ((0, None, None), (1, None, None), (2, res, None), (0, res, gate)):
+            leaves = [v.detach().requires_grad_(True) if v is not None else None for v in (x, w, b, rr, gg)]
+            torch.library.opcheck(L.linear_fwd.default, (*leaves, act, False, False), test_utils=both)
+            torch.library.opcheck(L.linear_fwd.default, (x, w, b, rr, gg, act, gg is not None or (act > 0 and dtype == torch.float32), True), test_utils=which)
+            pre = L.linear_fwd(x, w, b, rr, gg, act, True, False)[1]
+            torch.library.opcheck(L.linear_bwd.default, (dy, x, w, b, pre, gg, None, None, act, 15 if gg is not None else 7), test_utils=which)
+    pos = torch.arange(40, device=DEV)[:, None]
+    for x in (r(2, 3, 40, 64), r(2, 40, 3, 64).transpose(1, 2), r(2, 3, 64, 40).transpose(2, 3)):
+        torch.library.opcheck(L.rope_axes.default, (x.detach().requires_grad_(True), pos, (64,), 1e4, False), test_utils=both)
+
+
+@pytest.mark.gpu
+def test_model_without_permutation_traces():
+    """Its first layer norm reads the transposed view that the convolution leaves."""
+    from llsa_b200.dit import RopeDiT
+    torch.manual_seed(3)
+    m = RopeDiT(heads=2, layers=1, sample_size=16, attn_type="pixel", token_permutation=False, fused_block=True).to(DEV)
+    x, t = torch.randn(2, 3, 16, 16, device=DEV), torch.tensor([321, 7], device=DEV)
+    with torch.no_grad():
+        want = m(x, t)
+        got = torch.compile(m, backend="aot_eager", fullgraph=True)(x, t)
+    # the projection in front is a convolution of torch's either way, in fp32
+    assert float((got - want).norm()) <= 1e-4 * float(want.norm())
