@@ -198,9 +198,13 @@ def _register_fakes() -> None:
         F, K = weight.shape
         M = x.numel() // K
         out = [x.new_empty((*x.shape[:-1], F))]
-        if want_pre:      # not kept for a gate of long samples (csrc/linear.cu: by_sample)
+        if want_pre:      # as llsa_linear_keeps_product says; not for a gate of long samples (csrc/linear.cu: by_sample)
             N = M // x.shape[0] if gate is not None and x.shape[0] else M
-            kept = M > 0 and not (x.dtype == torch.bfloat16 and gate is not None and N >= 512 and N >= 2 * K and K % 8 == 0 and F % 8 == 0 and x.shape[0] <= 65535)
+            if x.dtype == torch.bfloat16:
+                kept = gate is not None and not (N >= 512 and N >= 2 * K and K % 8 == 0 and F % 8 == 0 and x.shape[0] <= 65535)
+            else:
+                kept = gate is not None or activation != 0
+            kept = kept and M > 0
             out.append(x.new_empty((M if kept else 0, F)))
         if want_copies and x.dtype == torch.bfloat16 and K % 8:
             out += [x.new_empty_strided((n, K), ((K + 7) // 8 * 8, 1)) for n in (M, F)]

@@ -141,6 +141,26 @@ def test_kept_product_is_what_tracing_expects(B, N, K, F, dtype, gated):
     assert out[0].shape == (B, N, F) and out[1].shape == (B * N if keeps else 0, F)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act,gated", [(0, False), (1, False), (2, False), (0, True)])
+@pytest.mark.parametrize("N", [40, 600, 0])
+def test_traced_forward_keeps_the_product_where_the_library_does(dtype, act, gated, N):
+    """Asked to keep it, whatever stands behind the product."""
+    from llsa_b200 import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    B, K, F = 2, 64, 48
+    a, keep = linear_args(M=B * N, K=K, F=F, x=fake_rows(B * N, K, K, dtype), weight=fake_rows(F, K, K, dtype), y=None, act=act,
+                          gate=fake_rows(B, F, F, dtype) if gated else None)
+    keeps = _lib.lib().llsa_linear_keeps_product(ref(a))
+    assert keeps >= 0, _lib.lib().llsa_last_error_string()
+    ops._native()
+    with FakeTensorMode():
+        x, w = torch.empty(B, N, K, dtype=dtype, device="cuda"), torch.empty(F, K, dtype=dtype, device="cuda")
+        r, g = torch.empty(B, N, F, dtype=dtype, device="cuda"), torch.empty(B, F, dtype=dtype, device="cuda")
+        out = torch.ops.llsa_b200.linear_fwd(x, w, None, r if gated else None, g if gated else None, act, True, False)
+    assert out[1].shape == (B * N if keeps else 0, F)
+
+
 def fake_rows(rows, cols, ld, dtype):
     """A descriptor of [rows, cols] with rows `ld` apart, of memory that is nowhere."""
     d = fake((1, cols), dtype)
