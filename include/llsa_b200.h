@@ -145,7 +145,8 @@ int llsa_layer_norm_fwd(const LlsaTensor* x, const LlsaTensor* weight, const Lls
 /* Backward: dx (x's shape, any strides) and those of dweight, dbias [C], dscale, dshift [B,C] that are not NULL (contiguous, F32 or x's type).
  * weight, bias, scale, stats as in the forward.  partial: 1-D F32 scratch of llsa_layer_norm_bwd_partial_elems() elements, wanted where a parameter's
  * gradient is; per_sample = scale or dshift is given.  Where neither is, the samples of dy, x and dx must follow one another
- * (stride[0] == N * stride[1]).  Sums are added in a fixed order. */
+ * (stride[0] == N * stride[1]).  Sums are added in a fixed order, over parts of a sample where either is given and of all rows where neither is: with a
+ * shift and no scale, ask for dshift in every call whose dweight and dbias are to have the same bits. */
 int64_t llsa_layer_norm_bwd_partial_elems(int64_t B, int64_t N, int64_t C, int per_sample);
 int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, const LlsaTensor* weight, const LlsaTensor* bias, const LlsaTensor* scale,
                         const LlsaTensor* stats, const LlsaTensor* dx, const LlsaTensor* dweight, const LlsaTensor* dbias,

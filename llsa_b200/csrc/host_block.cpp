@@ -95,9 +95,10 @@ std::vector<Tensor> layer_norm_fwd(const Tensor& x_, const OptTensor& weight, co
   return out;
 }
 
-// want: 1 weight, 2 bias, 4 scale, 8 shift.  Returns dx and the gradients asked for, in that order; shift's gradient is of shift_type.
+// want: 1 weight, 2 bias, 4 scale, 8 shift.  Returns dx and the gradients asked for, in that order; shift's gradient is of shift_type, which is given where the
+// forward had a shift.
 std::vector<Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const OptTensor& weight, const OptTensor& bias, const OptTensor& scale,
-                                   const Tensor& stats, int64_t want, at::ScalarType shift_type, at::ScalarType bias_type) {
+                                   const Tensor& stats, int64_t want, std::optional<at::ScalarType> shift_type, at::ScalarType bias_type) {
   const Tensor w = or_none(weight), b = or_none(bias), s = or_none(scale);
   same_device(x_, {dy_, w, b, s, stats});
   check_float({&x_, &dy_});
@@ -107,8 +108,9 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Op
   check_param("bias", b, x_, {C});
   check_param("scale", s, x_, {x_.size(0), C});
   TORCH_CHECK(s.defined() || !(want & 4), "llsa_b200.layer_norm_bwd: scale is missing");
+  TORCH_CHECK(shift_type || !(want & 8), "llsa_b200.layer_norm_bwd: shift's type is missing");
   const c10::cuda::CUDAGuard guard(x_.device());
-  const at::ScalarType types[4] = {w.defined() ? w.scalar_type() : at::kFloat, bias_type, s.defined() ? s.scalar_type() : at::kFloat, shift_type};
+  const at::ScalarType types[4] = {w.defined() ? w.scalar_type() : at::kFloat, bias_type, s.defined() ? s.scalar_type() : at::kFloat, shift_type.value_or(at::kFloat)};
   const bool empty = x_.numel() == 0;
   Tensor dx = at::empty(x_.sizes(), x_.options());
   std::vector<Tensor> out = {dx};
@@ -123,15 +125,18 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Op
       gp[i] = &gd[i];
     }
   if (empty) return out;
-  // all rows in one where nothing is per sample
-  const bool per_sample = s.defined() || (want & 8);
+  // All rows in one where nothing is per sample: by what the forward had, not by what is asked for, so that a gradient's sums are over the same parts, and its
+  // bits the same, whichever others are asked for.  The library goes by samples for a scale or a gradient of the shift: one that nobody asked for goes to scratch.
+  // dx alone depends on neither, where its rows are those of one matrix.
+  const bool per_sample = s.defined() || shift_type;
+  auto one_matrix = [](const Tensor& t) { return t.size(0) == 1 || (t.size(1) > 1 && t.stride(0) == t.size(1) * t.stride(1)); };
   auto view = [&](const Tensor& t) { return per_sample ? samples(t) : t.reshape({1, -1, C}); };
   const Tensor x = view(unit_columns(x_)), dy = view(unit_columns(dy_)), dx3 = view(dx);
   TORCH_CHECK(stats.is_contiguous() && stats.numel() == x.size(0) * x.size(1) * 2 && stats.scalar_type() == at::kFloat,
               "llsa_b200.layer_norm_bwd: `stats` is not from the matching layer_norm_fwd");
   const LlsaTensor xd = desc(x), dyd = desc(dy), dxd = desc(dx3), st = packed(stats.data_ptr(), LLSA_F32, {x.size(0), x.size(1), 2});
   const Tensor p[3] = {w, b, s};
-  Tensor keep[3], partial;
+  Tensor keep[3], partial, unasked;
   LlsaTensor pd[3];
   const LlsaTensor* pp[3] = {};
   for (int i = 0; i < 3; ++i)
@@ -140,12 +145,18 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Op
       pd[i] = desc(keep[i]);
       pp[i] = &pd[i];
     }
-  if (want) {
+  if (per_sample && !s.defined() && !(want & 8) && (want || !one_matrix(x) || !one_matrix(dy))) {
+    unasked = at::empty({x.size(0), C}, x.options().dtype(at::kFloat));
+    gd[3] = desc(unasked);
+    gp[3] = &gd[3];
+  }
+  const bool sums = want || unasked.defined();
+  if (sums) {
     partial = at::empty({llsa_layer_norm_bwd_partial_elems(x.size(0), x.size(1), C, per_sample)}, x.options().dtype(at::kFloat));
     part = desc(partial);
   }
   mark("layer_norm_bwd");
-  ok(llsa_layer_norm_bwd(&dyd, &xd, pp[0], pp[1], pp[2], &st, &dxd, gp[0], gp[1], gp[2], gp[3], want ? &part : nullptr,
+  ok(llsa_layer_norm_bwd(&dyd, &xd, pp[0], pp[1], pp[2], &st, &dxd, gp[0], gp[1], gp[2], gp[3], sums ? &part : nullptr,
                          at::cuda::getCurrentCUDAStream(x.device().index())),
      "layer_norm_bwd");
   mark("end");
@@ -364,8 +375,8 @@ const c10::TypedOperatorHandle<Sig>& op(const char* name) {      // once per sig
   return handle;
 }
 using NormFwd = std::vector<Tensor>(const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, double, bool);
-using NormBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Tensor&, int64_t, at::ScalarType,
-                                    at::ScalarType);
+using NormBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const Tensor&, int64_t,
+                                    std::optional<at::ScalarType>, at::ScalarType);
 using LinearFwd = std::vector<Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, int64_t, bool, bool);
 using LinearBwd = std::vector<Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
                                       const OptTensor&, int64_t, int64_t);
@@ -409,7 +420,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     int64_t want = 0;
     for (int i = 0; i < 4; ++i)
       if (e.wants(i < 3 ? s[1 + i] : shift)) want |= 1 << i;
-    const auto shift_type = (at::ScalarType) ctx->saved_data["shift_type"].toInt();
+    std::optional<at::ScalarType> shift_type;
+    if (shift.defined()) shift_type = (at::ScalarType) ctx->saved_data["shift_type"].toInt();
     const auto bias_type = s[2].defined() ? s[2].scalar_type() : at::kFloat;
     const std::vector<Tensor> r =
         below_unless_recorded([&] { return norm_bwd_op().call(grads[0], s[0], opt(s[1]), opt(s[2]), opt(s[3]), s[4], want, shift_type, bias_type); });
@@ -515,7 +527,7 @@ Tensor rope_axes_autograd(const Tensor& x, const Tensor& positions, at::IntArray
 
 TORCH_LIBRARY_FRAGMENT(llsa_b200, m) {
   m.def("layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, float eps, bool want_stats) -> Tensor[]");
-  m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor stats, int want, ScalarType shift_type, "
+  m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor stats, int want, ScalarType? shift_type, "
         "ScalarType bias_type) -> Tensor[]");
   m.def("linear_fwd(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, Tensor? gate, int activation, bool want_pre, bool want_copies) -> "
         "Tensor[]");

@@ -171,6 +171,26 @@ def test_layer_norm_keeps_a_bad_row_to_itself():
     assert torch.equal(llsa_b200.layer_norm(far, eps=0.0).abs(), torch.ones(1, 1, 64, device=DEV))      # a large common offset cancels nothing
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("layout", ["dense", "gaps", "upstream with gaps", "one token"])
+@pytest.mark.parametrize("given", ["t", "wbt", "wb", "wbst", "s"])
+def test_layer_norm_gradients_have_the_same_bits_whichever_are_asked_for(given, layout, dtype):
+    B, N, C = (9, 1, 130) if layout == "one token" else (3, 777, 130)
+    g = gen(17)
+    make = lambda gaps: normal(g, B, N + 2, C + 3, dtype=dtype)[:, 1:-1, 2:-1] if gaps else normal(g, B, N, C, dtype=dtype)
+    data = dict(x=make(layout in ("gaps", "one token")), w=normal(g, C, dtype=dtype, std=0.2, mean=1), b=normal(g, C, dtype=dtype), s=normal(g, B, C, dtype=dtype, std=0.3),
+                t=normal(g, B, C, dtype=dtype))
+    dy = make("gaps" in layout)
+    names = ["x"] + [k for k in "wbst" if k in given]
+    full = {}
+    for mask in reversed(range(1, 1 << len(names))):              # all of them first
+        wanted = [k for i, k in enumerate(names) if mask >> i & 1]
+        v = {k: data[k].detach().requires_grad_(k in wanted) for k in names}
+        y = llsa_b200.layer_norm(v["x"], v.get("w"), v.get("b"), 1e-5, scale=v.get("s"), shift=v.get("t"))
+        for k, d in zip(wanted, torch.autograd.grad(y, [v[k] for k in wanted], dy)):
+            assert torch.equal(full.setdefault(k, d), d), (wanted, k)
+
+
 # ------------------------------------------------------------------------------------------------------ projection
 def act64(z, act):
     """The activation and its slope."""
