@@ -431,6 +431,14 @@ product_tc_kernel(const __grid_constant__ ProductMaps maps, const __grid_constan
               float v[32];
               tc::tmem_ld_16x64(src + ((uint32_t) h << 16), v);
               if (h) accumulator_read();                       // a tile has one chunk for this warpgroup
+              if (i0 + kBM > M) {                              // rows that are not there: zeros times an infinite weight are no numbers, which the sums would keep
+                const int lo = i0 + (warp & 3) * 32 + h + (lane >> 2);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  if (lo >= M) v[4 * j] = v[4 * j + 1] = 0.f;
+                  if (lo + 8 >= M) v[4 * j + 2] = v[4 * j + 3] = 0.f;
+                }
+              }
               // this lane's row of the pieces it addresses: rows 0-7 or 8-15 (lane bit 3) of columns j or j + 1 (bit 4)
               const int pr = (warp & 3) * 32 + h + (lane & 15);
               const uint32_t piece = tc::smem_u32(buf) + pr * 128 + ((pr & 7) << 4);

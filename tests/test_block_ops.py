@@ -679,6 +679,35 @@ def test_a_bad_value_stays_where_the_formula_puts_it():
         assert torch.equal(y, want[0]) and torch.equal(dx, want[1])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M", [9, 128, 200, 256, 300])
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
+def test_an_infinite_weight_keeps_to_the_rows_that_are_there(M, act, dtype):
+    """Rows of a tile behind the last one have no product, not 0 times infinity: far out an activation's slope is 1 or 0, and so is that of an infinite z."""
+    g = gen(72)
+    x, w, b, dy = normal(g, M, 64, dtype=dtype).abs() + 1, normal(g, 72, 64, dtype=dtype, std=0.2), normal(g, 72, dtype=dtype), normal(g, M, 72, dtype=dtype)
+    up, down = [0, 40], [7, 71]
+    others = [f for f in range(72) if f not in up + down]
+
+    def grads(w):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = llsa_b200.linear(*leaves, activation=act)
+        return y.detach(), *torch.autograd.grad(y, leaves[1:], dy)
+
+    _, dw, db = grads(w)
+    w2 = w.clone()
+    w2[up, 3], w2[down, 3] = float("inf"), float("-inf")
+    y2, dw2, db2 = grads(w2)
+    assert torch.equal(dw2[others], dw[others]) and torch.equal(db2[others], db[others])
+    assert (y2[:, up] == float("inf")).all()
+    d64, x64 = dy.double(), x.double()
+    within("db", db2[up], d64[:, up].sum(0), (M + 100) * U * d64[:, up].abs().sum(0))
+    # dz of slope 1 is dy, to a rounding of the slope in fp32 that may take it a half step of dy's type off
+    within("dw", dw2[up], d64[:, up].T @ x64, (2 * M * U + half_step(dtype)) * (d64[:, up].abs().T @ x64))
+    # slope 0: s(-7) of GELU is below 1e-15, s(-30) of SiLU times 30 below 3e-12
+    assert float(db2[down].abs().max()) <= 3e-12 * float(d64.abs().sum(0).max()) and float(dw2[down].abs().max()) <= 3e-12 * float((d64.abs().T @ x64).max())
+
+
 def _long_samples(seed, B=3, N=1030, K=96, F=136):
     g = gen(seed)
     leaves = [normal(g, B, N, K, dtype=BF16), normal(g, F, K, dtype=BF16, std=K ** -0.5), normal(g, F, dtype=BF16, std=0.1), normal(g, B, N, F, dtype=BF16),
