@@ -156,7 +156,7 @@ int llsa_layer_norm_bwd(const LlsaTensor* dy, const LlsaTensor* x, const LlsaTen
  * y = residual + gate_b * act(x weight^T + bias); bf16 or F32 throughout, sums fp32, y rounded once.  Zero-initialise the struct. */
 enum LlsaActivation { LLSA_ACT_NONE = 0, LLSA_ACT_GELU_TANH = 1, LLSA_ACT_SILU = 2 };
 typedef struct LlsaLinearArgs {
-  const LlsaTensor* x;         /* [M,K], fewer than 2^31 rows; bf16: rows on 16-byte boundaries */
+  const LlsaTensor* x;         /* [M,K], fewer than 2^31 rows; bf16: rows on 16-byte boundaries that do not overlap */
   const LlsaTensor* weight;    /* [F,K], likewise */
   const LlsaTensor* bias;      /* [F] contiguous, or NULL */
   const LlsaTensor* residual;  /* [M,F], any row stride, or NULL */
@@ -167,7 +167,7 @@ typedef struct LlsaLinearArgs {
                                   again behind an activation, and do without it for a gate of long samples; both read bias, as in the forward */
   int32_t activation;          /* LlsaActivation */
   /* backward: dy in, those of the others that are not NULL out */
-  const LlsaTensor* dy;        /* [M,F], any row stride; for a gate of long bf16 samples (llsa_linear_keeps_product() is 0) rows on 16-byte boundaries */
+  const LlsaTensor* dy;        /* [M,F], any row stride; for a gate of long bf16 samples (llsa_linear_keeps_product() is 0) rows as those of x */
   const LlsaTensor* dx;        /* [M,K], likewise */
   const LlsaTensor* dweight;   /* [F,K] contiguous, x's type; for such a gate on a 16-byte boundary */
   const LlsaTensor* dbias;     /* [F] contiguous, F32 or x's type */

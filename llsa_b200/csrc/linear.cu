@@ -502,7 +502,10 @@ int check_matrix(const LlsaTensor* t, const char* name, int dtype, int64_t rows,
   return LLSA_OK;
 }
 
-bool rows16(const LlsaTensor* t) { return (uintptr_t) t->ptr % 16 == 0 && (t->shape[0] == 1 || t->stride[0] * (int64_t) dtype_size(t->dtype) % 16 == 0); }
+// Rows on 16-byte boundaries that do not overlap, such as those of one that stands for all: tensor maps are specified for strides that reach past a row
+bool rows16(const LlsaTensor* t) {
+  return (uintptr_t) t->ptr % 16 == 0 && (t->shape[0] == 1 || (t->stride[0] * (int64_t) dtype_size(t->dtype) % 16 == 0 && t->stride[0] >= t->shape[1]));
+}
 
 struct Plan {
   int64_t M, K, F, B, N;       // rows, input and output features, samples (1 without a gate), rows of a sample
@@ -537,7 +540,7 @@ int check_common(const LlsaLinearArgs* a, Plan* p) {
   LLSA_REQUIRE(p->M <= INT32_MAX, LLSA_ERR_SHAPE, "linear: more than 2^31 - 1 rows");
   int rc;
   if ((rc = check_matrix(a->x, "x", p->dtype, p->M, p->K)) || (rc = check_matrix(a->weight, "weight", p->dtype, p->F, p->K))) return rc;
-  if (p->dtype == LLSA_BF16) LLSA_REQUIRE(rows16(a->x) && rows16(a->weight), LLSA_ERR_STRIDE, "linear: rows of x and weight must start on 16-byte boundaries");
+  if (p->dtype == LLSA_BF16) LLSA_REQUIRE(rows16(a->x) && rows16(a->weight), LLSA_ERR_STRIDE, "linear: rows of x and weight must start on 16-byte boundaries, and not overlap");
   LLSA_REQUIRE(a->activation >= kActNone && a->activation <= kActSilu, LLSA_ERR_ARG, "linear: activation %d is not known", a->activation);
   p->B = 1;
   if (a->gate) {
@@ -787,8 +790,8 @@ extern "C" int llsa_linear_bwd(const LlsaLinearArgs* a, void* stream) {
   if (rc) return rc;
   plan_bwd(a, &p);
   if ((rc = check_matrix(a->dy, "dy", p.dtype, p.M, p.F))) return rc;
-  LLSA_REQUIRE(!p.by_sample || rows16(a->dy), LLSA_ERR_STRIDE, "dy: rows must start on 16-byte boundaries for a gate of long samples");
-  LLSA_REQUIRE(!p.by_sample || !a->dx || rows16(a->dx), LLSA_ERR_STRIDE, "dx: rows must start on 16-byte boundaries for a gate of long samples");
+  LLSA_REQUIRE(!p.by_sample || rows16(a->dy), LLSA_ERR_STRIDE, "dy: rows must start on 16-byte boundaries, and not overlap, for a gate of long samples");
+  LLSA_REQUIRE(!p.by_sample || !a->dx || rows16(a->dx), LLSA_ERR_STRIDE, "dx: rows must start on 16-byte boundaries, and not overlap, for a gate of long samples");
   LLSA_REQUIRE(!p.by_sample || !a->dweight || (uintptr_t) a->dweight->ptr % 16 == 0, LLSA_ERR_STRIDE, "dweight: must start on a 16-byte boundary for a gate of long samples");
   LLSA_REQUIRE(p.M == 0 || a->pre || !((a->dgate && !p.by_sample) || (p.dtype == LLSA_F32 && a->activation != kActNone)), LLSA_ERR_NULL, "pre: null tensor");
   if (a->dx && (rc = check_matrix(a->dx, "dx", p.dtype, p.M, p.K))) return rc;

@@ -593,8 +593,9 @@ inline int matrix_map(CUtensorMap* m, const void* base, int64_t ld, int64_t rows
   const uint64_t dims[3] = {(uint64_t) cols, (uint64_t) rows, (uint64_t) samples}, strides[2] = {(uint64_t) ld * 2, (uint64_t) apart * 2};
   return tma::make_map(m, base, samples ? 3 : 2, dims, strides, box_rows);
 }
+// Rows of `cols` on 16-byte boundaries that do not overlap
 template <typename T>
-inline bool rows16(const Mat<T>& m) { return m.p && ((uintptr_t) m.p & 15) == 0 && m.ld % 8 == 0; }
+inline bool rows16(const Mat<T>& m, int64_t cols) { return m.p && ((uintptr_t) m.p & 15) == 0 && m.ld % 8 == 0 && m.ld >= cols; }
 
 template <int BN, bool PAIR, bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES, bool TMA>
 int launch(const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
@@ -607,7 +608,7 @@ int launch(const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status
   if (rc) return rc;
   maps.in = maps.y = maps.a;
   if (KIND != kParts) {
-    out.vec_pre = rows16(out.e.pre);
+    out.vec_pre = rows16(out.e.pre, p.N);
     if (IN && TMA && (rc = matrix_map(&maps.in, out.in.p, out.in.ld, p.M, p.N, kBM, 0, 0))) return rc;
     if (TMA && (rc = matrix_map(&maps.y, out.e.y.p, out.e.y.ld, p.M, p.N, kBM, p.samples, p.M * out.e.y.ld))) return rc;
   }
@@ -642,7 +643,7 @@ int launch_tile(const Choice& c, const Product<bf16>& p, Outputs& out, int wait_
 template <bool A_MN, bool B_MN, int KIND, int ACT, bool IN, bool GATED, int G, bool SAMPLES = false>
 int launch_choice(const Choice& c, const Product<bf16>& p, Outputs& out, int wait_limit, int32_t* status, cudaStream_t st) {
   if constexpr (KIND == kParts || SAMPLES) return launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, true>(c, p, out, wait_limit, status, st);
-  return (!IN || rows16(out.in)) && rows16(out.e.y) ? launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, true>(c, p, out, wait_limit, status, st)
+  return (!IN || rows16(out.in, p.N)) && rows16(out.e.y, p.N) ? launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, true>(c, p, out, wait_limit, status, st)
                                                     : launch_tile<A_MN, B_MN, KIND, ACT, IN, GATED, G, SAMPLES, false>(c, p, out, wait_limit, status, st);
 }
 // A forward with a long epilogue: by the length of its sums

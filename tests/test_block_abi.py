@@ -96,6 +96,22 @@ def test_linear_backward_wants_its_workspace():
     assert lib.llsa_linear_bwd_workspace_bytes(ref(bad)) == -1 and lib.llsa_linear_keeps_product(ref(bad)) == -1
 
 
+@pytest.mark.parametrize("change", [dict(x=fake((64, 32), strides=(0, 1))), dict(x=fake((64, 32), strides=(16, 1))), dict(weight=fake((48, 32), strides=(0, 1))),
+                                    dict(weight=fake((48, 32), strides=(24, 1)))])
+def test_linear_refuses_rows_that_overlap(change):
+    """bf16 operands of the products: tensor maps are specified for strides that reach past a row.  One row has no stride."""
+    lib = _lib.lib()
+    a, keep = linear_args(**change)
+    assert lib.llsa_linear_fwd(ref(a), None) == ERR_STRIDE and b"overlap" in lib.llsa_last_error_string()
+    assert lib.llsa_linear_keeps_product(ref(a)) == -1 and lib.llsa_linear_bwd_workspace_bytes(ref(a)) == -1
+    a, keep = linear_args(M=1, x=fake((1, 32), strides=(0, 1)))
+    assert lib.llsa_linear_keeps_product(ref(a)) == 0
+    long = dict(x=fake((1024, 32)), dy=fake((1024, 48), strides=(0, 1)), gate=fake((2, 48)), dx=fake((1024, 32)))      # a gate of long samples
+    a, keep = linear_args(M=1024, y=None, **long)
+    a.workspace, a.workspace_bytes = 0x100000, max(0, lib.llsa_linear_bwd_workspace_bytes(ref(a)))
+    assert lib.llsa_linear_bwd(ref(a), None) == ERR_STRIDE and b"dy" in lib.llsa_last_error_string()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("act,gated", [(0, False), (1, False), (2, False), (0, True)])
 def test_linear_backward_without_rows_wants_no_workspace(dtype, act, gated):

@@ -909,6 +909,45 @@ def test_outputs_of_the_c_entries_leave_their_surroundings_alone():
                 assert bool((big == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act,gated", [(0, False), (1, False), (0, True)])
+def test_c_entries_take_a_residual_and_an_upstream_gradient_of_rows_that_overlap(dtype, act, gated):
+    """One row for all, and a window that moves by eight: the bits of the same rows written out."""
+    import ctypes as C
+    from llsa_b200 import _lib
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    M, K, F = 300, 64, 72
+    g = gen(19)
+    x, w, gate, line = normal(g, M, K, dtype=dtype), normal(g, F, K, dtype=dtype, std=0.1), normal(g, 3, F, dtype=dtype), normal(g, 8 * M + F, dtype=dtype)
+
+    def call(rows):
+        d = dict(x=x, weight=w, residual=rows, y=torch.empty(M, F, device=DEV, dtype=dtype), dy=rows, dx=torch.empty(M, K, device=DEV, dtype=dtype),
+                 dweight=torch.empty(F, K, device=DEV, dtype=dtype), dbias=torch.empty(F, device=DEV, dtype=dtype))
+        if gated:
+            d.update(gate=gate, pre=torch.empty(M, F, device=DEV, dtype=dtype), dgate=torch.empty(3, F, device=DEV, dtype=dtype))
+        elif act and dtype == F32:
+            d.update(pre=torch.empty(M, F, device=DEV, dtype=dtype))
+        a, keep = _lib.LlsaLinearArgs(), {k: _lib.desc(t) for k, t in d.items()}
+        for k in keep:
+            setattr(a, k, C.pointer(keep[k]))
+        a.activation = act
+        assert lib.llsa_linear_fwd(C.byref(a), stream) == 0, lib.llsa_last_error_string()
+        ws = torch.empty(max(1, lib.llsa_linear_bwd_workspace_bytes(C.byref(a))) + 256, device=DEV, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = (ws.data_ptr() + 255) // 256 * 256, ws.numel() - 256
+        assert lib.llsa_linear_bwd(C.byref(a), stream) == 0, lib.llsa_last_error_string()
+        torch.cuda.synchronize()
+        return [d[k] for k in ("y", "dx", "dweight", "dbias") + (("dgate",) if gated else ())]
+
+    for step in (0, 8):
+        rows = line.as_strided((M, F), (step, 1))
+        for k, p, q in zip(("y", "dx", "dweight", "dbias", "dgate"), call(rows), call(rows.contiguous())):
+            if k in ("dbias", "dgate"):                          # a thread owns one column or eight neighbours: the same terms, below `most`, in another order, rounded on either side
+                most = float(rows.abs().max()) * max(1.13, float(gate.abs().max()), float((x.float().abs() @ w.float().abs().T).max()))
+                assert bool(((p.double() - q.double()).abs() <= 2.02 * half_step(dtype) * q.double().abs() + 2 * (M + 100) * U * M * most).all()), k
+            else:
+                assert torch.equal(p, q), k
+
+
 # ------------------------------------------------------------------------------------------------------ the model
 @pytest.mark.parametrize("attn,fused_rope,side", [("sparse_l2", True, 128), ("sparse_l1", False, 32), ("pixel", True, 16)])
 def test_model_on_the_fused_block_agrees_with_the_eager_block(attn, fused_rope, side):
