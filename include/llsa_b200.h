@@ -17,7 +17,9 @@
  *   - tensors are described by LlsaTensor: up to 4 dims, strides in ELEMENTS.
  *     Attention tensors are [B,H,N,D] with stride[3]==1 and 16-byte aligned
  *     rows; any batch/head/token strides are accepted (the model passes
- *     [B,H,N,D] views of [B,N,H,D] storage).
+ *     [B,H,N,D] views of [B,N,H,D] storage).  A tensor that is to be
+ *     `contiguous` also begins on a 16-byte boundary, or the call is refused
+ *     with LLSA_ERR_STRIDE; only 1-D scratch of partial sums need not.
  */
 #ifndef LLSA_B200_H_
 #define LLSA_B200_H_

@@ -84,6 +84,25 @@ def test_linear_backward_refuses(code, change):
     assert lib.llsa_linear_bwd(ref(a), None) == code, lib.llsa_last_error_string()
 
 
+@pytest.mark.parametrize("dtype,act,gated", [(F32, 1, False), (F32, 0, True), (BF16, 0, True)])
+def test_linear_refuses_a_kept_product_off_its_boundary(dtype, act, gated):
+    """The pass over dy reads 16 bytes of dy and of the kept product at once: `contiguous` includes a base on a 16-byte boundary, in either direction."""
+    lib = _lib.lib()
+    step = 4 if dtype == F32 else 2
+    mk = lambda *shape, **k: fake(shape, dtype, **k)
+    for off, code in ((step, ERR_STRIDE), (8, ERR_STRIDE), (16 - step, ERR_STRIDE)):
+        given = dict(x=mk(64, 32), weight=mk(48, 32), pre=mk(64, 48, ptr=0x10000 + off))
+        if gated:
+            given.update(gate=mk(2, 48), residual=mk(64, 48))
+        a, keep = linear_args(dtype=dtype, act=act, **given)
+        assert lib.llsa_linear_fwd(ref(a), None) == code and b"pre" in lib.llsa_last_error_string()
+        given.update(y=None, residual=None, dy=mk(64, 48), dx=mk(64, 32))
+        a, keep = linear_args(dtype=dtype, act=act, **given)
+        a.workspace, a.workspace_bytes = 0x100000, 1 << 30
+        assert lib.llsa_linear_bwd_workspace_bytes(ref(a)) == -1
+        assert lib.llsa_linear_bwd(ref(a), None) == code and b"pre" in lib.llsa_last_error_string()
+
+
 def test_linear_backward_wants_its_workspace():
     lib = _lib.lib()
     a, keep = linear_args(y=None, dy=fake((64, 48)), dx=fake((64, 32)), dweight=fake((48, 32)), dbias=fake((48,)), act=1)
