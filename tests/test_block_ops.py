@@ -324,6 +324,39 @@ def test_linear_strides_ranks_and_partial_gradients(dtype):
     check_linear(t, torch.ones(4, 21, F, device=DEV, dtype=dtype), None, llsa_b200.linear(x, w), dict(x=d, w=linear_reference(x, w, None, None, None, None, torch.ones(4, 21, F, device=DEV))["w"]), dtype)
 
 
+@pytest.mark.parametrize("act", ["gelu_tanh", "silu"])
+@pytest.mark.parametrize("M,K,F,std", [(300, 64, 96, 1.0), (2000, 384, 200, 1.0), (131, 1536, 72, 3.0), (4100, 128, 200, 0.2)])
+def test_slope_of_bf16_data_is_taken_from_an_fp32_product(M, K, F, std, act):
+    """z is computed again and not rounded, and the bias' gradient is the sum of an unrounded dz: read in fp32 over the C ABI, it is off by fp32 roundings alone.
+
+    The logistic s of u(z): its argument, 4 roundings, moves it by s (1 - s) |u| 4 u <= 0.9 u; 2^t is off by 2^-22 of itself, 1/4 * 4 u = 1 u; the reciprocal shared by a pair, its
+    two factors and what they are made of 6 u: 8 u in all.  The slope s + z s (1 - s) u' moves by at most 1 + |z| u' for each of s, and has 8 roundings of its own."""
+    import ctypes as C
+    from llsa_b200 import _lib
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    g = gen(M + K)
+    x, w, b, dy = normal(g, M, K, dtype=BF16), normal(g, F, K, dtype=BF16, std=std * K ** -0.5), normal(g, F, dtype=BF16, std=0.3), normal(g, M, F, dtype=BF16)
+    d = dict(x=x, weight=w, bias=b, dy=dy, dx=torch.empty_like(x), dweight=torch.empty_like(w), dbias=torch.empty(F, device=DEV))
+    a, keep = _lib.LlsaLinearArgs(), {k: _lib.desc(t) for k, t in d.items()}
+    for k in keep:
+        setattr(a, k, C.pointer(keep[k]))
+    a.activation = 1 if act == "gelu_tanh" else 2
+    ws = torch.empty(lib.llsa_linear_bwd_workspace_bytes(C.byref(a)) + 256, device=DEV, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = (ws.data_ptr() + 255) // 256 * 256, ws.numel() - 256
+    assert lib.llsa_linear_bwd(C.byref(a), stream) == 0, lib.llsa_last_error_string()
+    ref = linear_reference(x, w, b, act, None, None, dy)
+    z, ez = ref["z"].abs(), (2 * K + 4) * U * ref["zb"]
+    # beyond 7 (SiLU: 30) the kernel's slope stays what it is there, which is within 1e-11 of 1 or 0
+    far, rise = (7.0, 2 * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z.clamp(max=7.0) ** 2)) if act == "gelu_tanh" else (30.0, 1.0)
+    edz = (1.6 * ez + 8 * U * (2 + z.clamp(max=far) * rise) + 1e-11) * dy.double().abs()
+    within("db", d["dbias"], ref["b"], edz.sum(0) + (M + 100) * U * ref["bb"])
+    hs = half_step(BF16)
+    edz = edz + 1.01 * hs * (ref["dz"].abs() + edz)              # in front of the two products dz is rounded
+    wd, xd = w.double().abs(), x.double().abs()
+    within("dx", d["dx"], ref["x"], edz @ wd + (2 * F + 4) * U * (ref["xb"] + edz @ wd))
+    within("dw", d["dweight"], ref["w"], edz.T @ xd + (2 * M + 400) * U * (ref["wb"] + edz.T @ xd))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_linear_far_values(dtype):
     """Activations far out on either side, a zero gate, and rows that are not numbers."""
@@ -717,6 +750,27 @@ def _long_samples(seed, B=3, N=1030, K=96, F=136):
 
 def _gated(x, w, b, r, gate):
     return llsa_b200.linear(x, w, b, residual=r, gate=gate)
+
+
+@pytest.mark.parametrize("B,N,K,F", [(3, 1030, 96, 136), (1, 4096, 64, 72), (5, 520, 256, 64)])
+def test_gradient_of_a_gate_of_long_samples_does_without_the_product(B, N, K, F):
+    """No z is kept and rounded: dgate in fp32 over the C ABI is a sum over the features of sums over the rows, 2 N + 2 K roundings deep and some 100 of their joining."""
+    import ctypes as C
+    from llsa_b200 import _lib
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    (x, w, b, r, gate), dy = _long_samples(83, B, N, K, F)
+    x, w, b, gate = [t.detach() for t in (x, w, b, gate)]
+    d = dict(x=x.view(B * N, K), weight=w, bias=b, gate=gate, dy=dy.view(B * N, F), dgate=torch.empty(B, F, device=DEV), dbias=torch.empty(F, device=DEV))
+    a, keep = _lib.LlsaLinearArgs(), {k: _lib.desc(t) for k, t in d.items()}
+    for k in keep:
+        setattr(a, k, C.pointer(keep[k]))
+    assert lib.llsa_linear_keeps_product(C.byref(a)) == 0
+    ws = torch.empty(lib.llsa_linear_bwd_workspace_bytes(C.byref(a)) + 256, device=DEV, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = (ws.data_ptr() + 255) // 256 * 256, ws.numel() - 256
+    assert lib.llsa_linear_bwd(C.byref(a), stream) == 0, lib.llsa_last_error_string()
+    ref = linear_reference(x, w, b, None, None, gate, dy)
+    within("dgate", d["dgate"], ref["g"], (2 * N + 2 * K + 100) * U * ref["gb"])
+    within("db", d["dbias"], ref["b"], (B * N + 100) * U * ref["bb"])
 
 
 def test_gate_of_long_samples_in_parts_in_graphs_and_traced():
