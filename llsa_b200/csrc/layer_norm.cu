@@ -399,7 +399,9 @@ Split split_of(int64_t C, bool whole, bool alike, bool fwd) {
   s.r = (int) ((span + vec * 32 * s.warps - 1) / (vec * 32 * s.warps));
   // rows a multiple of four apart begin alike: four groups at least
   s.threads = s.form == kShifted && s.warps == 4 ? 512 : 256;
-  // forward: two warps with 20 values a thread have two CTAs to an SM (3 x 5377 rows of 1155: fp32 32.5 us, four warps of 512 threads 43; bf16 29.6 and 46)
+  // forward: two warps, with 20 values a thread, have two CTAs to an SM where four warps of 512 threads have one.  They hold up to 1277 channels behind the boundary.
+  // us, two warps / four, 16384 rows in fp32, 32768 in bf16: 1029 channels 30.8 / 41.2, 60.9 / 98.7; 1155 32.0 / 41.0, 59.5 / 93.6; 1277 33.6 / 41.0, 60.4 / 95.0; four
+  // warps take 41.2 and 93.8 for 1281, which two do not hold.  (Backward: bf16 63 / 69, fp32 78 / 56 at 3 x 5377 x 1155.)
   if (fwd && s.threads == 512 && span <= 1280) {
     s.warps = 2;
     s.r = 5;

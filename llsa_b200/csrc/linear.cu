@@ -362,7 +362,8 @@ int sum_parts(const float* partial, int64_t ld, int split, bool turned, int64_t 
 // ------------------------------------------------------------------------------------------------ a gate by samples
 // Of long samples the gate is applied to what is small instead of to dy.  With G_b = dy_b^T x_b (the parts of dw, taken sample by sample) and S_b = sum_n dy:
 //   dx_b = dy_b (gate_b w),   dw = sum_b gate_b G_b,   dgate_b = rowsum(w G_b) + bias S_b,   dbias = sum_b gate_b S_b
-// so that the product of the forward is not kept, dz is neither written nor rounded, and what passes through memory for it is B weights and parts.
+// so that the product of the forward is not kept, dz is neither written nor rounded, and what passes through memory for it is B weights and parts.  gate_b w is
+// rounded to bf16, as the tensor cores take their operands: a half step in dx beside the one of dx itself, where a rounded dz would put it into dx and dw.
 // us, 131072 rows in 8 samples, 1536 -> 384, forward and backward: 490 with z kept and dz written, 465 so.
 __global__ void __launch_bounds__(256)
 gated_weight_kernel(Mat<const bf16> w, Mat<const bf16> gate, bf16* __restrict__ out, int F, int K) {      // out [B][F][K]; K a multiple of 8
@@ -522,8 +523,11 @@ struct Plan {
   size_t o_dz, o_cols, o_parts, o_wg, o_pg, bytes;
 };
 
-// Long samples: twice as many rows as input features, what the B weights and parts cost beside z and dz; rows on 16-byte boundaries throughout;
-// samples that a grid's second dimension takes
+// Long samples: twice as many rows as input features, where the B weights and parts hold no more bytes than z and dz; rows on 16-byte boundaries throughout;
+// samples that a grid's second dimension takes.  us, forward and backward in a graph, so / with z kept: samples x rows, features: 8 x 16384, 1536 -> 384 461 / 488;
+// 8 x 4096, 384 -> 1536 171 / 233; 64 x 1024, 64 -> 512 148 / 152; 4 x 2048, 1024 -> 1024 84 to 91 / 84; beside the line 16 x 512, 256 -> 1024 68 / 66; 2 x 1024,
+// 256 -> 256 26 to 29 / 27.  Of many samples the parts of a narrow dw are added by few CTAs, one pair of samples after another (gated_parts_kernel), and z kept would be
+// the faster way: 32 x 1024, 384 -> 384 98 / 90; 64 x 512, 256 -> 1024 203 / 169; 256 x 512, 256 -> 256 389 / 204; 1024 x 512, 64 -> 64 1003 / 227.
 bool by_sample(const LlsaLinearArgs* a, const Plan& p) {
   return p.dtype == LLSA_BF16 && a->gate && p.N >= 512 && p.N >= 2 * p.K && p.K % 8 == 0 && p.F % 8 == 0 && p.B <= 65535;
 }

@@ -14,7 +14,8 @@ struct Mat {
   int64_t ld;
 };
 
-// What stands behind the product z of a forward: y = residual + gate act(z + bias); `pre`, if given, keeps z + bias for the backward.
+// What stands behind the product z of a forward: y = residual + gate act(z + bias); `pre`, if given, keeps z + bias for the backward (in the data's type, as it is as
+// large as y: a half step of each term of the gate's gradient).
 template <typename T>
 struct Epilogue {
   const T* bias;

@@ -2,7 +2,9 @@
 //
 //   forward   A = x, B = w, both along k in memory:  y = residual + gate act(D + bias)
 //   slope     the same product again:                dz = dy act'(D + bias), and its column sums.  z is not kept between the passes: that would cost 4 bytes a
-//             value of memory traffic and 2 of storage (123 us and 400 MB at 131072 x 1536), and z would be rounded
+//             value of memory traffic and 2 of storage (123 us and 400 MB at 131072 x 1536), and z would be rounded.  dz is rounded to bf16, which is how the
+//             tensor cores take it in the next two products (a half step of each term: dx and dw are 2.35e-3 off in the norm where one rounding leaves
+//             1.66e-3); its column sums take it unrounded
 //   forward   A = dz, B = w taken across:            dx
 //   parts     A = dz, B = x, both taken across:      dw, in parts of the sum over the tokens, which a second kernel adds in order
 //
